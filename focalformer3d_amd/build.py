@@ -23,7 +23,10 @@ OBJ_DIR = os.path.join(LIB_DIR, 'obj_exp' if _EXP else 'obj')
 LIB_PATH = os.path.join(LIB_DIR, 'libff3d_hip_exp.so' if _EXP else 'libff3d_hip.so')
 SOURCES = sorted(glob.glob(os.path.join(PKG, 'csrc', '*.hip')))
 HEADERS = sorted(glob.glob(os.path.join(PKG, 'csrc', '*.h'))) + [os.path.join(ROOT, 'include', 'ff3d.h')]
-CFLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-I' + os.path.join(ROOT, 'include')]
+# packed fp32 instructions are off: some of their forms have given wrong results on these cards (the host pass warns that it does not
+# know the feature)
+CFLAGS = ['--offload-arch=gfx950', '-O3', '-std=c++17', '-fPIC', '-Xclang', '-target-feature', '-Xclang', '-packed-fp32-ops',
+          '-I' + os.path.join(ROOT, 'include')]
 # FF3D_BUILD_EXPERIMENTS=1: also compile the measured-slower kernel variants and timing ablations that round 1-4's A/B
 # records in profiles/ came from (hand-scheduled / 8 x 64 halo convs, 192-column and periodic weight-stationary GEMMs,
 # FF3D_HALO_ABLATE / FF3D_WS_ABLATE instances).  The shipped library does not carry them.
