@@ -104,6 +104,12 @@ SIGNATURES = {
     'ff3d_lss_cells': (_i, [_vp] * 9 + [_i] * 5 + [_vp] * 5),
     'ff3d_lss_splat': (_i, [_vp, _i64, _vp, _i, _vp, _vp, _vp, _i, _i, _vp]),
     'ff3d_nchw_to_nhwc': (_i, [_vp, _vp, _i, _i, _i, _vp]),
+    'ff3d_gated_linear_workspace_bytes': (_i64, [_i] * 6),
+    'ff3d_gated_linear_fwd': (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    'ff3d_gated_linear_bwd': (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    'ff3d_grad_norm_workspace_bytes': (_i64, [_vp, _i]),
+    'ff3d_grad_norm': (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
+    'ff3d_clip_grads': (_i, [_vp] * 5 + [_i, _i, _f, _vp, _vp, _vp]),
     'ff3d_cam_sample': (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp]),
 }
 

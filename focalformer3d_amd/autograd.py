@@ -171,6 +171,28 @@ class MaskedSelfAttentionFunction(Function):
         return gq, gk, gv, None, None, None
 
 
+class GatedLinearFunction(Function):
+    """``h = act(x Wg^T + bg) * (x Wu^T + bu)`` (ops.gated_linear); backward = ops.gated_linear_bwd, which recomputes both projections:
+    only the inputs are saved."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, act):
+        ctx.save_for_backward(x, weight, bias)
+        ctx.act = act
+        return ops.gated_linear(x, weight, bias, act)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dh):
+        x, weight, bias = ctx.saved_tensors
+        return (*ops.gated_linear_bwd(x, weight, bias, ctx.act, dh, ctx.needs_input_grad[:3]), None)
+
+
+def gated_linear(x, weight, bias=None, act='silu'):
+    """Differentiable ``ops.gated_linear``: x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F) or None, one type of fp32, bf16, fp16."""
+    return GatedLinearFunction.apply(x, weight, bias, act)
+
+
 class SimilarFunction(Function):
     """``similarFunction`` (encoder_utils.py:61-83) over libff3d_hip.so: forward = locatt_ops similar_forward (cc2k), backward =
     similar_backward(is_ori=True / False) = ck2c_ori / ck2c_loc (ff3d.h)."""

@@ -1,0 +1,131 @@
+// 32 x 32 matrix-core tiles in bf16, fp16 and fp32 for the kernels that take all three types.
+//
+// One step multiplies 32 x 16 by 16 x 32.  A lane l holds 8 elements of each operand, element e being
+//   A[l % 32][8 * (l / 32) + e]   and   B[8 * (l / 32) + e][l % 32],
+// in every type: 16-bit types feed them to one v_mfma_f32_32x32x16, fp32 feeds element e of all lanes to the e-th of eight
+// v_mfma_f32_32x32x2 (which pairs the k = e of the lower half with the k = 8 + e of the upper).  The order of k inside a step
+// is free as long as both operands agree, which the callers use: the accumulator layout
+//   reg r of lane l  =  C[8 * (r / 4) + 4 * (l / 32) + r % 4][l % 32]
+// read as the operand of a following product has element e of step s = reg 8 s + e, i.e. k = 16 s + 8 (e / 4) + 4 (l / 32) + e % 4
+// (col_frag_acc below): a score tile becomes the next operand without leaving its lanes.
+#pragma once
+#include "ff3d_common.h"
+
+namespace mma {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Type {
+  typedef T vec8 __attribute__((ext_vector_type(8)));
+  static constexpr int PER16 = 16 / sizeof(T);     // elements in a 16-byte granule
+};
+template <typename T>
+using vec8 = typename Type<T>::vec8;
+
+__device__ __forceinline__ f32x16 mfma16(vec8<__bf16> a, vec8<__bf16> b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma16(vec8<_Float16> a, vec8<_Float16> b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma16(vec8<float> a, vec8<float> b, f32x16 c) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+  return c;
+}
+
+__device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v) { return (float)v; }
+template <typename T>
+__device__ __forceinline__ T from_f(float v) { return (T)v; }      // round to nearest even
+
+// ---- LDS tiles -----------------------------------------------------------------------------------------------------------
+// A tile is a number of rows of GR 16-byte granules.  Two kinds of reads: along a row (the rows are rows of the operand, k runs along
+// them; the 8 lanes that one access serves together read granule g of 8 consecutive rows) and down the columns (k runs over the
+// rows; ds_read_b64_tr_b16 hands each lane of a group of 16 the 4 elements of its column from a 4 x 16 block, lane 4 i + j of the
+// group addressing row i, columns 4 j .. 4 j + 3).  Granule g of row r lies at granule place(r, g) of the row, so that the 8 rows of
+// the first kind and the 4 rows x 2 granules of the second fall on different banks; tiles that are only read down their columns
+// (COL) keep two neighbouring groups of 16 apart as well.
+template <int GR, bool COL = false>
+__device__ __forceinline__ int place(int r, int g) {
+  if constexpr (COL && GR >= 16) return g ^ ((r & 3) << 2);
+  else if constexpr (GR >= 8) return g ^ (((r & 3) << 1) | ((r >> 2) & 1));
+  else if constexpr (GR == 4) return g ^ ((((r >> 1) & 1) << 1) | ((r >> 2) & 1));
+  else if constexpr (GR == 2) return g ^ ((r >> 2) & 1);
+  else return g;
+}
+
+// elements k0 + 8 half .. + 7 of a row (k0 a multiple of 16)
+template <typename T, int GR>
+__device__ __forceinline__ vec8<T> row_frag(const char* tile, int row, int k0, int half) {
+  vec8<T> v;
+  if constexpr (sizeof(T) == 2) {
+    v = *(const vec8<T>*)(tile + (row * GR + place<GR>(row, k0 / 8 + half)) * 16);
+  } else {
+    const int g = k0 / 4 + 2 * half;
+    *(u32x4*)&v = *(const u32x4*)(tile + (row * GR + place<GR>(row, g)) * 16);
+    *((u32x4*)&v + 1) = *(const u32x4*)(tile + (row * GR + place<GR>(row, g + 1)) * 16);
+  }
+  return v;
+}
+
+// column col0 + lane % 32 (col0 a multiple of 32): elements 0..3 = rows k_lo .. k_lo + 3, 4..7 = rows k_hi .. k_hi + 3 (multiples of 4)
+template <typename T, int GR, bool COL>
+__device__ __forceinline__ vec8<T> col_frag_at(const char* tile, int k_lo, int k_hi, int col0, int lane) {
+  vec8<T> v;
+  if constexpr (sizeof(T) == 2) {
+    typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+    const int i = (lane & 15) >> 2, c = col0 + (lane & 16) + 4 * (lane & 3);
+    const int g = c >> 3, in = (c & 7) * 2, r0 = k_lo + i, r1 = k_hi + i;
+    *(s16x4*)&v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (r0 * GR + place<GR, COL>(r0, g)) * 16 + in));
+    *((s16x4*)&v + 1) = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(tile + (r1 * GR + place<GR, COL>(r1, g)) * 16 + in));
+  } else {
+    const int c = col0 + (lane & 31), g = c >> 2, in = (c & 3) * 4;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = *(const T*)(tile + ((k_lo + e) * GR + place<GR, COL>(k_lo + e, g)) * 16 + in);
+      v[4 + e] = *(const T*)(tile + ((k_hi + e) * GR + place<GR, COL>(k_hi + e, g)) * 16 + in);
+    }
+  }
+  return v;
+}
+// rows k0 .. k0 + 15 in their plain order: k = k0 + 8 half + e
+template <typename T, int GR, bool COL>
+__device__ __forceinline__ vec8<T> col_frag(const char* tile, int k0, int col0, int lane) {
+  const int k = k0 + 8 * (lane >> 5);
+  return col_frag_at<T, GR, COL>(tile, k, k + 4, col0, lane);
+}
+// in the accumulator's order: k = k0 + 8 (e / 4) + 4 half + e % 4
+template <typename T, int GR, bool COL>
+__device__ __forceinline__ vec8<T> col_frag_acc(const char* tile, int k0, int col0, int lane) {
+  const int k = k0 + 4 * (lane >> 5);
+  return col_frag_at<T, GR, COL>(tile, k, k + 8, col0, lane);
+}
+// accumulator registers 8 step .. 8 step + 7 (rows 16 step .. 16 step + 15) as the operand that col_frag_acc's k order goes with
+template <typename T>
+__device__ __forceinline__ vec8<T> acc_frag(const f32x16& c, int step) {
+  vec8<T> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = from_f<T>(c[8 * step + e]);
+  return v;
+}
+
+// ---- global -> LDS ---------------------------------------------------------------------------------------------------------
+// 16 bytes per lane straight into LDS: lane i's granule lands at lds + 16 i (lds uniform in the wave).  Offsets at or beyond
+// `bytes` (the descriptor's limit) deliver zeros, which is how tile edges are padded.
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+constexpr unsigned OUT = 0x80000000u;                              // an offset that is never inside
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p, long long bytes) {
+  const unsigned n = bytes > 0x7fffffffll ? 0x7fffffffu : bytes < 0 ? 0u : (unsigned)bytes;
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, n, 0x00020000);
+}
+__device__ __forceinline__ void load_lds16(rsrc_t r, char* lds, unsigned off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
+}
+
+}  // namespace mma

@@ -6,6 +6,7 @@ Reference call sites are cited per function (FD = focal_decoder.py, EU = encoder
 UT = utils.py, BC = transfusion_bbox_coder.py of the reference plugin).
 """
 import ctypes as C
+import functools
 import os
 
 import torch
@@ -1756,3 +1757,180 @@ def unsplit_f16(pair, B, H, W):
                               H * W, _stream())
     _lib.check(st, 'ff3d_unsplit_f16')
     return out
+
+
+# ------------------------------------------------------------------- operators in fp32, bf16 and fp16 (dtype codes of ff3d.h)
+_DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 3}
+_ACTS = {'silu': 0, 'gelu': 1, 'relu': 2, 'sigmoid': 3}
+
+
+def _on_device_of(first):
+    """Decorator: run the wrapper with the device of its first tensor (``first(*args)``) current, as the launch and the stream need."""
+    def deco(fn):
+        @functools.wraps(fn)
+        def call(*a, **k):
+            t = first(*a)
+            if not isinstance(t, torch.Tensor) or not t.is_cuda:
+                raise RuntimeError(f'{fn.__name__}: expected CUDA (HIP) tensors - the HIP decoder path has no CPU fallback')
+            if t.get_device() == torch._C._cuda_getDevice():
+                return fn(*a, **k)
+            with torch.cuda.device(t.device):
+                return fn(*a, **k)
+        return call
+    return deco
+
+
+def _same(t, like, name, shape=None):
+    """t: a CUDA tensor of the device and dtype of ``like`` (and of ``shape``), or a RuntimeError."""
+    if not isinstance(t, torch.Tensor) or t.device != like.device or t.dtype != like.dtype:
+        raise RuntimeError(f'{name}: expected a {like.dtype} tensor on {like.device}, got '
+                           + (f'{t.dtype} on {t.device}' if isinstance(t, torch.Tensor) else type(t).__name__))
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise RuntimeError(f'{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}')
+
+
+def _ptr(t):
+    return C.c_void_p(0 if t is None else t.data_ptr())
+
+
+def _gated_args(x, weight, bias, act):
+    if x.dtype not in _DTYPE:
+        raise RuntimeError(f'gated_linear: expected fp32, bf16 or fp16 tensors, got {x.dtype}')
+    if act not in _ACTS:
+        raise ValueError(f'gated_linear: unknown activation {act!r} (one of {", ".join(_ACTS)})')
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[0] % 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+        raise RuntimeError(f'gated_linear: expected x (..., C) and weight (2 F, C), got {tuple(x.shape)} and {tuple(weight.shape)}')
+    F2, C_ = weight.shape
+    _same(weight, x, 'weight')
+    _same(x, x, 'x', (*x.shape[:-1], C_))
+    if bias is not None:
+        _same(bias, x, 'bias', (F2,))
+        bias = bias.contiguous()
+    x2 = x.reshape(-1, C_)
+    if x2.stride(1) != 1 or x2.stride(0) < C_:
+        x2 = x2.contiguous()
+    weight = weight.contiguous()
+    per = 16 // x.element_size()
+    pack = (1 if C_ % per or x2.stride(0) % per or x2.data_ptr() % 16 else 0) | (2 if C_ % per or weight.data_ptr() % 16 else 0)
+    return x2, weight, bias, F2 // 2, C_, pack
+
+
+@_on_device_of(lambda x, *a: x)
+def gated_linear(x, weight, bias=None, act='silu'):
+    """h = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel (ff3d_gated_linear_fwd): x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F)
+    or None, all fp32, bf16 or fp16 -> (..., F).  act: 'silu', 'gelu' (erf form), 'relu' or 'sigmoid'.  Sums in fp32, one rounding.
+    The differentiable form is ``autograd.gated_linear``."""
+    x2, weight, bias, F_, C_, pack = _gated_args(x, weight, bias, act)
+    M, code = x2.shape[0], _DTYPE[x.dtype]
+    h = torch.empty(*x.shape[:-1], F_, dtype=x.dtype, device=x.device)
+    if M == 0:
+        return h
+    lib = _lib.load()
+    n = lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
+    _lib.check(lib.ff3d_gated_linear_fwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(h), M, C_, F_, _ACTS[act], code, pack, _ptr(ws),
+                                         _stream()), 'ff3d_gated_linear_fwd')
+    return h
+
+
+@_on_device_of(lambda x, *a: x)
+def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
+    """Gradients of ``gated_linear`` for dh (..., F) -> (dx, dweight, dbias); None where ``want`` is false (or there is no bias)."""
+    x2, weight, bias, F_, C_, pack = _gated_args(x, weight, bias, act)
+    M, code = x2.shape[0], _DTYPE[x.dtype]
+    _same(dh, x, 'dh', (*x.shape[:-1], F_))
+    want_b = want[2] and bias is not None
+    new = torch.zeros if M == 0 else torch.empty
+    dx = new(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
+    dw = new(2 * F_, C_, dtype=x.dtype, device=x.device) if want[1] else None
+    db = new(2 * F_, dtype=x.dtype, device=x.device) if want_b else None
+    if M == 0 or not (want[0] or want[1] or want_b):
+        return dx, dw, db
+    dh2 = dh.reshape(-1, F_)
+    if dh2.stride(1) != 1 or dh2.stride(0) < F_:
+        dh2 = dh2.contiguous()
+    lib = _lib.load()
+    ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 1), dtype=torch.uint8, device=x.device)
+    _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh2.stride(0), _ptr(dx), _ptr(dw), _ptr(db),
+                                         M, C_, F_, _ACTS[act], code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
+    return dx, dw, db
+
+
+_NORM_KINDS = {2: 2, 1: 1, float('inf'): 0}
+
+
+def _grad_list(tensors, name):
+    """Host arrays (pointers, element counts, dtype codes) of a list of dense CUDA tensors on one device."""
+    dev = tensors[0].device
+    for i, t in enumerate(tensors):
+        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in _DTYPE or t.layout != torch.strided:
+            raise RuntimeError(f'{name}[{i}]: expected a dense fp32, bf16 or fp16 tensor on {dev}')
+        if not _dense(t):
+            raise RuntimeError(f'{name}[{i}]: expected a tensor without gaps or overlaps, got shape {tuple(t.shape)}, strides {t.stride()}')
+    n = len(tensors)
+    return ((C.c_void_p * n)(*[t.data_ptr() for t in tensors]), (C.c_int64 * n)(*[t.numel() for t in tensors]),
+            (C.c_int32 * n)(*[_DTYPE[t.dtype] for t in tensors]))
+
+
+def _dense(t):
+    """Do the elements of ``t`` fill one block of memory, in whatever order of dimensions?"""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((st, n) for n, st in zip(t.shape, t.stride()) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+def _norm_kind(norm_type):
+    kind = _NORM_KINDS.get(float(norm_type))
+    if kind is None:
+        raise ValueError(f'norm_type {norm_type!r}: 2, 1 or inf')
+    return kind
+
+
+@_on_device_of(lambda g, *a, **k: g[0] if len(g) else None)
+def grad_norm(grads, norm_type=2.0):
+    """Norm (2, 1 or inf) over all elements of a list of dense fp32 / bf16 / fp16 tensors of one device -> fp32 scalar on the device
+    (ff3d_grad_norm; sums in fp64, no host synchronisation)."""
+    kind = _norm_kind(norm_type)
+    ptrs, numel, codes = _grad_list(grads, 'grads')
+    lib = _lib.load()
+    dev = grads[0].device
+    norm = torch.empty((), device=dev)
+    ws = torch.empty(lib.ff3d_grad_norm_workspace_bytes(numel, len(grads)), dtype=torch.uint8, device=dev)
+    _lib.check(lib.ff3d_grad_norm(ptrs, numel, codes, len(grads), kind, _ptr(ws), _ptr(norm), _stream()), 'ff3d_grad_norm')
+    return norm
+
+
+@_on_device_of(lambda g, *a, **k: g[0] if len(g) else None)
+def clip_grads(grads, max_norm, norm_type=2.0, out=None):
+    """out_i = grads_i * min(1, max_norm / (norm + 1e-6)) with norm = ``grad_norm(grads, norm_type)`` -> norm (ff3d_clip_grads: one
+    launch per pass for up to 120 tensors).  ``out``: tensors of the same shapes and layouts (types may differ), disjoint from each
+    other and from every gradient but their own; None = in place."""
+    kind = _norm_kind(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f'max_norm {max_norm}: expected a number >= 0')
+    ptrs, numel, codes = _grad_list(grads, 'grads')
+    optrs, ocodes = ptrs, codes
+    if out is not None:
+        if len(out) != len(grads) or any(o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))
+                                         for o, g in zip(out, grads)):
+            raise RuntimeError('out: expected one tensor per gradient, of its shape and strides')
+        if out[0].device != grads[0].device:
+            raise RuntimeError(f'out: expected tensors on {grads[0].device}')
+        optrs, _, ocodes = _grad_list(out, 'out')
+    lib = _lib.load()
+    dev = grads[0].device
+    norm = torch.empty((), device=dev)
+    ws = torch.empty(lib.ff3d_grad_norm_workspace_bytes(numel, len(grads)), dtype=torch.uint8, device=dev)
+    st = lib.ff3d_clip_grads(ptrs, optrs, numel, codes, ocodes, len(grads), kind, max_norm, _ptr(ws), _ptr(norm), _stream())
+    if st == -5:
+        raise RuntimeError('clip_grads: two outputs share memory, or an output overlaps a gradient that is not its own')
+    _lib.check(st, 'ff3d_clip_grads')
+    for t in (grads if out is None else out):           # written through raw pointers: tell autograd
+        torch.autograd.graph.increment_version(t)
+    return norm

@@ -205,6 +205,33 @@ class HeuristicAssigner3D:
         return AssignResult(G, gt_inds, overlaps, labels=labels)
 
 
+# ------------------------------------------------------------------------------------------------ gradient clipping
+def clip_grads(grads, max_norm, norm_type=2.0, out=None):
+    """Scales a list of gradients by min(1, max_norm / (norm + 1e-6)), in place or into ``out``; returns their norm before the
+    scaling as a device scalar (``ops.clip_grads``; no host synchronisation)."""
+    return ops.clip_grads(grads, max_norm, norm_type, out)
+
+
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """``torch.nn.utils.clip_grad_norm_`` (mmcv's ``optimizer_config = dict(grad_clip=dict(max_norm, norm_type))``) on the own kernels:
+    the gradients of ``parameters`` (those that are not None) are clipped in place by their global norm, which is returned.
+    ``error_if_nonfinite`` reads the norm on the host."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    seen, grads = set(), []
+    for p in parameters:                                         # a parameter given twice counts once
+        if p.grad is not None and id(p) not in seen:
+            seen.add(id(p))
+            grads.append(p.grad)
+    if not grads:
+        return torch.zeros(())
+    if error_if_nonfinite:
+        norm = ops.grad_norm(grads, norm_type)
+        if not bool(torch.isfinite(norm)):
+            raise RuntimeError(f'the {norm_type}-norm of the gradients is not finite, so they are not clipped')
+    return ops.clip_grads(grads, max_norm, norm_type)
+
+
 # ------------------------------------------------------------------------------------------------ losses (mmdet 2.14)
 def clip_sigmoid(x, eps=1e-4):
     """mmdet3d ``clip_sigmoid``."""

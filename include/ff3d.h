@@ -42,7 +42,7 @@ typedef enum {
   FF3D_ERR_LAUNCH = -6       /* hipGetLastError() != hipSuccess after the launch        */
 } ff3d_status;
 
-enum { FF3D_F32 = 0, FF3D_BF16 = 1, FF3D_F16_SPLIT = 2 /* two fp16 planes: hi = fp16(x), then lo' = fp16((x - hi) * 2048) */ };
+enum { FF3D_F32 = 0, FF3D_BF16 = 1, FF3D_F16 = 3, FF3D_F16_SPLIT = 2 /* two fp16 planes: hi = fp16(x), then lo' = fp16((x - hi) * 2048) */ };
 enum { FF3D_MAX_LEVELS = 8, FF3D_HIST_BINS = 4096, FF3D_SPLIT_HINT_INTS = 65 * 64 };
 
 int ff3d_version(void);
@@ -743,6 +743,36 @@ int ff3d_conv3x3_halo_f16x3_group(int n, const void* const* x_hi, const void* co
 int ff3d_conv3x3_small_f16x3_group(int n, const void* const* x_hi, const void* const* x_lo, const void* const* w_hi,
                                    const void* const* w_lo, const float* const* bias, float* const* out, int B, int C, int H,
                                    int W, int K, const ff3d_scale_t* const* scale_host, ff3d_stream_t stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Gated projection of a feed-forward block (ABI 2.12), fp32 / bf16 / fp16 (dtype = FF3D_F32, FF3D_BF16, FF3D_F16; sums in fp32):
+ *   h = act(x Wg^T + bg) * (x Wu^T + bu)
+ *   x (M, C) with row stride ldx, weight (2 F, C) = [Wg ; Wu], bias (2 F) or NULL, h (M, F); act 0 silu, 1 gelu (erf), 2 relu,
+ *   3 sigmoid.
+ * ff3d_gated_linear_bwd: dh (M, F) with row stride lddh -> dx (M, C), dw (2 F, C), db (2 F); each may be NULL.  g and u are recomputed.
+ * pack: bit 0 / bit 1 = x / weight are first copied into the workspace with rows of whole 16-byte granules; needed where C or the row
+ *   stride is no multiple of 16 bytes or the base is not 16-byte aligned (without the bit such an operand is FF3D_ERR_ALIGNMENT).
+ * workspace: ff3d_gated_linear_workspace_bytes of the same M, C, F, dtype, pack and backward, 16-byte aligned; its content is
+ *   scratch.  2 F * C and M-independent row offsets stay below 2^31 bytes; results do not depend on timing (ordered sums). */
+int64_t ff3d_gated_linear_workspace_bytes(int M, int C, int F, int dtype, int pack, int backward);
+int ff3d_gated_linear_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, void* h, int M, int C, int F, int act,
+                          int dtype, int pack, void* workspace, ff3d_stream_t stream);
+int ff3d_gated_linear_bwd(const void* x, int64_t ldx, const void* weight, const void* bias, const void* dh, int64_t lddh, void* dx,
+                          void* dw, void* db, int M, int C, int F, int act, int dtype, int pack, void* workspace,
+                          ff3d_stream_t stream);
+
+/* Norm over all elements of n tensors and clipping by it (ABI 2.12):
+ *   norm = (sum |g|^2)^(1/2) (kind 2), sum |g| (kind 1) or max |g| (kind 0), sums in fp64, result fp32 on the device;
+ *   out_i = g_i * min(1, max_norm / (norm + 1e-6)), rounded once to the type of out_i.
+ * grads_host / out_host: HOST arrays of n device pointers to dense tensors of numel_host[i] elements (0 allowed) and type
+ *   dtype_host[i] / out_dtype_host[i] (FF3D_F32, FF3D_BF16, FF3D_F16).  An output may be its own gradient (in place); other overlaps are
+ *   not allowed.  The host arrays may be freed on return.  workspace: ff3d_grad_norm_workspace_bytes, 8-byte aligned. */
+int64_t ff3d_grad_norm_workspace_bytes(const int64_t* numel_host, int n);
+int ff3d_grad_norm(const void* const* grads_host, const int64_t* numel_host, const int32_t* dtype_host, int n, int kind,
+                   void* workspace, float* norm, ff3d_stream_t stream);
+int ff3d_clip_grads(const void* const* grads_host, void* const* out_host, const int64_t* numel_host, const int32_t* dtype_host,
+                    const int32_t* out_dtype_host, int n, int kind, float max_norm, void* workspace, float* norm,
+                    ff3d_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,62 @@
+"""What the operators in three types refuse before anything reaches the GPU, and their workspace sizes."""
+import ctypes
+
+import pytest
+import torch
+
+from focalformer3d_amd import _lib, ops, training
+
+
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(3, 8), torch.zeros(4, 8)
+    for call in (lambda: ops.gated_linear(x, w), lambda: ops.gated_linear_bwd(x, w, None, 'silu', torch.zeros(3, 2)), lambda: ops.grad_norm([x]),
+                 lambda: ops.clip_grads([x], 1.0), lambda: training.clip_grads([], 1.0)):
+        with pytest.raises(RuntimeError, match='CUDA'):
+            call()
+
+
+def test_no_gradients_have_norm_zero():
+    p = torch.nn.Parameter(torch.zeros(3))
+    assert float(training.clip_grad_norm_([p], 1.0)) == 0.0
+
+
+def test_norm_kinds():
+    with pytest.raises(ValueError):
+        ops._norm_kind(3)
+    assert [ops._norm_kind(k) for k in (2, 1.0, float('inf'))] == [2, 1, 0]
+
+
+def test_dense_layouts():
+    t = torch.zeros(4, 6, 5)
+    assert ops._dense(t) and ops._dense(t.permute(2, 0, 1)) and ops._dense(t[1:3]) and ops._dense(torch.zeros(3, 1, 4).transpose(0, 1))
+    assert not ops._dense(t[:, ::2]) and not ops._dense(t[:, 1:3]) and not ops._dense(torch.zeros(1).expand(4))
+
+
+def test_c_entries_check_their_arguments():
+    """Every refusal returns its status without touching a pointer: the addresses here are none."""
+    lib = _lib.load()
+    f = lib.ff3d_gated_linear_fwd
+    p = ctypes.c_void_p(4096)
+    ok = dict(x=p, ldx=16, w=p, b=None, h=p, M=2, C=16, F=4, act=0, dt=0, pack=0, ws=None)
+    run = lambda **k: f(*{**ok, **k}.values(), None)  # noqa: E731
+    assert run(x=None) == -4 and run(w=None) == -4 and run(h=None) == -4
+    assert run(dt=2) == -2 and run(dt=7) == -2
+    for bad in (dict(M=0), dict(C=0), dict(F=-1), dict(ldx=15), dict(act=4), dict(pack=4), dict(C=1 << 20, F=1 << 20, ldx=1 << 20)):
+        assert run(**bad) == -1, bad
+    assert run(ldx=17) == -3 and run(x=ctypes.c_void_p(4100)) == -3 and run(w=ctypes.c_void_p(4104)) == -3
+    assert run(C=15) == -3 and run(C=15, pack=1) == -3
+    assert run(C=15, pack=3) == -4 and run(C=15, pack=3, ws=ctypes.c_void_p(4100)) == -3          # needs a workspace
+    assert lib.ff3d_gated_linear_workspace_bytes(2, 16, 4, 0, 0, 0) == 0
+    # packed rows of 16 floats, each part on 256 bytes
+    assert lib.ff3d_gated_linear_workspace_bytes(2, 15, 4, 0, 3, 0) == 256 + 512
+    norm = lib.ff3d_grad_norm
+    ptrs, numel, code = (ctypes.c_void_p * 1)(4096), (ctypes.c_int64 * 1)(5), (ctypes.c_int32 * 1)(0)
+    assert norm(ptrs, numel, code, 1, 3, p, p, None) == -1 and norm(ptrs, (ctypes.c_int64 * 1)(-1), code, 1, 2, p, p, None) == -1
+    assert norm(ptrs, numel, (ctypes.c_int32 * 1)(2), 1, 2, p, p, None) == -2
+    assert norm((ctypes.c_void_p * 1)(None), numel, code, 1, 2, p, p, None) == -4 and norm(ptrs, numel, code, 1, 2, None, p, None) == -4
+    clip = lib.ff3d_clip_grads
+    two, n2, c2 = (ctypes.c_void_p * 2)(4096, 4096 + 12), (ctypes.c_int64 * 2)(5, 5), (ctypes.c_int32 * 2)(0, 0)
+    assert clip(two, two, n2, c2, c2, 2, 2, 1.0, p, p, None) == -5
+    assert clip(ptrs, None, numel, code, code, 1, 2, 1.0, p, p, None) == -4
+    # four elements, one piece, one more for none
+    assert lib.ff3d_grad_norm_workspace_bytes((ctypes.c_int64 * 2)(4, 0), 2) == 16
