@@ -25,6 +25,16 @@ class Scale(C.Structure):
 
 _sp = C.POINTER(Scale)
 
+
+class DiffAttention(C.Structure):
+    """ff3d_diff_attention_t (include/ff3d.h): operands, strides and shape of one differential attention."""
+    _fields_ = ([(n, _vp) for n in ('q', 'k', 'v', 'lam', 'mask', 'kv_lens')]
+                + [(n, _i64) for n in ('q_batch', 'q_row', 'k_batch', 'k_row', 'v_batch', 'v_row', 'mask_batch', 'mask_row')]
+                + [(n, C.c_int32) for n in ('B', 'Nq', 'Nk', 'heads', 'kv_heads', 'd', 'causal', 'dtype')] + [('scale', _f)])
+
+
+_dp = C.POINTER(DiffAttention)
+
 # name -> (restype, argtypes); must list exactly the symbols include/ff3d.h declares
 SIGNATURES = {
     'ff3d_version': (_i, []),
@@ -107,6 +117,9 @@ SIGNATURES = {
     'ff3d_gated_linear_workspace_bytes': (_i64, [_i] * 6),
     'ff3d_gated_linear_fwd': (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     'ff3d_gated_linear_bwd': (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    'ff3d_diff_attention_workspace_bytes': (_i64, [_dp, _i]),
+    'ff3d_diff_attention_fwd': (_i, [_dp] + [_vp] * 5),
+    'ff3d_diff_attention_bwd': (_i, [_dp] + [_vp] * 4 + [_i64, _i64] + [_vp] * 6),
     'ff3d_grad_norm_workspace_bytes': (_i64, [_vp, _i]),
     'ff3d_grad_norm': (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     'ff3d_clip_grads': (_i, [_vp] * 5 + [_i, _i, _f, _vp, _vp, _vp]),

@@ -171,6 +171,32 @@ class MaskedSelfAttentionFunction(Function):
         return gq, gk, gv, None, None, None
 
 
+class DifferentialAttentionFunction(Function):
+    """softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v per head (ops.diff_attention_train_fwd / _bwd)."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale):
+        out, out2, lse = ops.diff_attention_train_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+        ctx.save_for_backward(q, k, v, lam, out, out2, lse, mask, kv_lens)
+        ctx.meta = heads, kv_heads, causal, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, lam, out, out2, lse, mask, kv_lens = ctx.saved_tensors
+        heads, kv_heads, causal, scale = ctx.meta
+        grads = ops.diff_attention_bwd(q, k, v, lam, heads, out, out2, lse, dout, kv_heads, mask, kv_lens, causal, scale, ctx.needs_input_grad[:4])
+        return (*grads, None, None, None, None, None, None)
+
+
+def differential_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
+    """Differentiable ``ops.diff_attention`` (same arguments); without gradients to compute it is that operator."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
+        return DifferentialAttentionFunction.apply(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    return ops.diff_attention(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+
+
 class GatedLinearFunction(Function):
     """``h = act(x Wg^T + bg) * (x Wu^T + bu)`` (ops.gated_linear); backward = ops.gated_linear_bwd, which recomputes both projections:
     only the inputs are saved."""

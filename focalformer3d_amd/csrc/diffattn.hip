@@ -1,0 +1,814 @@
+// Differential attention, forward and backward, in fp32, bf16 and fp16: per head
+//   out = P1 v - lam P2 v,   Pm = softmax_j(scale <q_m, k_m>)       head of q and k: [1 | 2] of d each, of v: 2 d
+// and, given dO, with dP = dO v^T (one product serves both maps) and W = P1 - lam P2 (one product for dv):
+//   dv = W^T dO,  D1 = rowsum(P1 dP) = <dO, O1>,  D2 = <dO, O2>,  dS1 = P1 (dP - D1),  dS2 = -lam P2 (dP - D2),
+//   dq_m = scale dS_m k_m,  dk_m = scale dS_m^T q_m,  dlam = -sum D2.
+// Keys that a boolean mask, a length or the causal order excludes count as absent; a row without keys gives zeros.
+//
+// The query heads that share a key head are rows of one problem: row = i r + (head within its group), so a block's keys and values
+// serve all of them, a single new token fills r columns of a tile, and the gradients of shared heads are summed where they arise.
+// Score tiles are 32 x 32 with the long-lived side as columns (queries in the forward and dq kernels, keys in the dk / dv kernel):
+// a lane owns half a column of scores, so the softmax statistics of a row are one value per lane, and the tile, rounded, is already
+// the operand of the next product (ff3d_mma.h).  Keys and values (queries and dO) pass through LDS once per block in two stages, by
+// DMA; their transposed reads use ds_read_b64_tr_b16.
+//   forward  one pass with running maximum and sum per map; with few rows the keys are cut into slices that a second kernel joins
+//   dq       columns = queries, loops over keys;  dk / dv  columns = keys, loops over the rows.  No atomics: results do not depend
+//            on timing.  Scores are recomputed from q, k and the saved log-sum-exp.
+// fp16: dS of a long row is far below fp16's normal range, so its columns carry a running power-of-two scale (Scaled).
+#include "ff3d_mma.h"
+
+namespace {
+
+using namespace mma;
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr int ROWDATA = 5;        // fp32 values per row of the backward pass: log2-sum-exp 1, 2, D1, D2, lam
+
+struct Args {
+  const char *q, *k, *v, *dout;
+  const void* lam;
+  const uint8_t* mask;
+  const int32_t* lens;
+  long long q_b, q_r, k_b, k_r, v_b, v_r, do_b, do_r;     // elements
+  long long m_b, m_r;                                     // bytes
+  char *out, *dq, *dk, *dv;
+  float *out2, *lse, *part, *rowdata;
+  int B, Nq, Nk, H, G, r, d, R, Rp, causal, mask4, splits, split_len, tiles;
+  float scale, c;                 // c = scale * log2(e)
+};
+
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Where a column's values are rounded to fp16, they are multiplied by a power of two that keeps the largest so far in [2^9, 2^15];
+// the accumulators of the column follow when it changes.  The other types have the exponent range and skip this.
+template <typename T>
+struct Scaled {
+  float s = 0.f;                  // 0: nothing but zeros so far
+  template <int N>
+  __device__ __forceinline__ void see(float mx, f32x16* acc) {
+    if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const bool need = mx * s > 32768.f || (s == 0.f && mx > 0.f);
+      if (__any(need)) {
+        if (need) {
+          const int e = (int)((__float_as_uint(mx) >> 23) & 0xff) - 127;
+          const float n = ff3d_pow2(9 - e), f = s > 0.f ? n / s : 1.f;
+          s = n;
+#pragma unroll
+          for (int t = 0; t < N; ++t) acc[t] *= f;
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ float mul() const {
+    if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) return s;
+    else return 1.f;
+  }
+  __device__ __forceinline__ float undo() const {
+    if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) return s > 0.f ? 1.f / s : 1.f;
+    else return 1.f;
+  }
+};
+template <typename T>
+__device__ __forceinline__ vec8<T> scaled_frag(const f32x16& c, int step, float mul) {
+  if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
+    vec8<T> v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = from_f<T>(c[8 * step + e] * mul);
+    return v;
+  } else {
+    return acc_frag<T>(c, step);
+  }
+}
+
+// ROWS rows of 2 D elements in LDS, in granules: [map 1 | map 2] of D each (SPLIT; the d of a map may fill only a part) or 2 d elements
+template <typename T, int D, int ROWS, int NT, bool SPLIT>
+struct Tile {
+  static constexpr int P = Type<T>::PER16, GR = 2 * D / P, N = ROWS * GR / NT;
+  static_assert(ROWS * GR % NT == 0, "whole granules per thread");
+  __device__ __forceinline__ static int source(int g, int d) {         // element offset in a row of the tensor, or -1
+    const int e = g * P;
+    if constexpr (SPLIT) {
+      const int w = e % D;
+      return w < d ? (e / D) * d + w : -1;
+    } else {
+      return e < 2 * d ? e : -1;
+    }
+  }
+  // rows row0 .. of one sequence: row j at base + j * ld (bytes); rows from `limit` on are zeros
+  __device__ __forceinline__ static void keys(char* lds, const char* base, long long ld, int row0, int limit, int d, int tid, int wave) {
+    const char* p = base + row0 * ld;
+    const rsrc_t rs = make_rsrc(p, (long long)(limit - row0) * ld);     // the last row's tail may lie outside: guarded by `limit` below
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+      const int at = it * NT + tid, r = at / GR, g = place<GR>(r, at % GR), s = source(g, d);
+      load_lds16(rs, lds + (it * NT + wave * 64) * 16, row0 + r < limit && s >= 0 ? (unsigned)r * (unsigned)ld + s * (unsigned)sizeof(T) : OUT);
+    }
+  }
+  // packed rows row0 ..: row = i r + h, at base + i * ld + h * head bytes
+  __device__ __forceinline__ static void rows(char* lds, const char* base, long long ld, int head, int row0, int R, int per, int d, int tid, int wave) {
+    const int i0 = row0 / per;
+    const char* p = base + i0 * ld;
+    const rsrc_t rs = make_rsrc(p, 0x7fffffff);
+#pragma unroll
+    for (int it = 0; it < N; ++it) {
+      const int at = it * NT + tid, r = at / GR, g = place<GR>(r, at % GR), s = source(g, d);
+      const int row = row0 + r, i = row / per, h = row - i * per;
+      load_lds16(rs, lds + (it * NT + wave * 64) * 16,
+                 row < R && s >= 0 ? (unsigned)(i - i0) * (unsigned)ld + (unsigned)h * (unsigned)head + s * (unsigned)sizeof(T) : OUT);
+    }
+  }
+};
+
+// 8 consecutive elements of a row held in registers as an operand (zeros where `in` is false)
+template <typename T>
+__device__ __forceinline__ vec8<T> load8(const char* p, bool in) {
+  vec8<T> v;
+  u32x4* w = (u32x4*)&v;
+#pragma unroll
+  for (int k = 0; k < (int)sizeof(vec8<T>) / 16; ++k) w[k] = in ? *(const u32x4*)(p + 16 * k) : (u32x4)(0u);
+  return v;
+}
+
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T v[4];
+};
+template <typename T>
+__device__ __forceinline__ void put4(T* p, float a, float b, float c, float d) {
+  Four<T> f = {{from_f<T>(a), from_f<T>(b), from_f<T>(c), from_f<T>(d)}};
+  *(Four<T>*)p = f;
+}
+
+__device__ __forceinline__ int key_limit(const Args& a, int b) {
+  int n = a.Nk;
+  if (a.lens) n = max(0, min(n, a.lens[b]));
+  return n;
+}
+
+// whether keys j .. j + 3 are blocked for a row of the mask, as 4 bits
+__device__ __forceinline__ unsigned blocked4(const Args& a, const uint8_t* mrow, int j) {
+  unsigned bits = 0;
+  if (a.mask4 && j + 3 < a.Nk) {
+    const unsigned w = *(const unsigned*)(mrow + j);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) bits |= (((w >> (8 * e)) & 0xff) ? 1u : 0u) << e;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e < a.Nk && mrow[j + e]) bits |= 1u << e;
+  }
+  return bits;
+}
+
+// Excludes keys from a 32 x 32 tile with queries as columns: both maps' scores become -inf.
+__device__ __forceinline__ void exclude_cols_q(const Args& a, const uint8_t* mrow, f32x16& s1, f32x16& s2, int j0, int jlast, int half, bool use_mask) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int j = j0 + 8 * q + 4 * half;
+    const unsigned m = use_mask ? blocked4(a, mrow, j) : 0u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (j + e > jlast || (m >> e & 1)) s1[4 * q + e] = -INFINITY, s2[4 * q + e] = -INFINITY;
+  }
+}
+
+template <typename T, int D, int KT>
+__device__ __forceinline__ f32x16 scores(const char* tile, int kb, int map, const vec8<T>* other, int lane) {
+  constexpr int GR = 2 * D / Type<T>::PER16;
+  f32x16 s = (f32x16)(0.f);
+#pragma unroll
+  for (int st = 0; st < D / 16; ++st) s = mfma16(row_frag<T, GR>(tile, kb * 32 + (lane & 31), map * D + 16 * st, lane >> 5), other[st], s);
+  return s;
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------------------
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
+  constexpr int NT = NW * 64, KT = (sizeof(T) == 2 && NW > 1) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
+  constexpr int VT = 2 * D / 32, ST = D / 16;
+  __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+
+  int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  const int split = bid % a.splits;
+  bid /= a.splits;
+  const int tile = a.tiles - 1 - bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;   // causal: the long ones first
+  const int row = tile * NW * 32 + wave * 32 + (lane & 31);
+  const bool in = row < a.R;
+  const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
+
+  vec8<T> q[2][ST];
+  {
+    const char* p = a.q + (b * a.q_b + (long long)i * a.q_r + (long long)h * 2 * a.d) * (long long)sizeof(T);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int e = 16 * st + 8 * half;
+        q[m][st] = load8<T>(p + (m * a.d + e) * (int)sizeof(T), in && e < a.d);
+      }
+  }
+  const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
+  int kend = limit;
+  if (a.causal) kend = min(kend, min(a.R - 1, tile * NW * 32 + NW * 32 - 1) / a.r + shift + 1);
+  const int kbeg = split * a.split_len;
+  kend = min(kend, kbeg + a.split_len);
+  const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;       // last key of this lane's row
+  const int wave_first = a.causal ? min(limit - 1, min(tile * NW * 32 + wave * 32, a.R - 1) / a.r + shift) : limit - 1;   // smallest in the wave
+  const uint8_t* mrow = a.mask ? a.mask + b * a.m_b + i * a.m_r : nullptr;
+
+  f32x16 o[2][VT];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < VT; ++t) o[m][t] = (f32x16)(0.f);
+  float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
+  const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
+  const long long kld = a.k_r * (long long)sizeof(T), vld = a.v_r * (long long)sizeof(T);
+  typedef Tile<T, D, KT, NT, true> KTile;
+  typedef Tile<T, D, KT, NT, false> VTile;
+  const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
+  if (nt > 0) {
+    KTile::keys(lds, kbase, kld, kbeg, limit, a.d, tid, wave);
+    VTile::keys(lds + BYTES, vbase, vld, kbeg, limit, a.d, tid, wave);
+  }
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = kbeg + t * KT;
+    const char* kt = lds + (t & 1) * 2 * BYTES;
+    const char* vt = kt + BYTES;
+    __syncthreads();
+    if (t + 1 < nt) {
+      char* nx = lds + ((t + 1) & 1) * 2 * BYTES;
+      KTile::keys(nx, kbase, kld, j0 + KT, limit, a.d, tid, wave);
+      VTile::keys(nx + BYTES, vbase, vld, j0 + KT, limit, a.d, tid, wave);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      const int jb = j0 + kb * 32;
+      if (jb >= kend) break;
+      f32x16 s[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) s[m] = scores<T, D, KT>(kt, kb, m, q[m], lane);
+      if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
+      vec8<T> p[2][2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        float x = s[m][0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) x = fmaxf(x, s[m][e]);
+        x = fmaxf(x, __shfl_xor(x, 32));
+        const float mn = fmaxf(mx[m], x), base = mn == -INFINITY ? 0.f : mn * a.c;
+        const float alpha = exp2_(mx[m] * a.c - base);
+        mx[m] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          s[m][e] = exp2_(fmaf(s[m][e], a.c, -base));
+          sum += s[m][e];
+        }
+        l[m] = fmaf(l[m], alpha, sum);
+        if (__any(alpha != 1.f)) {
+#pragma unroll
+          for (int v = 0; v < VT; ++v) o[m][v] *= alpha;
+        }
+        p[m][0] = acc_frag<T>(s[m], 0);
+        p[m][1] = acc_frag<T>(s[m], 1);
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st)
+#pragma unroll
+        for (int v = 0; v < VT; ++v) {
+          const vec8<T> f = col_frag_acc<T, GR, false>(vt, kb * 32 + 16 * st, v * 32, lane);
+          o[0][v] = mfma16(f, p[0][st], o[0][v]);
+          o[1][v] = mfma16(f, p[1][st], o[1][v]);
+        }
+    }
+  }
+  l[0] += __shfl_xor(l[0], 32);
+  l[1] += __shfl_xor(l[1], 32);
+  if (!in) return;
+  if (a.splits > 1) {              // [split][bg][row]: O1, O2 (2 d each), then maximum and sum of both maps
+    float* p = a.part + (((long long)split * a.B * a.G + bg) * a.R + row) * (4 * a.d + 4);
+    if (half == 0)
+#pragma unroll
+      for (int m = 0; m < 2; ++m) p[4 * a.d + 2 * m] = mx[m] == -INFINITY ? -INFINITY : mx[m] * a.c, p[4 * a.d + 2 * m + 1] = l[m];
+    if (l[0] == 0.f && l[1] == 0.f) return;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int v = 0; v < VT; ++v)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int e = v * 32 + 8 * x + 4 * half;
+          if (e < 2 * a.d) put4(p + m * 2 * a.d + e, o[m][v][4 * x], o[m][v][4 * x + 1], o[m][v][4 * x + 2], o[m][v][4 * x + 3]);
+        }
+    return;
+  }
+  const float i0 = l[0] == 0.f ? 0.f : 1.f / l[0], i1 = l[1] == 0.f ? 0.f : 1.f / l[1], lam = to_f(((const T*)a.lam)[h]);
+  const long long at = ((long long)b * a.Nq + i) * a.H + h;
+#pragma unroll
+  for (int v = 0; v < VT; ++v)
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int e = v * 32 + 8 * x + 4 * half;
+      if (e < 2 * a.d) {
+        float y[4], z[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[k] = o[1][v][4 * x + k] * i1, y[k] = o[0][v][4 * x + k] * i0 - lam * z[k];
+        put4((T*)a.out + at * 2 * a.d + e, y[0], y[1], y[2], y[3]);
+        if (a.out2) put4(a.out2 + at * 2 * a.d + e, z[0], z[1], z[2], z[3]);
+      }
+    }
+  if (a.lse && half == 0)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) a.lse[((long long)bg * 2 + m) * a.R + row] = l[m] == 0.f ? INFINITY : mx[m] * a.c + log2f(l[m]);
+}
+
+// joins the slices of the keys: one wave per row
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(Args a) {
+  const int lane = threadIdx.x & 63;
+  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (at >= (long long)a.B * a.G * a.R) return;
+  const int bg = (int)(at / a.R), row = (int)(at % a.R), b = bg / a.G, g = bg % a.G, i = row / a.r, h = g * a.r + row % a.r;
+  const long long step = (long long)a.B * a.G * a.R * (4 * a.d + 4);
+  const float* p = a.part + at * (4 * a.d + 4);
+  float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s)
+#pragma unroll
+    for (int m = 0; m < 2; ++m) top[m] = fmaxf(top[m], p[s * step + 4 * a.d + 2 * m]);
+  float o[2][2] = {};              // [map][element lane, lane + 64]
+  for (int s = 0; s < a.splits; ++s) {
+    const float* ps = p + s * step;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      const float ls = ps[4 * a.d + 2 * m + 1];
+      if (ls == 0.f) continue;     // no key in this slice
+      const float w = exp2_(ps[4 * a.d + 2 * m] - top[m]);
+      l[m] += w * ls;
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        if (lane + 64 * k < 2 * a.d) o[m][k] = fmaf(w, ps[m * 2 * a.d + lane + 64 * k], o[m][k]);
+    }
+  }
+  const float i0 = l[0] == 0.f ? 0.f : 1.f / l[0], i1 = l[1] == 0.f ? 0.f : 1.f / l[1], lam = to_f(((const T*)a.lam)[h]);
+  const long long to = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d;
+#pragma unroll
+  for (int k = 0; k < 2; ++k)
+    if (lane + 64 * k < 2 * a.d) {
+      const float z = o[1][k] * i1;
+      ((T*)a.out)[to + lane + 64 * k] = from_f<T>(o[0][k] * i0 - lam * z);
+      if (a.out2) a.out2[to + lane + 64 * k] = z;
+    }
+  if (a.lse && lane < 2) a.lse[((long long)bg * 2 + lane) * a.R + row] = l[lane] == 0.f ? INFINITY : top[lane] + log2f(l[lane]);
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------------------
+// rowdata (B G, ROWDATA, Rp): log2-sum-exps, D1 = <dO, out> + lam D2, D2 = <dO, O2>, lam; zeros behind R.  16 lanes per row.
+template <typename T>
+__global__ __launch_bounds__(256) void rows_kernel(Args a) {
+  const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (at >= (long long)a.B * a.G * a.Rp) return;
+  const int bg = (int)(at / a.Rp), row = (int)(at % a.Rp), lane = threadIdx.x & 15;
+  float v[ROWDATA] = {};
+  if (row < a.R) {
+    const int b = bg / a.G, g = bg % a.G, i = row / a.r, h = g * a.r + row % a.r;
+    const long long o = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d;
+    const T* go = (const T*)a.dout + b * a.do_b + i * a.do_r + (long long)h * 2 * a.d;
+    float d = 0.f, d2 = 0.f;
+    for (int e = lane; e < 2 * a.d; e += 16) {
+      const float x = to_f(go[e]);
+      d = fmaf(x, to_f(((const T*)a.out)[o + e]), d);
+      d2 = fmaf(x, a.out2[o + e], d2);
+    }
+#pragma unroll
+    for (int x = 8; x > 0; x >>= 1) d += __shfl_xor(d, x), d2 += __shfl_xor(d2, x);
+    const float lam = to_f(((const T*)a.lam)[h]);
+    v[0] = a.lse[((long long)bg * 2) * a.R + row], v[1] = a.lse[((long long)bg * 2 + 1) * a.R + row];
+    v[2] = fmaf(lam, d2, d), v[3] = d2, v[4] = lam;
+  }
+  if (lane == 0)
+#pragma unroll
+    for (int k = 0; k < ROWDATA; ++k) a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + row] = v[k];
+}
+
+// dlam[h] = -sum over batch and queries of D2: one block per head, fp64 sums in a fixed order
+template <typename T>
+__global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
+  __shared__ double part[16];
+  const int h = blockIdx.x, g = h / a.r, x = h % a.r;
+  double s = 0.0;
+  for (int b = 0; b < a.B; ++b) {
+    const float* p = a.rowdata + ((long long)(b * a.G + g) * ROWDATA + 3) * a.Rp + x;
+    for (int i = threadIdx.x; i < a.Nq; i += 1024) s += (double)p[(long long)i * a.r];
+  }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int k = 0; k < 16; ++k) s += part[k];
+    dlam[h] = from_f<T>((float)-s);
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dq_kernel(Args a) {
+  constexpr int NT = 256, KT = sizeof(T) == 2 ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
+  constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1;
+  __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+  const int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  const int tile = a.tiles - 1 - bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;
+  const int row = tile * 128 + wave * 32 + (lane & 31);
+  const bool in = row < a.R;
+  const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
+
+  vec8<T> q[2][ST], go[VS];
+  {
+    const char* p = a.q + (b * a.q_b + (long long)i * a.q_r + (long long)h * 2 * a.d) * (long long)sizeof(T);
+    const char* po = a.dout + (b * a.do_b + (long long)i * a.do_r + (long long)h * 2 * a.d) * (long long)sizeof(T);
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int e = 16 * st + 8 * half;
+        q[m][st] = load8<T>(p + (m * a.d + e) * (int)sizeof(T), in && e < a.d);
+      }
+#pragma unroll
+    for (int st = 0; st < VS; ++st) {
+      const int e = 16 * st + 8 * half;
+      go[st] = load8<T>(po + e * (int)sizeof(T), in && e < 2 * a.d);
+    }
+  }
+  float rd[ROWDATA];
+#pragma unroll
+  for (int k = 0; k < ROWDATA; ++k) rd[k] = a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + rowc];
+  const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
+  int kend = limit;
+  if (a.causal) kend = min(kend, min(a.R - 1, tile * 128 + 127) / a.r + shift + 1);
+  const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;
+  const int wave_first = a.causal ? min(limit - 1, min(tile * 128 + wave * 32, a.R - 1) / a.r + shift) : limit - 1;
+  const uint8_t* mrow = a.mask ? a.mask + b * a.m_b + i * a.m_r : nullptr;
+
+  f32x16 acc[2][QT];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < QT; ++t) acc[m][t] = (f32x16)(0.f);
+  Scaled<T> sc[2];
+
+  const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
+  const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
+  const long long kld = a.k_r * (long long)sizeof(T), vld = a.v_r * (long long)sizeof(T);
+  typedef Tile<T, D, KT, NT, true> KTile;
+  typedef Tile<T, D, KT, NT, false> VTile;
+  const int nt = kend > 0 ? (kend + KT - 1) / KT : 0;
+  if (nt > 0) {
+    KTile::keys(lds, kbase, kld, 0, limit, a.d, tid, wave);
+    VTile::keys(lds + BYTES, vbase, vld, 0, limit, a.d, tid, wave);
+  }
+  for (int t = 0; t < nt; ++t) {
+    const int j0 = t * KT;
+    const char* kt = lds + (t & 1) * 2 * BYTES;
+    const char* vt = kt + BYTES;
+    __syncthreads();
+    if (t + 1 < nt) {
+      char* nx = lds + ((t + 1) & 1) * 2 * BYTES;
+      KTile::keys(nx, kbase, kld, j0 + KT, limit, a.d, tid, wave);
+      VTile::keys(nx + BYTES, vbase, vld, j0 + KT, limit, a.d, tid, wave);
+    }
+#pragma unroll
+    for (int kb = 0; kb < KT / 32; ++kb) {
+      const int jb = j0 + kb * 32;
+      if (jb >= kend) break;
+      f32x16 s[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) s[m] = scores<T, D, KT>(kt, kb, m, q[m], lane);
+      const bool some = a.mask || jb + 31 > wave_first;
+      if (some) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
+      f32x16 dp = (f32x16)(0.f);
+#pragma unroll
+      for (int st = 0; st < VS; ++st) dp = mfma16(row_frag<T, GR>(vt, kb * 32 + (lane & 31), 16 * st, half), go[st], dp);
+      float top[2] = {0.f, 0.f};
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float pr = exp2_(fmaf(s[m][e], a.c, -rd[m]));
+          float ds = pr * (dp[e] - rd[2 + m]);
+          if (m == 1) ds *= -rd[4];
+          if (some && s[m][e] == -INFINITY) ds = 0.f;
+          s[m][e] = ds;
+          top[m] = fmaxf(top[m], fabsf(ds));
+        }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        sc[m].template see<QT>(top[m], acc[m]);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const vec8<T> f = scaled_frag<T>(s[m], st, sc[m].mul());
+#pragma unroll
+          for (int x = 0; x < QT; ++x)
+            acc[m][x] = mfma16(col_frag_acc<T, GR, false>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, acc[m][x]);
+        }
+      }
+    }
+  }
+  if (!in) return;
+  T* out = (T*)a.dq + (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d;
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float f = a.scale * sc[m].undo();
+#pragma unroll
+    for (int x = 0; x < QT; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int col = (D >= 32 ? m * D : 0) + x * 32 + 8 * y + 4 * half, w = col % D;
+        if (col / D == m && w < a.d) put4(out + m * a.d + w, acc[m][x][4 * y] * f, acc[m][x][4 * y + 1] * f, acc[m][x][4 * y + 2] * f, acc[m][x][4 * y + 3] * f);
+      }
+  }
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void dkv_kernel(Args a) {
+  constexpr int NT = 256, QR = (sizeof(T) == 2 && D == 16) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = QR * GR * 16;
+  constexpr int RG = ROWDATA * QR / 4, STAGE = 2 * BYTES + (RG + 63) / 64 * 1024;      // RG granules of row values
+  constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1, VT = 2 * D / 32;
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+  const int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  const int tile = bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;
+  const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
+  const int jw = tile * 128 + wave * 32, j = jw + (lane & 31);
+  const bool in = j < limit;
+
+  const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
+  const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
+  vec8<T> k[2][ST], v[VS];
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int st = 0; st < ST; ++st) {
+      const int e = 16 * st + 8 * half;
+      k[m][st] = load8<T>(kbase + ((long long)j * a.k_r + m * a.d + e) * (long long)sizeof(T), in && e < a.d);
+    }
+#pragma unroll
+  for (int st = 0; st < VS; ++st) {
+    const int e = 16 * st + 8 * half;
+    v[st] = load8<T>(vbase + ((long long)j * a.v_r + e) * (long long)sizeof(T), in && e < 2 * a.d);
+  }
+
+  f32x16 dv[VT], dk[2][QT];
+#pragma unroll
+  for (int t = 0; t < VT; ++t) dv[t] = (f32x16)(0.f);
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int t = 0; t < QT; ++t) dk[m][t] = (f32x16)(0.f);
+  Scaled<T> sv, sk[2];
+
+  const int head = 2 * a.d * (int)sizeof(T);
+  const char* qbase = a.q + (b * a.q_b + (long long)g * a.r * 2 * a.d) * (long long)sizeof(T);
+  const char* obase = a.dout + (b * a.do_b + (long long)g * a.r * 2 * a.d) * (long long)sizeof(T);
+  const long long qld = a.q_r * (long long)sizeof(T), old_ = a.do_r * (long long)sizeof(T);
+  const float* rdata = a.rowdata + (long long)bg * ROWDATA * a.Rp;
+  typedef Tile<T, D, QR, NT, true> QTile;
+  typedef Tile<T, D, QR, NT, false> OTile;
+  int rbeg = 0;
+  if (a.causal) rbeg = (int)(min((long long)max(0, tile * 128 - shift) * a.r, (long long)a.Rp) / QR * QR);
+  const int nt = tile * 128 < limit ? (a.R - rbeg + QR - 1) / QR : 0;
+
+  auto stage = [&](char* to, int row0) {
+    QTile::rows(to, qbase, qld, head, row0, a.R, a.r, a.d, tid, wave);
+    OTile::rows(to + BYTES, obase, old_, head, row0, a.R, a.r, a.d, tid, wave);
+    if (wave * 64 < RG) {          // QR / 4 granules of each of the arrays
+      const rsrc_t rs = make_rsrc(rdata + row0, ((long long)ROWDATA * a.Rp - row0) * 4);
+      load_lds16(rs, to + 2 * BYTES + wave * 1024, tid < RG ? (unsigned)(tid / (QR / 4)) * (unsigned)a.Rp * 4u + (tid % (QR / 4)) * 16u : OUT);
+    }
+  };
+  if (nt > 0) stage(lds, rbeg);
+  for (int t = 0; t < nt; ++t) {
+    const int row0 = rbeg + t * QR;
+    const char* qt = lds + (t & 1) * STAGE;
+    const char* ot = qt + BYTES;
+    const float* rd = (const float*)(qt + 2 * BYTES);
+    __syncthreads();
+    if (t + 1 < nt) stage(lds + ((t + 1) & 1) * STAGE, row0 + QR);
+#pragma unroll
+    for (int rb = 0; rb < QR / 32; ++rb) {
+      f32x16 s[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) s[m] = scores<T, D, QR>(qt, rb, m, k[m], lane);
+      // (row, key) pairs to leave out: keys past the limit, the causal order, the mask
+      const bool some = a.mask || jw + 31 >= limit || (a.causal && jw + 31 > (row0 + rb * 32) / a.r + shift);
+      if (some) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int row = min(row0 + rb * 32 + acc_row(e, half), a.R - 1), i = row / a.r;
+          bool no = !in || (a.causal && j > i + shift);
+          if (a.mask && !no) no = a.mask[b * a.m_b + i * a.m_r + j] != 0;
+          if (no) s[0][e] = -INFINITY, s[1][e] = -INFINITY;
+        }
+      }
+      f32x16 dp = (f32x16)(0.f);
+#pragma unroll
+      for (int st = 0; st < VS; ++st) dp = mfma16(row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * st, half), v[st], dp);
+      f32x16 w;
+      float top[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int rr = rb * 32 + 8 * y + 4 * half;
+        float r4[ROWDATA][4];
+#pragma unroll
+        for (int n = 0; n < ROWDATA; ++n) *(u32x4*)r4[n] = *(const u32x4*)(rd + n * QR + rr);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int e = 4 * y + x;
+          const bool out = some && s[0][e] == -INFINITY && s[1][e] == -INFINITY;
+          const float p1 = exp2_(fmaf(s[0][e], a.c, -r4[0][x])), p2 = exp2_(fmaf(s[1][e], a.c, -r4[1][x])) * r4[4][x];
+          w[e] = p1 - p2;
+          s[0][e] = out ? 0.f : p1 * (dp[e] - r4[2][x]);
+          s[1][e] = out ? 0.f : -p2 * (dp[e] - r4[3][x]);
+          top[0] = fmaxf(top[0], fabsf(w[e])), top[1] = fmaxf(top[1], fabsf(s[0][e])), top[2] = fmaxf(top[2], fabsf(s[1][e]));
+        }
+      }
+      sv.template see<VT>(top[0], dv);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        const vec8<T> f = scaled_frag<T>(w, st, sv.mul());
+#pragma unroll
+        for (int x = 0; x < VT; ++x) dv[x] = mfma16(col_frag_acc<T, GR, false>(ot, rb * 32 + 16 * st, x * 32, lane), f, dv[x]);
+      }
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        sk[m].template see<QT>(top[1 + m], dk[m]);
+#pragma unroll
+        for (int st = 0; st < 2; ++st) {
+          const vec8<T> f = scaled_frag<T>(s[m], st, sk[m].mul());
+#pragma unroll
+          for (int x = 0; x < QT; ++x) dk[m][x] = mfma16(col_frag_acc<T, GR, false>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, dk[m][x]);
+        }
+      }
+    }
+  }
+  if (j >= a.Nk) return;           // keys past their sequence's length get zeros
+  const long long at = (((long long)b * a.Nk + j) * a.G + g) * 2 * a.d;
+#pragma unroll
+  for (int x = 0; x < VT; ++x)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const int e = x * 32 + 8 * y + 4 * half;
+      const float f = sv.undo();
+      if (e < 2 * a.d) put4((T*)a.dv + at + e, dv[x][4 * y] * f, dv[x][4 * y + 1] * f, dv[x][4 * y + 2] * f, dv[x][4 * y + 3] * f);
+    }
+#pragma unroll
+  for (int m = 0; m < 2; ++m) {
+    const float f = a.scale * sk[m].undo();
+#pragma unroll
+    for (int x = 0; x < QT; ++x)
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int col = (D >= 32 ? m * D : 0) + x * 32 + 8 * y + 4 * half, w = col % D;
+        if (col / D == m && w < a.d)
+          put4((T*)a.dk + at + m * a.d + w, dk[m][x][4 * y] * f, dk[m][x][4 * y + 1] * f, dk[m][x][4 * y + 2] * f, dk[m][x][4 * y + 3] * f);
+      }
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------------------------------------
+inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+struct Split {
+  int waves, tiles, splits, len;
+};
+// Blocks of 4 waves (128 rows) share keys and values among more rows; blocks of one wave fill the chip where there are few rows.
+// Where even those leave most of it idle, the keys are cut into slices of at least 256.
+Split split_of(const ff3d_diff_attention_t& p) {
+  const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
+  Split s;
+  s.waves = bg * cdiv(R, 128) >= 256 ? 4 : 1;
+  s.tiles = cdiv(R, 32 * s.waves);
+  const long long blocks = bg * s.tiles;
+  long long n = blocks >= 512 ? 1 : cdiv(1024, blocks);
+  n = n < p.Nk / 256 ? n : p.Nk / 256;
+  if (n < 1) n = 1;
+  s.len = (int)((cdiv(p.Nk, n) + 63) / 64 * 64);
+  s.splits = cdiv(p.Nk, s.len);
+  return s;
+}
+
+int check(const ff3d_diff_attention_t* p) {
+  FF3D_REQUIRE(p && p->q && p->k && p->v && p->lam, FF3D_ERR_NULL);
+  FF3D_REQUIRE(p->dtype == FF3D_F32 || p->dtype == FF3D_BF16 || p->dtype == FF3D_F16, FF3D_ERR_BAD_DTYPE);
+  FF3D_REQUIRE(p->B > 0 && p->Nq > 0 && p->Nk > 0 && p->heads > 0 && p->kv_heads > 0 && p->heads % p->kv_heads == 0 && p->scale > 0.f, FF3D_ERR_BAD_SHAPE);
+  FF3D_REQUIRE(p->d == 8 || p->d == 16 || p->d == 32 || p->d == 64, FF3D_ERR_UNSUPPORTED);
+  const long long r = p->heads / p->kv_heads, size = p->dtype == FF3D_F32 ? 4 : 2, per = 16 / size;
+  FF3D_REQUIRE((long long)p->Nq * r < (1ll << 30) && p->Nk < (1 << 30) && (long long)p->B * p->heads < (1ll << 30), FF3D_ERR_BAD_SHAPE);
+  const long long w = 2ll * p->d;
+  FF3D_REQUIRE(p->q_row >= w * p->heads && p->k_row >= w * p->kv_heads && p->v_row >= w * p->kv_heads, FF3D_ERR_BAD_SHAPE);
+  // offsets inside a tile of 128 rows are 31 bits
+  FF3D_REQUIRE(p->q_row * size < (1ll << 24) && p->k_row * size < (1ll << 24) && p->v_row * size < (1ll << 24), FF3D_ERR_BAD_SHAPE);
+  FF3D_REQUIRE(((p->q_batch | p->q_row | p->k_batch | p->k_row | p->v_batch | p->v_row) % per) == 0, FF3D_ERR_ALIGNMENT);
+  FF3D_REQUIRE(ff3d_aligned16(p->q) && ff3d_aligned16(p->k) && ff3d_aligned16(p->v), FF3D_ERR_ALIGNMENT);
+  FF3D_REQUIRE(p->q_batch >= 0 && p->k_batch >= 0 && p->v_batch >= 0 && p->mask_batch >= 0 && p->mask_row >= 0, FF3D_ERR_BAD_SHAPE);
+  return FF3D_OK;
+}
+
+Args args_of(const ff3d_diff_attention_t& p) {
+  Args a = {};
+  a.q = (const char*)p.q, a.k = (const char*)p.k, a.v = (const char*)p.v, a.lam = p.lam, a.mask = p.mask, a.lens = p.kv_lens;
+  a.q_b = p.q_batch, a.q_r = p.q_row, a.k_b = p.k_batch, a.k_r = p.k_row, a.v_b = p.v_batch, a.v_r = p.v_row;
+  a.m_b = p.mask_batch, a.m_r = p.mask_row;
+  a.mask4 = p.mask && ((p.mask_batch | p.mask_row | (long long)reinterpret_cast<uintptr_t>(p.mask)) & 3) == 0;
+  a.B = p.B, a.Nq = p.Nq, a.Nk = p.Nk, a.H = p.heads, a.G = p.kv_heads, a.r = p.heads / p.kv_heads, a.d = p.d, a.causal = p.causal;
+  a.R = a.Nq * a.r, a.Rp = (a.R + 63) / 64 * 64;
+  a.scale = p.scale, a.c = p.scale * LOG2E, a.splits = 1, a.split_len = p.Nk;
+  return a;
+}
+
+template <typename T, int D>
+int fwd(const ff3d_diff_attention_t& p, Args a, hipStream_t st) {
+  const Split s = split_of(p);
+  a.tiles = s.tiles, a.splits = s.splits, a.split_len = s.len;
+  const long long blocks = (long long)a.B * a.G * s.tiles * s.splits;
+  if (blocks > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
+  if (s.waves == 4) fwd_kernel<T, D, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
+  else fwd_kernel<T, D, 1><<<(unsigned)blocks, 64, 0, st>>>(a);
+  if (s.splits > 1) join_kernel<T><<<(unsigned)cdiv((long long)a.B * a.G * a.R, 4), 256, 0, st>>>(a);
+  return ff3d_launch_status();
+}
+
+template <typename T, int D>
+int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
+  const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128), kb = bg * cdiv(a.Nk, 128);
+  if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
+  rows_kernel<T><<<(unsigned)cdiv(rows, 16), 256, 0, st>>>(a);
+  if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
+  if (a.dk) {
+    a.tiles = cdiv(a.Nk, 128);
+    dkv_kernel<T, D><<<(unsigned)kb, 256, 0, st>>>(a);
+  }
+  if (a.dq) {
+    a.tiles = cdiv(a.R, 128);
+    dq_kernel<T, D><<<(unsigned)qb, 256, 0, st>>>(a);
+  }
+  return ff3d_launch_status();
+}
+
+template <typename T>
+int fwd_d(const ff3d_diff_attention_t& p, const Args& a, hipStream_t st) {
+  return p.d <= 16 ? fwd<T, 16>(p, a, st) : p.d == 32 ? fwd<T, 32>(p, a, st) : fwd<T, 64>(p, a, st);
+}
+template <typename T>
+int bwd_d(const ff3d_diff_attention_t& p, const Args& a, void* dlam, hipStream_t st) {
+  return p.d <= 16 ? bwd<T, 16>(p, a, (T*)dlam, st) : p.d == 32 ? bwd<T, 32>(p, a, (T*)dlam, st) : bwd<T, 64>(p, a, (T*)dlam, st);
+}
+
+}  // namespace
+
+extern "C" int64_t ff3d_diff_attention_workspace_bytes(const ff3d_diff_attention_t* p, int backward) {
+  if (!p || p->B <= 0 || p->Nq <= 0 || p->Nk <= 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads) return 0;
+  const long long bg = (long long)p->B * p->kv_heads, R = (long long)p->Nq * (p->heads / p->kv_heads);
+  if (backward) return bg * ROWDATA * ((R + 63) / 64 * 64) * 4;
+  const Split s = split_of(*p);
+  return s.splits > 1 ? (long long)s.splits * bg * R * (4 * p->d + 4) * 4 : 0;
+}
+
+extern "C" int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* lse, void* workspace, ff3d_stream_t stream) {
+  const int s = check(p);
+  if (s != FF3D_OK) return s;
+  FF3D_REQUIRE(out && (!out2 == !lse), FF3D_ERR_NULL);
+  FF3D_REQUIRE(ff3d_aligned16(out) && ff3d_aligned16(out2) && ff3d_aligned16(workspace), FF3D_ERR_ALIGNMENT);
+  FF3D_REQUIRE(workspace || ff3d_diff_attention_workspace_bytes(p, 0) == 0, FF3D_ERR_NULL);
+  ff3d_clear_error();
+  Args a = args_of(*p);
+  a.out = (char*)out, a.out2 = out2, a.lse = lse, a.part = (float*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  return p->dtype == FF3D_F32 ? fwd_d<float>(*p, a, st) : p->dtype == FF3D_BF16 ? fwd_d<__bf16>(*p, a, st) : fwd_d<_Float16>(*p, a, st);
+}
+
+extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* lse, const void* dout,
+                                       int64_t dout_batch, int64_t dout_row, void* dq, void* dk, void* dv, void* dlam, void* workspace,
+                                       ff3d_stream_t stream) {
+  const int s = check(p);
+  if (s != FF3D_OK) return s;
+  FF3D_REQUIRE(out && out2 && lse && dout && workspace && (!dk == !dv), FF3D_ERR_NULL);
+  const long long size = p->dtype == FF3D_F32 ? 4 : 2;
+  FF3D_REQUIRE(dout_row >= 2ll * p->d * p->heads && dout_batch >= 0 && dout_row * size < (1ll << 24), FF3D_ERR_BAD_SHAPE);
+  FF3D_REQUIRE((dout_batch | dout_row) % (16 / size) == 0 && ff3d_aligned16(dout) && ff3d_aligned16(dq) && ff3d_aligned16(dk) && ff3d_aligned16(dv) &&
+                   ff3d_aligned16(workspace),
+               FF3D_ERR_ALIGNMENT);
+  // the row values of one sequence are addressed with 31 bits
+  FF3D_REQUIRE((long long)ROWDATA * 4 * p->Nq * (p->heads / p->kv_heads) < 0x7fff0000ll, FF3D_ERR_BAD_SHAPE);
+  ff3d_clear_error();
+  Args a = args_of(*p);
+  a.out = (char*)const_cast<void*>(out), a.out2 = const_cast<float*>(out2), a.lse = const_cast<float*>(lse);
+  a.dout = (const char*)dout, a.do_b = dout_batch, a.do_r = dout_row, a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dv, a.rowdata = (float*)workspace;
+  hipStream_t st = (hipStream_t)stream;
+  return p->dtype == FF3D_F32 ? bwd_d<float>(*p, a, dlam, st) : p->dtype == FF3D_BF16 ? bwd_d<__bf16>(*p, a, dlam, st) : bwd_d<_Float16>(*p, a, dlam, st);
+}

@@ -1764,14 +1764,17 @@ _DTYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 3}
 _ACTS = {'silu': 0, 'gelu': 1, 'relu': 2, 'sigmoid': 3}
 
 
-def _on_device_of(first):
-    """Decorator: run the wrapper with the device of its first tensor (``first(*args)``) current, as the launch and the stream need."""
+def _on_device_of(name):
+    """Decorator: run the wrapper with the device of its first argument ``name`` (a tensor, or a list of them) current, as the launch and
+    the stream need."""
     def deco(fn):
         @functools.wraps(fn)
         def call(*a, **k):
-            t = first(*a)
+            t = a[0] if a else k.get(name)
+            if isinstance(t, (list, tuple)):
+                t = t[0] if len(t) else None
             if not isinstance(t, torch.Tensor) or not t.is_cuda:
-                raise RuntimeError(f'{fn.__name__}: expected CUDA (HIP) tensors - the HIP decoder path has no CPU fallback')
+                raise RuntimeError(f'{fn.__name__}: {name}: expected CUDA (HIP) tensors - the HIP decoder path has no CPU fallback')
             if t.get_device() == torch._C._cuda_getDevice():
                 return fn(*a, **k)
             with torch.cuda.device(t.device):
@@ -1815,7 +1818,7 @@ def _gated_args(x, weight, bias, act):
     return x2, weight, bias, F2 // 2, C_, pack
 
 
-@_on_device_of(lambda x, *a: x)
+@_on_device_of('x')
 def gated_linear(x, weight, bias=None, act='silu'):
     """h = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel (ff3d_gated_linear_fwd): x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F)
     or None, all fp32, bf16 or fp16 -> (..., F).  act: 'silu', 'gelu' (erf form), 'relu' or 'sigmoid'.  Sums in fp32, one rounding.
@@ -1833,7 +1836,7 @@ def gated_linear(x, weight, bias=None, act='silu'):
     return h
 
 
-@_on_device_of(lambda x, *a: x)
+@_on_device_of('x')
 def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     """Gradients of ``gated_linear`` for dh (..., F) -> (dx, dweight, dbias); None where ``want`` is false (or there is no bias)."""
     x2, weight, bias, F_, C_, pack = _gated_args(x, weight, bias, act)
@@ -1854,6 +1857,114 @@ def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh2.stride(0), _ptr(dx), _ptr(dw), _ptr(db),
                                          M, C_, F_, _ACTS[act], code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
     return dx, dw, db
+
+
+def _attn_rows(t, name, like, B, N, width):
+    """t (B, N, width) of ``like``'s type and device -> itself, or a copy where its rows are not dense, aligned and in range."""
+    _same(t, like, name, (B, N, width))
+    per = 16 // t.element_size()
+    if (t.stride(2) != 1 or t.stride(0) % per or t.stride(1) % per or t.stride(1) < width or t.data_ptr() % 16
+            or t.stride(1) * t.element_size() >= 1 << 24):
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
+def _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale):
+    """Checked arguments -> (struct, the tensors it points to)."""
+    if q.dtype not in _DTYPE:
+        raise RuntimeError(f'diff_attention: expected fp32, bf16 or fp16 tensors, got {q.dtype}')
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f'diff_attention: {heads} heads over {kv_heads} key heads: expected a multiple')
+    if q.dim() != 3 or k.dim() != 3 or q.shape[2] % (2 * heads) or q.shape[2] // (2 * heads) not in (8, 16, 32, 64):
+        raise RuntimeError(f'diff_attention: expected q (B, Nq, heads * 2 d) and k (B, Nk, kv_heads * 2 d) with d = 8, 16, 32 or 64, got '
+                           f'{tuple(q.shape)} and {tuple(k.shape)} for {heads} heads')
+    B, Nq, _ = q.shape
+    Nk, d = k.shape[1], q.shape[2] // (2 * heads)
+    q = _attn_rows(q, 'q', q, B, Nq, heads * 2 * d)
+    k = _attn_rows(k, 'k', q, B, Nk, kv_heads * 2 * d)
+    v = _attn_rows(v, 'v', q, B, Nk, kv_heads * 2 * d)
+    _same(lam, q, 'lam', (heads,))
+    lam = lam.contiguous()
+    mb = mr = 0
+    if mask is not None:
+        if not isinstance(mask, torch.Tensor) or mask.device != q.device or mask.dtype not in (torch.bool, torch.uint8):
+            raise RuntimeError(f'mask: expected a bool or uint8 tensor on {q.device} (True = not attended)')
+        if tuple(mask.shape) not in ((Nq, Nk), (1, Nq, Nk), (B, Nq, Nk)):
+            raise RuntimeError(f'mask: expected shape {(Nq, Nk)} or {(B, Nq, Nk)}, got {tuple(mask.shape)}')
+        mask = (mask if mask.dim() == 3 else mask[None])
+        if Nk > 1 and mask.stride(2) != 1:
+            mask = mask.contiguous()
+        mb, mr = mask.stride(0) if mask.shape[0] > 1 else 0, mask.stride(1)
+    if kv_lens is not None:
+        if not isinstance(kv_lens, torch.Tensor) or kv_lens.device != q.device or kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,):
+            raise RuntimeError(f'kv_lens: expected a ({B},) int32 tensor on {q.device}')
+        kv_lens = kv_lens.contiguous()
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float('inf'):
+        raise ValueError(f'diff_attention: scale {scale}: expected a positive number')
+    keep = (q, k, v, lam, mask, kv_lens)
+    p = _lib.DiffAttention(*[None if t is None else t.data_ptr() for t in keep], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
+                           v.stride(1), mb, mr, B, Nq, Nk, heads, kv_heads, d, 1 if causal else 0, _DTYPE[q.dtype], scale)
+    return p, keep
+
+
+def _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, save):
+    p, keep = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    dev, shape = q.device, q.shape
+    empty = p.B == 0 or p.Nq == 0 or p.Nk == 0
+    new = torch.zeros if empty else torch.empty
+    out = new(shape, dtype=q.dtype, device=dev)
+    out2 = new(shape, device=dev) if save else None
+    lse = new(p.B, p.kv_heads, 2, p.Nq * p.heads // p.kv_heads, device=dev) if save else None
+    if not empty:
+        lib = _lib.load()
+        n = lib.ff3d_diff_attention_workspace_bytes(p, 0)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        _lib.check(lib.ff3d_diff_attention_fwd(p, _ptr(out), _ptr(out2), _ptr(lse), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
+    return out, out2, lse
+
+
+@_on_device_of('q')
+def diff_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
+    """Differential attention (ff3d_diff_attention_fwd): per head softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v.
+
+    q (B, Nq, heads * 2 d) with a head's columns [q1 | q2], k (B, Nk, kv_heads * 2 d) likewise, v (B, Nk, kv_heads * 2 d), lam (heads,), all
+    fp32, bf16 or fp16; d = 8, 16, 32 or 64; heads / kv_heads consecutive heads share a key head -> (B, Nq, heads * 2 d).  Any batch and
+    row strides; rows that are not dense or not 16-byte aligned are copied.
+    mask (Nq, Nk) or (B, Nq, Nk) bool / uint8, True = not attended; kv_lens (B,) int32 on the device: keys from there on are absent and
+    not read; causal: query i attends keys j <= i + Nk - Nq.  A row without keys gives zeros.  scale: d ** -0.5 by default.
+    Keys and values that are read have to be finite.  The differentiable form is ``autograd.differential_attention``."""
+    return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, False)[0]
+
+
+@_on_device_of('q')
+def diff_attention_train_fwd(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
+    """``diff_attention`` -> (out, out2, lse) with what ``diff_attention_bwd`` needs."""
+    return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, True)
+
+
+@_on_device_of('q')
+def diff_attention_bwd(q, k, v, lam, heads, out, out2, lse, dout, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None,
+                       want=(True, True, True, True)):
+    """Gradients of ``diff_attention`` for dout (B, Nq, heads * 2 d) -> (dq, dk, dv, dlam); None where ``want`` is false (dk and dv are
+    computed together)."""
+    p, keep = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    dev, dt = q.device, q.dtype
+    _same(out, q, 'out', q.shape)
+    dout = _attn_rows(dout, 'dout', q, p.B, p.Nq, q.shape[2])
+    empty = p.B == 0 or p.Nq == 0 or p.Nk == 0
+    new = torch.zeros if empty else torch.empty
+    pair = want[1] or want[2]
+    dq = new(q.shape, dtype=dt, device=dev) if want[0] else None
+    dk, dv = (new(k.shape, dtype=dt, device=dev), new(v.shape, dtype=dt, device=dev)) if pair else (None, None)
+    dlam = new(heads, dtype=dt, device=dev) if want[3] else None
+    if not empty and any(want):
+        lib = _lib.load()
+        ws = torch.empty(lib.ff3d_diff_attention_workspace_bytes(p, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.ff3d_diff_attention_bwd(p, _ptr(out), _ptr(out2), _ptr(lse), _ptr(dout), dout.stride(0), dout.stride(1), _ptr(dq), _ptr(dk),
+                                               _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), 'ff3d_diff_attention_bwd')
+    return dq, dk if want[1] else None, dv if want[2] else None, dlam
 
 
 _NORM_KINDS = {2: 2, 1: 1, float('inf'): 0}
@@ -1891,7 +2002,7 @@ def _norm_kind(norm_type):
     return kind
 
 
-@_on_device_of(lambda g, *a, **k: g[0] if len(g) else None)
+@_on_device_of('grads')
 def grad_norm(grads, norm_type=2.0):
     """Norm (2, 1 or inf) over all elements of a list of dense fp32 / bf16 / fp16 tensors of one device -> fp32 scalar on the device
     (ff3d_grad_norm; sums in fp64, no host synchronisation)."""
@@ -1905,7 +2016,7 @@ def grad_norm(grads, norm_type=2.0):
     return norm
 
 
-@_on_device_of(lambda g, *a, **k: g[0] if len(g) else None)
+@_on_device_of('grads')
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """out_i = grads_i * min(1, max_norm / (norm + 1e-6)) with norm = ``grad_norm(grads, norm_type)`` -> norm (ff3d_clip_grads: one
     launch per pass for up to 120 tensors).  ``out``: tensors of the same shapes and layouts (types may differ), disjoint from each

@@ -761,6 +761,40 @@ int ff3d_gated_linear_bwd(const void* x, int64_t ldx, const void* weight, const 
                           void* dw, void* db, int M, int C, int F, int act, int dtype, int pack, void* workspace,
                           ff3d_stream_t stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Differential attention (ABI 2.12), fp32 / bf16 / fp16 (all tensors of one type; sums and softmax statistics in fp32): per head
+ *   out = softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v
+ *   q (B, Nq, heads * 2 d), a head = [q1 | q2];  k (B, Nk, kv_heads * 2 d), [k1 | k2];  v (B, Nk, kv_heads * 2 d);  lam (heads);
+ *   heads / kv_heads consecutive query heads share a key head.  d = 8, 16, 32 or 64; scale > 0.
+ *   Batch and row strides are in elements and multiples of 16 bytes, the columns of a row are dense, bases 16-byte aligned; a batch
+ *   stride may be 0.
+ *   mask: bytes, non-zero = query i does not attend key j, at mask + b * mask_batch + i * mask_row + j, or NULL (a stride may be 0).
+ *   kv_lens (B) int32 on the device: sequence b has min(max(kv_lens[b], 0), Nk) keys, what lies behind is never read; or NULL.
+ *   causal: query i attends keys j <= i + Nk - Nq.
+ *   A row that attends no key gives zeros.  Keys and values that are read have to be finite: a NaN or infinity may reach rows that
+ *   block its key (as 0 * NaN).
+ * ff3d_diff_attention_fwd: out (B, Nq, heads * 2 d) dense; for the backward pass also out2 (the same shape, fp32: the second map's
+ *   softmax times v) and lse (B, kv_heads, 2, Nq * heads / kv_heads) fp32, else both NULL.
+ * ff3d_diff_attention_bwd: dout with its own strides -> dq, (dk, dv) dense in their inputs' shapes, dlam (heads); dq, the pair and
+ *   dlam may be NULL.  Deterministic.  workspace: ff3d_diff_attention_workspace_bytes(p, backward), 16-byte aligned scratch. */
+typedef struct {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* lam;
+  const uint8_t* mask;
+  const int32_t* kv_lens;
+  int64_t q_batch, q_row, k_batch, k_row, v_batch, v_row, mask_batch, mask_row;
+  int32_t B, Nq, Nk, heads, kv_heads, d, causal, dtype;
+  float scale;
+} ff3d_diff_attention_t;
+int64_t ff3d_diff_attention_workspace_bytes(const ff3d_diff_attention_t* p, int backward);
+int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* lse, void* workspace,
+                            ff3d_stream_t stream);
+int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* lse, const void* dout,
+                            int64_t dout_batch, int64_t dout_row, void* dq, void* dk, void* dv, void* dlam, void* workspace,
+                            ff3d_stream_t stream);
+
 /* Norm over all elements of n tensors and clipping by it (ABI 2.12):
  *   norm = (sum |g|^2)^(1/2) (kind 2), sum |g| (kind 1) or max |g| (kind 0), sums in fp64, result fp32 on the device;
  *   out_i = g_i * min(1, max_norm / (norm + 1e-6)), rounded once to the type of out_i.

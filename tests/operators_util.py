@@ -65,3 +65,87 @@ def assert_within(got, want, what=''):
     off = (got.detach().double().reshape(value.shape) - value).abs()
     bad = ~(off <= bound)
     assert not bool(bad.any()), (what, int(bad.sum()), float((off / bound)[bad].max()), float(off[bad].max()))
+
+
+def blocked_pairs(B, Nq, Nk, mask, lens, causal, device):
+    """(B, Nq, Nk) truth values: the pairs that the mask, the lengths or the causal order leave out."""
+    j = torch.arange(Nk, device=device)
+    out = torch.zeros(B, Nq, Nk, dtype=torch.bool, device=device)
+    if mask is not None:
+        out |= (mask != 0)
+    if lens is not None:
+        out |= (j >= lens.clamp(0, Nk)[:, None])[:, None]
+    if causal:
+        out |= j > torch.arange(Nq, device=device)[:, None] + Nk - Nq
+    return out
+
+
+def diff_attention64(q, k, v, lam, heads, kv_heads, blocked, scale=None, dout=None):
+    """[(out, bound)] or with (dq, dk, dv, dlam) too, in fp64, (B, N, C) as the operator lays them out."""
+    dt = q.dtype
+    u, tiny = U[dt], TINY[dt]
+    up = 0.0 if dt == torch.float32 else u                              # rounding of the probabilities, and of dS, to the type
+    low = 2.0 ** -25 if dt == torch.float16 else 0.0                    # what fp16 loses of a probability next to one of 1
+    # the exponential gives zero where its result lies below the smallest normal number of fp32: a probability, which is at most such a
+    # result, is then off by up to 2^-126, and dS and dv by that times their other factors
+    under = 2.0 ** -126
+    B, Nq, Nk, r = q.shape[0], q.shape[1], k.shape[1], heads // kv_heads
+    d = q.shape[2] // (2 * heads)
+    scale = d ** -0.5 if scale is None else scale
+    q_ = q.double().view(B, Nq, heads, 2, d).permute(0, 2, 3, 1, 4)
+    k_ = k.double().view(B, Nk, kv_heads, 2, d).permute(0, 2, 3, 1, 4).repeat_interleave(r, 1)
+    v_ = v.double().view(B, Nk, kv_heads, 2 * d).transpose(1, 2).repeat_interleave(r, 1)
+    lam_ = lam.double().view(1, heads, 1, 1)
+    bl = blocked[:, None, None]
+    k_ = torch.where(k_.isfinite(), k_, 0.0)                            # keys that nobody attends may hold anything
+    v_ = torch.where(v_.isfinite(), v_, 0.0)
+    s = (q_ @ k_.transpose(-1, -2)) * scale
+    es = (d + 16) * E32 * scale * (q_.abs() @ k_.abs().transpose(-1, -2))
+    s = s.masked_fill(bl, -1e300)
+    es, mag = es.masked_fill(bl, 0.0), s.masked_fill(bl, 0.0).abs()
+    p = torch.softmax(s, -1).masked_fill(bl, 0.0)
+    # the exponent, scaled by log2(e) and less the maximum, is off by a few roundings of the scores; so is every term of the sum
+    delta = 2.1 * (es.amax(-1, keepdim=True) * 2 + (mag.amax(-1, keepdim=True) + 8) * 2.0 ** -22) + (Nk + 16) * E32
+    p1, p2, va = p[:, :, 0], p[:, :, 1], v_.abs()
+    d1, d2 = delta[:, :, 0], delta[:, :, 1]
+    some = (~blocked).any(-1)[:, None, :, None].double()
+    lost = (low + under) * some * torch.where(bl[:, :, 0], 0.0, 1.0) @ va
+    o2 = p2 @ v_
+    e1, e2 = (up + d1) * (p1 @ va) + lost, (up + d2) * (p2 @ va) + lost
+    o = p1 @ v_ - lam_ * o2
+    eo = u * o.abs() + 1.02 * (e1 + lam_.abs() * e2) + 4 * E32 * (lam_ * o2).abs() + tiny
+    rows = lambda t: t.transpose(1, 2).reshape(B, Nq, heads * 2 * d)  # noqa: E731
+    out = [(rows(o), rows(eo))]
+    if dout is None:
+        return out
+    do = dout.double().view(B, Nq, heads, 2 * d).transpose(1, 2)
+    da = do.abs()
+    dp, edp = do @ v_.transpose(-1, -2), (2 * d + 16) * E32 * (da @ va.transpose(-1, -2))
+    D2 = (do * o2).sum(-1, keepdim=True)
+    eD2 = (da * (e2 + 2 * d * E32 * o2.abs())).sum(-1, keepdim=True) * 1.02
+    D1 = (do * (o + lam_ * o2)).sum(-1, keepdim=True)
+    eD1 = (da * (eo + 2 * d * E32 * o.abs())).sum(-1, keepdim=True) * 1.02 + lam_.abs() * eD2 + 2 * E32 * (D1.abs() + (lam_ * D2).abs())
+    w = p1 - lam_ * p2
+    ew = (up * w.abs() + 1.02 * (d1 * p1 + d2 * p2 * lam_.abs())) + 2 * E32 * (p1 + p2 * lam_.abs())
+    ew = ew + (under + (2.0 ** -33 if low else 0.0)) * (1 + lam_.abs())
+    ds, eds = [], []
+    for pm, dm, D, eD, f in ((p1, d1, D1, eD1, torch.ones_like(lam_)), (p2, d2, D2, eD2, -lam_)):
+        x = f * pm * (dp - D)
+        e = f.abs() * under * (dp - D).abs() + f.abs() * pm * (1.02 * dm * (dp - D).abs() + edp + eD + 2 * E32 * (dp.abs() + D.abs())) * 1.02 + (up + 4 * E32) * x.abs()
+        if low:                                                         # a column shares one scale: its largest value sets the step
+            e = e + 2.0 ** -32 * torch.maximum(x.abs().amax(-1, keepdim=True), x.abs().amax(-2, keepdim=True))
+        ds.append(x)
+        eds.append(e)
+    group = lambda t: t.view(B, kv_heads, r, Nk, -1).sum(2).transpose(1, 2).reshape(B, Nk, -1)  # noqa: E731
+
+    def product(x, e, y, n, fold, f=1.0):
+        val, bound = fold(x @ y) * f, fold(e @ y.abs() + (n + 16) * E32 * (x.abs() @ y.abs())) * f
+        return val, 1.02 * (u * val.abs() + bound) + tiny
+    dq = [product(ds[m], eds[m], k_[:, :, m], Nk, lambda t: t.transpose(1, 2), scale) for m in range(2)]
+    out.append(tuple(torch.stack([a, b], 3).reshape(B, Nq, -1) for a, b in zip(*dq)))
+    dk = [product(ds[m].transpose(-1, -2), eds[m].transpose(-1, -2), q_[:, :, m], Nq * r, group, scale) for m in range(2)]
+    out.append(tuple(torch.stack([a.view(B, Nk, kv_heads, d), b.view(B, Nk, kv_heads, d)], 3).reshape(B, Nk, -1) for a, b in zip(*dk)))
+    out.append(product(w.transpose(-1, -2), ew.transpose(-1, -2), do, Nq * r, group))
+    dl = -D2.sum((0, 2, 3))
+    out.append((dl, 1.02 * (u * dl.abs() + eD2.sum((0, 2, 3))) + 4 * E32 * D2.abs().sum((0, 2, 3)) + tiny))
+    return out

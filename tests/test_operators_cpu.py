@@ -10,6 +10,7 @@ from focalformer3d_amd import _lib, ops, training
 def test_cpu_tensors_are_refused():
     x, w = torch.zeros(3, 8), torch.zeros(4, 8)
     for call in (lambda: ops.gated_linear(x, w), lambda: ops.gated_linear_bwd(x, w, None, 'silu', torch.zeros(3, 2)), lambda: ops.grad_norm([x]),
+                 lambda: ops.diff_attention(torch.zeros(1, 3, 32), torch.zeros(1, 3, 32), torch.zeros(1, 3, 32), torch.zeros(1), 1),
                  lambda: ops.clip_grads([x], 1.0), lambda: training.clip_grads([], 1.0)):
         with pytest.raises(RuntimeError, match='CUDA'):
             call()
@@ -60,3 +61,35 @@ def test_c_entries_check_their_arguments():
     assert clip(ptrs, None, numel, code, code, 1, 2, 1.0, p, p, None) == -4
     # four elements, one piece, one more for none
     assert lib.ff3d_grad_norm_workspace_bytes((ctypes.c_int64 * 2)(4, 0), 2) == 16
+
+
+def test_diff_attention_entry_checks_its_arguments():
+    lib = _lib.load()
+    P = 4096
+    ok = dict(q=P, k=P, v=P, lam=P, mask=None, kv_lens=None, q_batch=320, q_row=64, k_batch=320, k_row=64, v_batch=320, v_row=64, mask_batch=0, mask_row=0,
+              B=2, Nq=5, Nk=5, heads=2, kv_heads=2, d=16, causal=0, dtype=0, scale=0.25)
+
+    def run(out=P, out2=None, lse=None, ws=None, **k):
+        return lib.ff3d_diff_attention_fwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, ws, None)
+    assert lib.ff3d_diff_attention_fwd(None, P, None, None, None, None) == -4
+    for n in ('q', 'k', 'v', 'lam', 'out'):
+        assert run(**{n: None}) == -4, n
+    assert run(out2=P) == -4 and run(lse=P) == -4
+    assert run(dtype=2) == -2 and run(d=24) == -5
+    for bad in (dict(B=0), dict(Nq=0), dict(Nk=-1), dict(heads=3), dict(kv_heads=0), dict(scale=0.0), dict(scale=float('nan')), dict(q_row=60), dict(k_row=32),
+                dict(q_batch=-320), dict(mask_row=-1), dict(Nk=1 << 30), dict(q_row=1 << 22)):
+        assert run(**bad) == -1, bad
+    for bad in (dict(q=P + 4), dict(q_row=66), dict(v_batch=322), dict(out=P + 8)):
+        assert run(**bad) == -3, bad
+    # few rows over long keys need a place for the slices
+    assert run(Nq=1, Nk=2048, heads=2) == -4
+    p = _lib.DiffAttention(**{**ok, 'Nq': 1, 'Nk': 2048})
+    assert lib.ff3d_diff_attention_workspace_bytes(p, 0) == 8 * 4 * 1 * (4 * 16 + 4) * 4          # 8 slices of 256 keys, 4 rows
+    assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 0) == 0
+    assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 1) == 4 * 5 * 64 * 4  # rows rounded up to 64
+
+    def bwd(out=P, out2=P, lse=P, dout=P, db=320, dr=64, dq=P, dk=P, dv=P, dlam=P, ws=P, **k):
+        return lib.ff3d_diff_attention_bwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, dout, db, dr, dq, dk, dv, dlam, ws, None)
+    for n in ('out', 'out2', 'lse', 'dout', 'ws', 'dk', 'dv'):
+        assert bwd(**{n: None}) == -4, n
+    assert bwd(dr=32) == -1 and bwd(dr=66) == -3 and bwd(dq=P + 4) == -3
