@@ -29,6 +29,9 @@ struct AttnF16Params {
 __device__ __forceinline__ int at_swz(int row) { return (0x78 >> (2 * ((row >> 2) & 3))) & 3; }
 
 __device__ __forceinline__ void at_split(float x, _Float16& hi, _Float16& lo) {
+  // x has to be the same fp32 number in both lines: where it is a product (the pre-scaled query), the compiler may otherwise round the
+  // unrounded product straight to fp16 in one of them (v_fma_mixlo), and hi + lo is off by a step of hi in rare elements
+  asm("" : "+v"(x));
   hi = (_Float16)x;
   lo = (_Float16)((x - (float)hi) * 2048.f);
 }

@@ -237,7 +237,8 @@ __global__ __launch_bounds__(256, 1) void locatt_mfma_kernel(LaParams p) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float pv = sm[u][d][t][r] * inv;
+          float pv = sm[u][d][t][r] * inv;
+          asm("" : "+v"(pv));                            // one fp32 number for both halves of the pair, not rounded to fp16 unrounded
           const _Float16 h = (_Float16)pv;
           ph[u][d][4 * t + r] = h;
           pl[u][d][4 * t + r] = (_Float16)((pv - (float)h) * LA_LO_SCALE);
@@ -305,7 +306,8 @@ __global__ __launch_bounds__(256, 1) void locatt_mfma_kernel(LaParams p) {
       for (int ct = 0; ct < 2; ++ct)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const float v = om[u][ct][r] + ox[u][ct][r] * LA_LO_INV;
+          float v = om[u][ct][r] + ox[u][ct][r] * LA_LO_INV;
+          asm("" : "+v"(v));
           h[4 * ct + r] = (_Float16)v;
           l[4 * ct + r] = (_Float16)((v - (float)h[4 * ct + r]) * LA_LO_SCALE);
         }
