@@ -13,7 +13,8 @@
 // DMA; their transposed reads use ds_read_b64_tr_b16.
 //   forward  one pass with running maximum and sum per map; with few rows the keys are cut into slices that a second kernel joins
 //   dq       columns = queries, loops over keys;  dk / dv  columns = keys, loops over the rows.  No atomics: results do not depend
-//            on timing.  Scores are recomputed from q, k and the saved log-sum-exp.
+//            on timing.  Scores are recomputed from q, k and the saved maximum and sum of each row: the exponent
+//            of a large probability is then near zero and exact, where score - log-sum-exp would lose a digit.
 // fp16: dS of a long row is far below fp16's normal range, so its columns carry a running power-of-two scale (Scaled).
 #include "ff3d_mma.h"
 
@@ -22,7 +23,7 @@ namespace {
 using namespace mma;
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int ROWDATA = 5;        // fp32 values per row of the backward pass: log2-sum-exp 1, 2, D1, D2, lam
+constexpr int ROWDATA = 6;        // fp32 values per row of the backward pass: maximum 1, 2 (in log2 units), D1, D2, 1 / sum 1, lam / sum 2
 
 struct Args {
   const char *q, *k, *v, *dout;
@@ -32,7 +33,7 @@ struct Args {
   long long q_b, q_r, k_b, k_r, v_b, v_r, do_b, do_r;     // elements
   long long m_b, m_r;                                     // bytes
   char *out, *dq, *dk, *dv;
-  float *out2, *lse, *part, *rowdata;
+  float *out2, *stat, *part, *rowdata;
   int B, Nq, Nk, H, G, r, d, R, Rp, causal, mask4, splits, split_len, tiles;
   float scale, c;                 // c = scale * log2(e)
 };
@@ -322,9 +323,11 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
         if (a.out2) put4(a.out2 + at * 2 * a.d + e, z[0], z[1], z[2], z[3]);
       }
     }
-  if (a.lse && half == 0)
+  if (a.stat && half == 0) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) a.lse[((long long)bg * 2 + m) * a.R + row] = l[m] == 0.f ? INFINITY : mx[m] * a.c + log2f(l[m]);
+    for (int m = 0; m < 2; ++m) a.stat[((long long)bg * 4 + m) * a.R + row] = mx[m] == -INFINITY ? 0.f : mx[m] * a.c;
+    a.stat[((long long)bg * 4 + 2) * a.R + row] = i0, a.stat[((long long)bg * 4 + 3) * a.R + row] = i1;
+  }
 }
 
 // joins the slices of the keys: one wave per row
@@ -363,11 +366,16 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
       ((T*)a.out)[to + lane + 64 * k] = from_f<T>(o[0][k] * i0 - lam * z);
       if (a.out2) a.out2[to + lane + 64 * k] = z;
     }
-  if (a.lse && lane < 2) a.lse[((long long)bg * 2 + lane) * a.R + row] = l[lane] == 0.f ? INFINITY : top[lane] + log2f(l[lane]);
+  if (a.stat && lane == 0) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) a.stat[((long long)bg * 4 + m) * a.R + row] = top[m] == -INFINITY ? 0.f : top[m];
+    a.stat[((long long)bg * 4 + 2) * a.R + row] = i0, a.stat[((long long)bg * 4 + 3) * a.R + row] = i1;
+  }
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------
-// rowdata (B G, ROWDATA, Rp): log2-sum-exps, D1 = <dO, out> + lam D2, D2 = <dO, O2>, lam; zeros behind R.  16 lanes per row.
+// rowdata (B G, ROWDATA, Rp): maxima, D1 = <dO, out> + lam D2, D2 = <dO, O2>, 1 / sum 1, lam / sum 2; zeros behind R, whose
+// probabilities are therefore 0.  16 lanes per row.
 template <typename T>
 __global__ __launch_bounds__(256) void rows_kernel(Args a) {
   const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
@@ -387,8 +395,8 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
 #pragma unroll
     for (int x = 8; x > 0; x >>= 1) d += __shfl_xor(d, x), d2 += __shfl_xor(d2, x);
     const float lam = to_f(((const T*)a.lam)[h]);
-    v[0] = a.lse[((long long)bg * 2) * a.R + row], v[1] = a.lse[((long long)bg * 2 + 1) * a.R + row];
-    v[2] = fmaf(lam, d2, d), v[3] = d2, v[4] = lam;
+    const float* st = a.stat + (long long)bg * 4 * a.R + row;
+    v[0] = st[0], v[1] = st[a.R], v[2] = fmaf(lam, d2, d), v[3] = d2, v[4] = st[2ll * a.R], v[5] = lam * st[3ll * a.R];
   }
   if (lane == 0)
 #pragma unroll
@@ -499,9 +507,8 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
       for (int m = 0; m < 2; ++m)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const float pr = exp2_(fmaf(s[m][e], a.c, -rd[m]));
-          float ds = pr * (dp[e] - rd[2 + m]);
-          if (m == 1) ds *= -rd[4];
+          // 1 / sum and -lam are factors of the whole column: they wait for the end
+          float ds = exp2_(fmaf(s[m][e], a.c, -rd[m])) * (dp[e] - rd[2 + m]);
           if (some && s[m][e] == -INFINITY) ds = 0.f;
           s[m][e] = ds;
           top[m] = fmaxf(top[m], fabsf(ds));
@@ -523,7 +530,7 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
   T* out = (T*)a.dq + (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float f = a.scale * sc[m].undo();
+    const float f = a.scale * (m == 0 ? rd[4] : -rd[5]) * sc[m].undo();
 #pragma unroll
     for (int x = 0; x < QT; ++x)
 #pragma unroll
@@ -630,7 +637,7 @@ __global__ __launch_bounds__(256) void dkv_kernel(Args a) {
         for (int x = 0; x < 4; ++x) {
           const int e = 4 * y + x;
           const bool out = some && s[0][e] == -INFINITY && s[1][e] == -INFINITY;
-          const float p1 = exp2_(fmaf(s[0][e], a.c, -r4[0][x])), p2 = exp2_(fmaf(s[1][e], a.c, -r4[1][x])) * r4[4][x];
+          const float p1 = exp2_(fmaf(s[0][e], a.c, -r4[0][x])) * r4[4][x], p2 = exp2_(fmaf(s[1][e], a.c, -r4[1][x])) * r4[5][x];
           w[e] = p1 - p2;
           s[0][e] = out ? 0.f : p1 * (dp[e] - r4[2][x]);
           s[1][e] = out ? 0.f : -p2 * (dp[e] - r4[3][x]);
@@ -779,25 +786,25 @@ extern "C" int64_t ff3d_diff_attention_workspace_bytes(const ff3d_diff_attention
   return s.splits > 1 ? (long long)s.splits * bg * R * (4 * p->d + 4) * 4 : 0;
 }
 
-extern "C" int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* lse, void* workspace, ff3d_stream_t stream) {
+extern "C" int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* stat, void* workspace, ff3d_stream_t stream) {
   const int s = check(p);
   if (s != FF3D_OK) return s;
-  FF3D_REQUIRE(out && (!out2 == !lse), FF3D_ERR_NULL);
+  FF3D_REQUIRE(out && (!out2 == !stat), FF3D_ERR_NULL);
   FF3D_REQUIRE(ff3d_aligned16(out) && ff3d_aligned16(out2) && ff3d_aligned16(workspace), FF3D_ERR_ALIGNMENT);
   FF3D_REQUIRE(workspace || ff3d_diff_attention_workspace_bytes(p, 0) == 0, FF3D_ERR_NULL);
   ff3d_clear_error();
   Args a = args_of(*p);
-  a.out = (char*)out, a.out2 = out2, a.lse = lse, a.part = (float*)workspace;
+  a.out = (char*)out, a.out2 = out2, a.stat = stat, a.part = (float*)workspace;
   hipStream_t st = (hipStream_t)stream;
   return p->dtype == FF3D_F32 ? fwd_d<float>(*p, a, st) : p->dtype == FF3D_BF16 ? fwd_d<__bf16>(*p, a, st) : fwd_d<_Float16>(*p, a, st);
 }
 
-extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* lse, const void* dout,
+extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* stat, const void* dout,
                                        int64_t dout_batch, int64_t dout_row, void* dq, void* dk, void* dv, void* dlam, void* workspace,
                                        ff3d_stream_t stream) {
   const int s = check(p);
   if (s != FF3D_OK) return s;
-  FF3D_REQUIRE(out && out2 && lse && dout && workspace && (!dk == !dv), FF3D_ERR_NULL);
+  FF3D_REQUIRE(out && out2 && stat && dout && workspace && (!dk == !dv), FF3D_ERR_NULL);
   const long long size = p->dtype == FF3D_F32 ? 4 : 2;
   FF3D_REQUIRE(dout_row >= 2ll * p->d * p->heads && dout_batch >= 0 && dout_row * size < (1ll << 24), FF3D_ERR_BAD_SHAPE);
   FF3D_REQUIRE((dout_batch | dout_row) % (16 / size) == 0 && ff3d_aligned16(dout) && ff3d_aligned16(dq) && ff3d_aligned16(dk) && ff3d_aligned16(dv) &&
@@ -807,7 +814,7 @@ extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const voi
   FF3D_REQUIRE((long long)ROWDATA * 4 * p->Nq * (p->heads / p->kv_heads) < 0x7fff0000ll, FF3D_ERR_BAD_SHAPE);
   ff3d_clear_error();
   Args a = args_of(*p);
-  a.out = (char*)const_cast<void*>(out), a.out2 = const_cast<float*>(out2), a.lse = const_cast<float*>(lse);
+  a.out = (char*)const_cast<void*>(out), a.out2 = const_cast<float*>(out2), a.stat = const_cast<float*>(stat);
   a.dout = (const char*)dout, a.do_b = dout_batch, a.do_r = dout_row, a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dv, a.rowdata = (float*)workspace;
   hipStream_t st = (hipStream_t)stream;
   return p->dtype == FF3D_F32 ? bwd_d<float>(*p, a, dlam, st) : p->dtype == FF3D_BF16 ? bwd_d<__bf16>(*p, a, dlam, st) : bwd_d<_Float16>(*p, a, dlam, st);

@@ -186,23 +186,30 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
       A.stage(nxt, wave, kn - (t + 1) * BK);
       B.stage(nxt + ABYTES, wave, kn - (t + 1) * BK);
     }
-#pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      vec8<T> fa[TM], fb[TN];
+    // operands of step s + 1 are read while the matrix unit works on step s
+    vec8<T> fa[2][TM], fb[2][TN];
+    auto read = [&](int s) {
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        if constexpr (AROW) fa[j] = row_frag<T, 8>(cur, (wm * TM + j) * 32 + (lane & 31), 16 * s, half);
-        else fa[j] = col_frag<T, BM / P, true>(cur, 16 * s, (wm * TM + j) * 32, lane);
+        if constexpr (AROW) fa[s & 1][j] = row_frag<T, 8>(cur, (wm * TM + j) * 32 + (lane & 31), 16 * s, half);
+        else fa[s & 1][j] = col_frag<T, BM / P, true>(cur, 16 * s, (wm * TM + j) * 32, lane);
       }
 #pragma unroll
       for (int i = 0; i < TN; ++i) {
-        if constexpr (BROW) fb[i] = row_frag<T, 8>(cur + ABYTES, (wn * TN + i) * 32 + (lane & 31), 16 * s, half);
-        else fb[i] = col_frag<T, BN / P, true>(cur + ABYTES, 16 * s, (wn * TN + i) * 32, lane);
+        if constexpr (BROW) fb[s & 1][i] = row_frag<T, 8>(cur + ABYTES, (wn * TN + i) * 32 + (lane & 31), 16 * s, half);
+        else fb[s & 1][i] = col_frag<T, BN / P, true>(cur + ABYTES, 16 * s, (wn * TN + i) * 32, lane);
       }
+    };
+    read(0);
+#pragma unroll
+    for (int s = 0; s < STEPS; ++s) {
+      if (s + 1 < STEPS) read(s + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = mfma16(fb[i], fa[j], acc[i][j]);
+        for (int j = 0; j < TM; ++j) acc[i][j] = mfma16(fb[s & 1][i], fa[s & 1][j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 

@@ -338,7 +338,8 @@ class FocalDecoder(nn.Module):
         for m in self.modules():               # per module, not process-wide: two heads may run different modes
             if isinstance(m, _transformer.MultiheadAttention):
                 m.attn_f16x3 = mode == 'f16x3'
-            if isinstance(m, (_transformer.MultiheadAttention, _transformer.MultiScaleDeformableAttention, _transformer.FFN)):
+            if isinstance(m, (_transformer.MultiheadAttention, _transformer.DifferentialAttention, _transformer.MultiScaleDeformableAttention,
+                              _transformer.FFN, _transformer.GatedFFN)):
                 m.lin_f16x3 = mode == 'f16x3'
         self.invalidate_cache()
 

@@ -1916,13 +1916,13 @@ def _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, sc
     new = torch.zeros if empty else torch.empty
     out = new(shape, dtype=q.dtype, device=dev)
     out2 = new(shape, device=dev) if save else None
-    lse = new(p.B, p.kv_heads, 2, p.Nq * p.heads // p.kv_heads, device=dev) if save else None
+    stat = new(p.B, p.kv_heads, 4, p.Nq * p.heads // p.kv_heads, device=dev) if save else None
     if not empty:
         lib = _lib.load()
         n = lib.ff3d_diff_attention_workspace_bytes(p, 0)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.check(lib.ff3d_diff_attention_fwd(p, _ptr(out), _ptr(out2), _ptr(lse), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
-    return out, out2, lse
+        _lib.check(lib.ff3d_diff_attention_fwd(p, _ptr(out), _ptr(out2), _ptr(stat), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
+    return out, out2, stat
 
 
 @_on_device_of('q')
@@ -1940,12 +1940,12 @@ def diff_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, 
 
 @_on_device_of('q')
 def diff_attention_train_fwd(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
-    """``diff_attention`` -> (out, out2, lse) with what ``diff_attention_bwd`` needs."""
+    """``diff_attention`` -> (out, out2, stat) with what ``diff_attention_bwd`` needs."""
     return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, True)
 
 
 @_on_device_of('q')
-def diff_attention_bwd(q, k, v, lam, heads, out, out2, lse, dout, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None,
+def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None,
                        want=(True, True, True, True)):
     """Gradients of ``diff_attention`` for dout (B, Nq, heads * 2 d) -> (dq, dk, dv, dlam); None where ``want`` is false (dk and dv are
     computed together)."""
@@ -1962,7 +1962,7 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, lse, dout, kv_heads=None,
     if not empty and any(want):
         lib = _lib.load()
         ws = torch.empty(lib.ff3d_diff_attention_workspace_bytes(p, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.ff3d_diff_attention_bwd(p, _ptr(out), _ptr(out2), _ptr(lse), _ptr(dout), dout.stride(0), dout.stride(1), _ptr(dq), _ptr(dk),
+        _lib.check(lib.ff3d_diff_attention_bwd(p, _ptr(out), _ptr(out2), _ptr(stat), _ptr(dout), dout.stride(0), dout.stride(1), _ptr(dq), _ptr(dk),
                                                _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), 'ff3d_diff_attention_bwd')
     return dq, dk if want[1] else None, dv if want[2] else None, dlam
 

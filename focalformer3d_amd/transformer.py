@@ -207,6 +207,30 @@ def _per_level_ref(reference_points, num_levels):
     return reference_points
 
 
+def _frame_mask(attn_mask, B, heads, N):
+    """An attention mask as nn.MultiheadAttention takes it - (N, N), (B, N, N) or (B*heads, N, N), True / negative = blocked - as one
+    (B, N, N) boolean mask per frame, or None."""
+    if attn_mask is None:
+        return None
+    if attn_mask.dtype != torch.bool:
+        attn_mask = attn_mask < 0                           # additive float form: -inf = blocked
+    if attn_mask.dim() == 2:
+        return attn_mask[None].expand(B, -1, -1)
+    if attn_mask.shape[0] == B and heads > 1:               # one mask per frame (what train_forward.py passes): used as it is
+        return attn_mask
+    m4 = attn_mask.reshape(B, heads, N, N)                  # (B*heads, N, N): FD:856 repeats one mask per frame over the heads
+    # a per-head mask is not supported by the kernel.  The check costs a B*heads*N*N compare and a host sync, so
+    # it runs once per mask tensor (the six layers of a step share one), not once per layer; a mask that is a
+    # broadcast view over the heads (stride 0) needs no check at all
+    # (the verdict rides on the tensor OBJECT together with the version it was reached at - a (data_ptr, _version)
+    #  key in a module global could be matched by a NEW mask the allocator placed at the same address)
+    if heads > 1 and m4.stride(1) != 0 and getattr(attn_mask, '_ff3d_head_uniform', None) != attn_mask._version:
+        if not bool((m4 == m4[:, :1]).all()):
+            raise NotImplementedError('per-head attention masks (FocalFormer3D builds one mask per frame)')
+        attn_mask._ff3d_head_uniform = attn_mask._version
+    return m4[:, 0]
+
+
 @register(ATTENTION)
 class MultiheadAttention(nn.Module):
     """mmcv ``MultiheadAttention``: wraps ``nn.MultiheadAttention`` (parameters under ``.attn``), adds the
@@ -268,26 +292,7 @@ class MultiheadAttention(nn.Module):
             w, b = a.in_proj_weight, a.in_proj_bias
             qk = F.linear(xp, w[:2 * C], None if b is None else b[:2 * C])
             v = F.linear(x, w[2 * C:], None if b is None else b[2 * C:])
-            mask = None
-            if attn_mask is not None:
-                if attn_mask.dtype != torch.bool:
-                    attn_mask = attn_mask < 0                       # additive float form: -inf = blocked
-                if attn_mask.dim() == 2:
-                    mask = attn_mask[None].expand(B, -1, -1)
-                elif attn_mask.shape[0] == B and heads > 1:         # one mask per frame (what train_forward.py passes): used as it is
-                    mask = attn_mask
-                else:                                               # (B*heads, N, N): FD:856 repeats one mask per frame over the heads
-                    m4 = attn_mask.reshape(B, heads, N, N)
-                    mask = m4[:, 0]
-                    # a per-head mask is not supported by the kernel.  The check costs a B*heads*N*N compare and a host sync, so
-                    # it runs once per mask tensor (the six layers of a step share one), not once per layer; a mask that is a
-                    # broadcast view over the heads (stride 0) needs no check at all
-                    # (the verdict rides on the tensor OBJECT together with the version it was reached at - a (data_ptr, _version)
-                    #  key in a module global could be matched by a NEW mask the allocator placed at the same address)
-                    if heads > 1 and m4.stride(1) != 0 and getattr(attn_mask, '_ff3d_head_uniform', None) != attn_mask._version:
-                        if not bool((m4 == m4[:, :1]).all()):
-                            raise NotImplementedError('per-head attention masks (FocalFormer3D builds one mask per frame)')
-                        attn_mask._ff3d_head_uniform = attn_mask._version
+            mask = _frame_mask(attn_mask, B, heads, N)
             p_drop = a.dropout if a.training else 0.0           # (nn.MultiheadAttention's own flag, as its forward uses it)
             o = MaskedSelfAttentionFunction.apply(qk[..., :C], qk[..., C:], v, heads, mask, p_drop)
             out = F.linear(o, a.out_proj.weight, a.out_proj.bias)
@@ -321,6 +326,89 @@ class MultiheadAttention(nn.Module):
             return self.forward_bf(query, query_pos, attn_mask)
         out = self.forward_bf(query.transpose(0, 1).contiguous(),
                               None if query_pos is None else query_pos.transpose(0, 1).contiguous(), attn_mask)
+        return out.transpose(0, 1)
+
+
+@register(ATTENTION)
+class DifferentialAttention(nn.Module):
+    """Self-attention whose weights are the difference of two softmax maps, in the place and with the calling conventions of
+    ``MultiheadAttention`` (``attn_cfgs=[dict(type='DifferentialAttention', embed_dims=..., num_heads=...), ...]``):
+
+        identity + out_proj(concat_h (1 - lambda_init) * RMSNorm(softmax(q1 k1^T / sqrt(d)) v - lam softmax(q2 k2^T / sqrt(d)) v))
+        lam = exp(<lambda_q1, lambda_k1>) - exp(<lambda_q2, lambda_k2>) + lambda_init
+
+    with q = k = x + pos, v = x projected to ``num_heads`` heads of 2 d columns ([map 1 | map 2] of q and k) and to ``kv_heads`` (default:
+    as many) heads of k and v; d = embed_dims / num_heads / 2 is 8, 16, 32 or 64.  The core is ``ops.diff_attention`` (evaluation) /
+    ``autograd.differential_attention`` (training), fp32 or 16-bit as the input is.  Attention masks: one per frame, True / negative =
+    blocked; ``key_padding_mask`` (B, N), True = no key.  There is no dropout on the attention weights."""
+
+    def __init__(self, embed_dims, num_heads, kv_heads=None, lambda_init=0.8, eps=1e-5, attn_drop=0., proj_drop=0.,
+                 dropout_layer=dict(type='Dropout', drop_prob=0.), init_cfg=None, batch_first=False, **kwargs):
+        super().__init__()
+        dropout_layer = dict(dropout_layer) if dropout_layer else None
+        if 'dropout' in kwargs:                            # the decoder configs' spelling: the output dropout
+            dropout_layer = dict(type='Dropout', drop_prob=kwargs.pop('dropout'))
+        if attn_drop:
+            raise NotImplementedError('DifferentialAttention has no dropout on its attention weights (attn_drop)')
+        if dropout_layer and dropout_layer.get('type', 'Dropout') != 'Dropout':
+            raise NotImplementedError("dropout_layer: only type='Dropout'")
+        kv_heads = num_heads if kv_heads is None else kv_heads
+        d = embed_dims // (2 * num_heads)
+        if embed_dims != 2 * d * num_heads or d not in (8, 16, 32, 64) or kv_heads < 1 or num_heads % kv_heads:
+            raise ValueError(f'DifferentialAttention: embed_dims {embed_dims}, {num_heads} heads over {kv_heads}: expected heads of '
+                             '16, 32, 64 or 128 columns and a multiple of kv_heads')
+        self.embed_dims, self.num_heads, self.kv_heads, self.batch_first = embed_dims, num_heads, kv_heads, batch_first
+        self.lambda_init, self.eps = float(lambda_init), float(eps)
+        self.q_proj = nn.Linear(embed_dims, embed_dims)
+        self.k_proj = nn.Linear(embed_dims, kv_heads * 2 * d)
+        self.v_proj = nn.Linear(embed_dims, kv_heads * 2 * d)
+        self.out_proj = nn.Linear(embed_dims, embed_dims)
+        self.lambda_q1, self.lambda_k1, self.lambda_q2, self.lambda_k2 = (nn.Parameter(torch.randn(d) * 0.1) for _ in range(4))
+        self.head_norm = nn.Parameter(torch.ones(2 * d))
+        self.proj_drop = nn.Dropout(proj_drop)
+        self.dropout_layer = nn.Dropout(dropout_layer.get('drop_prob', 0.)) if dropout_layer else nn.Identity()
+
+    def invalidate_cache(self):
+        for name in ('_bf16_w', '_bf16_rows_w', '_f16_w'):
+            self.__dict__.pop(name, None)
+
+    def _project(self, x, linear):
+        if x.dtype != torch.float32 or torch.is_grad_enabled() or not x.is_contiguous():
+            return F.linear(x, linear.weight, linear.bias)
+        return _lin(self, x, linear.weight, linear.bias)
+
+    def lam(self):
+        """The weight of the second map, (num_heads,) - one value per layer, shared by its heads."""
+        a = torch.exp((self.lambda_q1.float() * self.lambda_k1.float()).sum())
+        b = torch.exp((self.lambda_q2.float() * self.lambda_k2.float()).sum())
+        return (a - b + self.lambda_init).to(self.lambda_q1.dtype).expand(self.num_heads)
+
+    def forward_bf(self, x, pos=None, attn_mask=None, key_padding_mask=None):
+        """x, pos (B, N, C) -> (B, N, C)."""
+        from .autograd import differential_attention
+        B, N, C = x.shape
+        xp = x if pos is None else x + pos
+        mask = _frame_mask(attn_mask, B, self.num_heads, N)
+        if key_padding_mask is not None:
+            pad = key_padding_mask.bool()[:, None, :].expand(B, N, N)
+            mask = pad if mask is None else mask | pad
+        o = differential_attention(self._project(xp, self.q_proj), self._project(xp, self.k_proj), self._project(x, self.v_proj), self.lam(),
+                                   self.num_heads, kv_heads=self.kv_heads, mask=mask)
+        heads = o.view(B, N, self.num_heads, -1)
+        o = F.rms_norm(heads, heads.shape[-1:], self.head_norm, self.eps) * (1.0 - self.lambda_init)
+        out = self._project(o.reshape(B, N, C), self.out_proj)
+        return x + self.dropout_layer(self.proj_drop(out))
+
+    def forward(self, query, key=None, value=None, identity=None, query_pos=None, key_pos=None, attn_mask=None,
+                key_padding_mask=None, **kwargs):
+        if (key is not None and key is not query) or (value is not None and value is not query) or identity is not None:
+            raise NotImplementedError("only the self-attention use of the decoder layer is implemented (operation 'self_attn')")
+        if key_pos is not None and key_pos is not query_pos:
+            raise NotImplementedError('key_pos must equal query_pos for self-attention')
+        if self.batch_first:
+            return self.forward_bf(query, query_pos, attn_mask, key_padding_mask)
+        out = self.forward_bf(query.transpose(0, 1).contiguous(),
+                              None if query_pos is None else query_pos.transpose(0, 1).contiguous(), attn_mask, key_padding_mask)
         return out.transpose(0, 1)
 
 
@@ -608,6 +696,61 @@ class FFN(nn.Module):
 
     def forward(self, x, identity=None):
         y = self.layers(x) if self.training else self.delta(x)      # training: Linear / ReLU / Dropout modules under autograd
+        if not self.add_identity:
+            return y
+        return (x if identity is None else identity) + y
+
+
+@register(FEEDFORWARD_NETWORK)
+class GatedFFN(nn.Module):
+    """Gated feed-forward step in the place of ``FFN`` (``ffn_cfgs=dict(type='GatedFFN', feedforward_channels=..., ...)``):
+    identity + fc_out(act(fc_g(x)) * fc_u(x)), both inner projections, the activation and the product in one kernel
+    (``ops.gated_linear`` / ``autograd.gated_linear``).  ``in_proj`` holds the gate's rows, then the value's.
+    act_cfg type: SiLU (default), GELU, ReLU or Sigmoid."""
+
+    def __init__(self, embed_dims=256, feedforward_channels=1024, num_fcs=2, act_cfg=dict(type='SiLU'), ffn_drop=0., dropout_layer=None,
+                 add_identity=True, init_cfg=None, **kwargs):
+        super().__init__()
+        if num_fcs != 2:
+            raise NotImplementedError('GatedFFN: one gated projection and one output projection (num_fcs=2)')
+        self.act = act_cfg.get('type', 'SiLU').lower()
+        if self.act not in ops._ACTS:
+            raise NotImplementedError(f"act_cfg: type {act_cfg.get('type')!r} (SiLU, GELU, ReLU or Sigmoid)")
+        self.embed_dims, self.feedforward_channels, self.add_identity = embed_dims, feedforward_channels, add_identity
+        self.in_proj = nn.Linear(embed_dims, 2 * feedforward_channels)
+        self.out_proj = nn.Linear(feedforward_channels, embed_dims)
+        self.drop = nn.Dropout(ffn_drop)
+
+    def invalidate_cache(self):
+        for name in ('_bf16_w', '_bf16_rows_w', '_f16_w', '_f16_tiled', '_f16_wk'):
+            self.__dict__.pop(name, None)
+
+    def hidden(self, x):
+        """Everything before the last Linear -> (hidden activation, last Linear)."""
+        w, b = self.in_proj.weight, self.in_proj.bias
+        if torch.is_grad_enabled():
+            from .autograd import gated_linear
+            return gated_linear(x, w, b, self.act), self.out_proj
+        if x.dtype == torch.float32 and getattr(self, 'gemm_dtype', torch.float32) == torch.bfloat16:
+            # bf16 mode: operands on the bf16 matrix cores, fp32 rows out
+            w16, b16 = _cached(self, '_bf16_w', w, b, lambda: (w.detach().to(torch.bfloat16), b.detach().to(torch.bfloat16)))
+            return ops.gated_linear(x.to(torch.bfloat16), w16, b16, self.act).float(), self.out_proj
+        return ops.gated_linear(x, w.detach(), b.detach(), self.act), self.out_proj
+
+    def delta(self, x):
+        y, last = self.hidden(x)
+        return _lin(self, y, last.weight, last.bias) if y.dtype == torch.float32 else F.linear(y, last.weight, last.bias)
+
+    def fused_add_ln(self, x, norm, pos=None):
+        """There is no one-launch form: the caller runs the projection and the fused add + LayerNorm."""
+        return None
+
+    def forward(self, x, identity=None):
+        if self.training or torch.is_grad_enabled():
+            y, last = self.hidden(x)
+            y = self.drop(last(self.drop(y)))
+        else:
+            y = self.delta(x)
         if not self.add_identity:
             return y
         return (x if identity is None else identity) + y
