@@ -23,7 +23,9 @@ namespace {
 using namespace mma;
 
 constexpr float LOG2E = 1.4426950408889634f;
-constexpr int ROWDATA = 6;        // fp32 values per row of the backward pass: maximum 1, 2 (in log2 units), D1, D2, 1 / sum 1, lam / sum 2
+constexpr int JOIN = 1024;         // most slices of the keys
+constexpr float SLACK = 8.f;      // 2^8 above the largest term: far inside fp16's range for the rounded probabilities
+constexpr int ROWDATA = 6;        // fp32 values per row of the backward pass: reference 1, 2 of the exponentials (log2 units), D1, D2, 1 / sum 1, lam / sum 2
 
 struct Args {
   const char *q, *k, *v, *dout;
@@ -183,9 +185,12 @@ __device__ __forceinline__ f32x16 scores(const char* tile, int kb, int map, cons
   return s;
 }
 
+// waves per SIMD that the registers are cut for: 2 where they fit (two waves hide each other's waits)
+constexpr int waves_of(int D, int size, bool fits64) { return D <= 32 || (size == 2 && fits64) ? 2 : 1; }
+
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
+__global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_kernel(Args a) {
   constexpr int NT = NW * 64, KT = (sizeof(T) == 2 && NW > 1) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
   constexpr int VT = 2 * D / 32, ST = D / 16;
   __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
@@ -224,7 +229,7 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int t = 0; t < VT; ++t) o[m][t] = (f32x16)(0.f);
-  float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
 
   const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
   const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
@@ -260,21 +265,24 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
         float x = s[m][0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) x = fmaxf(x, s[m][e]);
-        x = fmaxf(x, __shfl_xor(x, 32));
-        const float mn = fmaxf(mx[m], x), base = mn == -INFINITY ? 0.f : mn * a.c;
-        const float alpha = exp2_(mx[m] * a.c - base);
-        mx[m] = mn;
+        x = fmaxf(x, __shfl_xor(x, 32)) * a.c;
+        // the reference of the exponentials follows the maximum only when it lies 2^SLACK behind: what is kept in fp32 does not care,
+        // and the 2 D / 32 accumulators are rescaled a few times per row instead of at most steps
+        if (__any(x > ref[m] + SLACK)) {
+          const float n = fmaxf(ref[m], x), f = exp2_(ref[m] - (n == -INFINITY ? 0.f : n));
+          ref[m] = n;
+          l[m] *= f;
+#pragma unroll
+          for (int v = 0; v < VT; ++v) o[m][v] *= f;
+        }
+        const float base = ref[m] == -INFINITY ? 0.f : ref[m];
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           s[m][e] = exp2_(fmaf(s[m][e], a.c, -base));
           sum += s[m][e];
         }
-        l[m] = fmaf(l[m], alpha, sum);
-        if (__any(alpha != 1.f)) {
-#pragma unroll
-          for (int v = 0; v < VT; ++v) o[m][v] *= alpha;
-        }
+        l[m] += sum;
         p[m][0] = acc_frag<T>(s[m], 0);
         p[m][1] = acc_frag<T>(s[m], 1);
       }
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int v = 0; v < VT; ++v) {
-          const vec8<T> f = col_frag_acc<T, GR, false>(vt, kb * 32 + 16 * st, v * 32, lane);
+          const vec8<T> f = col_frag_acc<T, GR>(vt, kb * 32 + 16 * st, v * 32, lane);
           o[0][v] = mfma16(f, p[0][st], o[0][v]);
           o[1][v] = mfma16(f, p[1][st], o[1][v]);
         }
@@ -295,7 +303,7 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
     float* p = a.part + (((long long)split * a.B * a.G + bg) * a.R + row) * (4 * a.d + 4);
     if (half == 0)
 #pragma unroll
-      for (int m = 0; m < 2; ++m) p[4 * a.d + 2 * m] = mx[m] == -INFINITY ? -INFINITY : mx[m] * a.c, p[4 * a.d + 2 * m + 1] = l[m];
+      for (int m = 0; m < 2; ++m) p[4 * a.d + 2 * m] = ref[m], p[4 * a.d + 2 * m + 1] = l[m];
     if (l[0] == 0.f && l[1] == 0.f) return;
 #pragma unroll
     for (int m = 0; m < 2; ++m)
@@ -325,51 +333,57 @@ __global__ __launch_bounds__(NW * 64) void fwd_kernel(Args a) {
     }
   if (a.stat && half == 0) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m) a.stat[((long long)bg * 4 + m) * a.R + row] = mx[m] == -INFINITY ? 0.f : mx[m] * a.c;
+    for (int m = 0; m < 2; ++m) a.stat[((long long)bg * 4 + m) * a.R + row] = ref[m] == -INFINITY ? 0.f : ref[m];
     a.stat[((long long)bg * 4 + 2) * a.R + row] = i0, a.stat[((long long)bg * 4 + 3) * a.R + row] = i1;
   }
 }
 
-// joins the slices of the keys: one wave per row
+// joins the slices of the keys: one block per row; 4 d threads per group sum one element of O1 or O2 each over the group's slices
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(Args a) {
-  const int lane = threadIdx.x & 63;
-  const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (at >= (long long)a.B * a.G * a.R) return;
-  const int bg = (int)(at / a.R), row = (int)(at % a.R), b = bg / a.G, g = bg % a.G, i = row / a.r, h = g * a.r + row % a.r;
-  const long long step = (long long)a.B * a.G * a.R * (4 * a.d + 4);
-  const float* p = a.part + at * (4 * a.d + 4);
-  float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s)
+  __shared__ float wt[2][JOIN], sum[256], norm[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int bg = blockIdx.x / a.R, row = blockIdx.x % a.R, b = bg / a.G, g = bg % a.G, i = row / a.r, h = g * a.r + row % a.r;
+  const int width = 4 * a.d + 4;
+  const long long step = (long long)a.B * a.G * a.R * width;
+  const float* p = a.part + (long long)blockIdx.x * width;
+  if (wave < 2) {                  // a wave per map: the common reference, each slice's weight and the sum of all
+    float top = -INFINITY, l = 0.f;
+    for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, p[s * step + 4 * a.d + 2 * wave]);
 #pragma unroll
-    for (int m = 0; m < 2; ++m) top[m] = fmaxf(top[m], p[s * step + 4 * a.d + 2 * m]);
-  float o[2][2] = {};              // [map][element lane, lane + 64]
-  for (int s = 0; s < a.splits; ++s) {
-    const float* ps = p + s * step;
+    for (int x = 32; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+    for (int s = lane; s < a.splits; s += 64) {
+      const float ls = p[s * step + 4 * a.d + 2 * wave + 1], w = ls == 0.f ? 0.f : exp2_(p[s * step + 4 * a.d + 2 * wave] - top);
+      wt[wave][s] = w;
+      l = fmaf(w, ls, l);
+    }
 #pragma unroll
-    for (int m = 0; m < 2; ++m) {
-      const float ls = ps[4 * a.d + 2 * m + 1];
-      if (ls == 0.f) continue;     // no key in this slice
-      const float w = exp2_(ps[4 * a.d + 2 * m] - top[m]);
-      l[m] += w * ls;
-#pragma unroll
-      for (int k = 0; k < 2; ++k)
-        if (lane + 64 * k < 2 * a.d) o[m][k] = fmaf(w, ps[m * 2 * a.d + lane + 64 * k], o[m][k]);
+    for (int x = 32; x > 0; x >>= 1) l += __shfl_xor(l, x);
+    if (lane == 0) {
+      norm[wave] = l == 0.f ? 0.f : 1.f / l;
+      if (a.stat) {
+        a.stat[((long long)bg * 4 + wave) * a.R + row] = top == -INFINITY ? 0.f : top;
+        a.stat[((long long)bg * 4 + 2 + wave) * a.R + row] = l == 0.f ? 0.f : 1.f / l;
+      }
     }
   }
-  const float i0 = l[0] == 0.f ? 0.f : 1.f / l[0], i1 = l[1] == 0.f ? 0.f : 1.f / l[1], lam = to_f(((const T*)a.lam)[h]);
-  const long long to = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d;
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    if (lane + 64 * k < 2 * a.d) {
-      const float z = o[1][k] * i1;
-      ((T*)a.out)[to + lane + 64 * k] = from_f<T>(o[0][k] * i0 - lam * z);
-      if (a.out2) a.out2[to + lane + 64 * k] = z;
-    }
-  if (a.stat && lane == 0) {
-#pragma unroll
-    for (int m = 0; m < 2; ++m) a.stat[((long long)bg * 4 + m) * a.R + row] = top[m] == -INFINITY ? 0.f : top[m];
-    a.stat[((long long)bg * 4 + 2) * a.R + row] = i0, a.stat[((long long)bg * 4 + 3) * a.R + row] = i1;
+  __syncthreads();
+  const int w4 = 4 * a.d, e = tid % w4, groups = 256 / w4, m = e >= 2 * a.d;
+  float acc = 0.f;
+#pragma unroll 4
+  for (int s = tid / w4; s < a.splits; s += groups) {
+    const float w = wt[m][s];
+    if (w != 0.f) acc = fmaf(w, p[s * step + e], acc);      // a slice without keys has written nothing
+  }
+  sum[tid] = acc;
+  __syncthreads();
+  if (tid < 2 * a.d) {
+    float o1 = 0.f, o2 = 0.f;
+    for (int k = 0; k < groups; ++k) o1 += sum[k * w4 + tid], o2 += sum[k * w4 + 2 * a.d + tid];
+    const long long to = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d + tid;
+    const float z = o2 * norm[1];
+    ((T*)a.out)[to] = from_f<T>(o1 * norm[0] - to_f(((const T*)a.lam)[h]) * z);
+    if (a.out2) a.out2[to] = z;
   }
 }
 
@@ -424,13 +438,16 @@ __global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
   }
 }
 
+// Where there are few row tiles, the keys of a row tile are cut into a.splits slices, whose sums go to a.part in fp32
 template <typename T, int D>
-__global__ __launch_bounds__(256) void dq_kernel(Args a) {
+__global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(Args a) {
   constexpr int NT = 256, KT = sizeof(T) == 2 ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
   constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1;
   __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
-  const int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  const int split = bid % a.splits;
+  bid /= a.splits;
   const int tile = a.tiles - 1 - bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;
   const int row = tile * 128 + wave * 32 + (lane & 31);
   const bool in = row < a.R;
@@ -459,6 +476,12 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
   int kend = limit;
   if (a.causal) kend = min(kend, min(a.R - 1, tile * 128 + 127) / a.r + shift + 1);
+  int kbeg = 0;
+  if (a.splits > 1) {              // whole tiles of the keys that the rows attend
+    const int n = kend > 0 ? (kend + KT - 1) / KT : 0;
+    kbeg = (int)((long long)n * split / a.splits) * KT;
+    kend = min(kend, (int)((long long)n * (split + 1) / a.splits) * KT);
+  }
   const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;
   const int wave_first = a.causal ? min(limit - 1, min(tile * 128 + wave * 32, a.R - 1) / a.r + shift) : limit - 1;
   const uint8_t* mrow = a.mask ? a.mask + b * a.m_b + i * a.m_r : nullptr;
@@ -475,13 +498,13 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
   const long long kld = a.k_r * (long long)sizeof(T), vld = a.v_r * (long long)sizeof(T);
   typedef Tile<T, D, KT, NT, true> KTile;
   typedef Tile<T, D, KT, NT, false> VTile;
-  const int nt = kend > 0 ? (kend + KT - 1) / KT : 0;
+  const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
   if (nt > 0) {
-    KTile::keys(lds, kbase, kld, 0, limit, a.d, tid, wave);
-    VTile::keys(lds + BYTES, vbase, vld, 0, limit, a.d, tid, wave);
+    KTile::keys(lds, kbase, kld, kbeg, limit, a.d, tid, wave);
+    VTile::keys(lds + BYTES, vbase, vld, kbeg, limit, a.d, tid, wave);
   }
   for (int t = 0; t < nt; ++t) {
-    const int j0 = t * KT;
+    const int j0 = kbeg + t * KT;
     const char* kt = lds + (t & 1) * 2 * BYTES;
     const char* vt = kt + BYTES;
     __syncthreads();
@@ -497,8 +520,7 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
       f32x16 s[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) s[m] = scores<T, D, KT>(kt, kb, m, q[m], lane);
-      const bool some = a.mask || jb + 31 > wave_first;
-      if (some) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
+      if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
       for (int st = 0; st < VS; ++st) dp = mfma16(row_frag<T, GR>(vt, kb * 32 + (lane & 31), 16 * st, half), go[st], dp);
@@ -508,8 +530,7 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           // 1 / sum and -lam are factors of the whole column: they wait for the end
-          float ds = exp2_(fmaf(s[m][e], a.c, -rd[m])) * (dp[e] - rd[2 + m]);
-          if (some && s[m][e] == -INFINITY) ds = 0.f;
+          const float ds = exp2_(fmaf(s[m][e], a.c, -rd[m])) * (dp[e] - rd[2 + m]);
           s[m][e] = ds;
           top[m] = fmaxf(top[m], fabsf(ds));
         }
@@ -521,13 +542,13 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
           const vec8<T> f = scaled_frag<T>(s[m], st, sc[m].mul());
 #pragma unroll
           for (int x = 0; x < QT; ++x)
-            acc[m][x] = mfma16(col_frag_acc<T, GR, false>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, acc[m][x]);
+            acc[m][x] = mfma16(col_frag_acc<T, GR>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, acc[m][x]);
         }
       }
     }
   }
   if (!in) return;
-  T* out = (T*)a.dq + (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d;
+  const long long at = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d, all = (long long)a.B * a.Nq * a.H * 2 * a.d;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
     const float f = a.scale * (m == 0 ? rd[4] : -rd[5]) * sc[m].undo();
@@ -536,19 +557,25 @@ __global__ __launch_bounds__(256) void dq_kernel(Args a) {
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const int col = (D >= 32 ? m * D : 0) + x * 32 + 8 * y + 4 * half, w = col % D;
-        if (col / D == m && w < a.d) put4(out + m * a.d + w, acc[m][x][4 * y] * f, acc[m][x][4 * y + 1] * f, acc[m][x][4 * y + 2] * f, acc[m][x][4 * y + 3] * f);
+        if (col / D == m && w < a.d) {
+          const float o0 = acc[m][x][4 * y] * f, o1 = acc[m][x][4 * y + 1] * f, o2 = acc[m][x][4 * y + 2] * f, o3 = acc[m][x][4 * y + 3] * f;
+          if (a.splits > 1) put4(a.part + split * all + at + m * a.d + w, o0, o1, o2, o3);
+          else put4((T*)a.dq + at + m * a.d + w, o0, o1, o2, o3);
+        }
       }
   }
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(256) void dkv_kernel(Args a) {
+__global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel(Args a) {
   constexpr int NT = 256, QR = (sizeof(T) == 2 && D == 16) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = QR * GR * 16;
   constexpr int RG = ROWDATA * QR / 4, STAGE = 2 * BYTES + (RG + 63) / 64 * 1024;      // RG granules of row values
   constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1, VT = 2 * D / 32;
   __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
-  const int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
+  const int split = bid % a.splits;
+  bid /= a.splits;
   const int tile = bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
   const int jw = tile * 128 + wave * 32, j = jw + (lane & 31);
@@ -588,7 +615,11 @@ __global__ __launch_bounds__(256) void dkv_kernel(Args a) {
   typedef Tile<T, D, QR, NT, false> OTile;
   int rbeg = 0;
   if (a.causal) rbeg = (int)(min((long long)max(0, tile * 128 - shift) * a.r, (long long)a.Rp) / QR * QR);
-  const int nt = tile * 128 < limit ? (a.R - rbeg + QR - 1) / QR : 0;
+  int nt = tile * 128 < limit ? (a.R - rbeg + QR - 1) / QR : 0;
+  if (a.splits > 1 && nt > 0) {
+    const int from = (int)((long long)nt * split / a.splits), to = (int)((long long)nt * (split + 1) / a.splits);
+    rbeg += from * QR, nt = to - from;
+  }
 
   auto stage = [&](char* to, int row0) {
     QTile::rows(to, qbase, qld, head, row0, a.R, a.r, a.d, tid, wave);
@@ -636,11 +667,10 @@ __global__ __launch_bounds__(256) void dkv_kernel(Args a) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int e = 4 * y + x;
-          const bool out = some && s[0][e] == -INFINITY && s[1][e] == -INFINITY;
           const float p1 = exp2_(fmaf(s[0][e], a.c, -r4[0][x])) * r4[4][x], p2 = exp2_(fmaf(s[1][e], a.c, -r4[1][x])) * r4[5][x];
           w[e] = p1 - p2;
-          s[0][e] = out ? 0.f : p1 * (dp[e] - r4[2][x]);
-          s[1][e] = out ? 0.f : -p2 * (dp[e] - r4[3][x]);
+          s[0][e] = p1 * (dp[e] - r4[2][x]);
+          s[1][e] = -p2 * (dp[e] - r4[3][x]);
           top[0] = fmaxf(top[0], fabsf(w[e])), top[1] = fmaxf(top[1], fabsf(s[0][e])), top[2] = fmaxf(top[2], fabsf(s[1][e]));
         }
       }
@@ -649,7 +679,7 @@ __global__ __launch_bounds__(256) void dkv_kernel(Args a) {
       for (int st = 0; st < 2; ++st) {
         const vec8<T> f = scaled_frag<T>(w, st, sv.mul());
 #pragma unroll
-        for (int x = 0; x < VT; ++x) dv[x] = mfma16(col_frag_acc<T, GR, false>(ot, rb * 32 + 16 * st, x * 32, lane), f, dv[x]);
+        for (int x = 0; x < VT; ++x) dv[x] = mfma16(col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, x * 32, lane), f, dv[x]);
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -658,20 +688,23 @@ __global__ __launch_bounds__(256) void dkv_kernel(Args a) {
         for (int st = 0; st < 2; ++st) {
           const vec8<T> f = scaled_frag<T>(s[m], st, sk[m].mul());
 #pragma unroll
-          for (int x = 0; x < QT; ++x) dk[m][x] = mfma16(col_frag_acc<T, GR, false>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, dk[m][x]);
+          for (int x = 0; x < QT; ++x) dk[m][x] = mfma16(col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, dk[m][x]);
         }
       }
     }
   }
   if (j >= a.Nk) return;           // keys past their sequence's length get zeros
-  const long long at = (((long long)b * a.Nk + j) * a.G + g) * 2 * a.d;
+  const long long at = (((long long)b * a.Nk + j) * a.G + g) * 2 * a.d, all = (long long)a.B * a.Nk * a.G * 2 * a.d;
 #pragma unroll
   for (int x = 0; x < VT; ++x)
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int e = x * 32 + 8 * y + 4 * half;
       const float f = sv.undo();
-      if (e < 2 * a.d) put4((T*)a.dv + at + e, dv[x][4 * y] * f, dv[x][4 * y + 1] * f, dv[x][4 * y + 2] * f, dv[x][4 * y + 3] * f);
+      if (e < 2 * a.d) {
+        if (a.splits > 1) put4(a.part + (2ll * split + 1) * all + at + e, dv[x][4 * y] * f, dv[x][4 * y + 1] * f, dv[x][4 * y + 2] * f, dv[x][4 * y + 3] * f);
+        else put4((T*)a.dv + at + e, dv[x][4 * y] * f, dv[x][4 * y + 1] * f, dv[x][4 * y + 2] * f, dv[x][4 * y + 3] * f);
+      }
     }
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -681,9 +714,26 @@ __global__ __launch_bounds__(256) void dkv_kernel(Args a) {
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const int col = (D >= 32 ? m * D : 0) + x * 32 + 8 * y + 4 * half, w = col % D;
-        if (col / D == m && w < a.d)
-          put4((T*)a.dk + at + m * a.d + w, dk[m][x][4 * y] * f, dk[m][x][4 * y + 1] * f, dk[m][x][4 * y + 2] * f, dk[m][x][4 * y + 3] * f);
+        if (col / D == m && w < a.d) {
+          const float o0 = dk[m][x][4 * y] * f, o1 = dk[m][x][4 * y + 1] * f, o2 = dk[m][x][4 * y + 2] * f, o3 = dk[m][x][4 * y + 3] * f;
+          if (a.splits > 1) put4(a.part + 2ll * split * all + at + m * a.d + w, o0, o1, o2, o3);
+          else put4((T*)a.dk + at + m * a.d + w, o0, o1, o2, o3);
+        }
       }
+  }
+}
+
+// out[i] = sum over the slices of part[slice * step + i], in order
+template <typename T>
+__global__ __launch_bounds__(256) void sum_kernel(const float* part, T* out, long long n, long long step, int slices) {
+  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
+    float s[4] = {};
+    for (int k = 0; k < slices; ++k) {
+      const Four<float> v = *(const Four<float>*)(part + k * step + i);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] += v.v[e];
+    }
+    put4(out + i, s[0], s[1], s[2], s[3]);
   }
 }
 
@@ -703,11 +753,35 @@ Split split_of(const ff3d_diff_attention_t& p) {
   const long long blocks = bg * s.tiles;
   long long n = blocks >= 512 ? 1 : cdiv(1024, blocks);
   n = n < p.Nk / 256 ? n : p.Nk / 256;
+  if (n > JOIN) n = JOIN;
   if (n < 1) n = 1;
   s.len = (int)((cdiv(p.Nk, n) + 63) / 64 * 64);
   s.splits = cdiv(p.Nk, s.len);
   return s;
 }
+
+// Backward pass: the loop of a key tile (over rows) or of a row tile (over keys) is cut where the tiles alone leave the chip short of
+// blocks, to slices of at least 128 rows or keys; the slices' fp32 sums are added in order.  Both kernels use one place for them.
+struct BwdSplit {
+  int q, k;
+  long long rowdata, total;        // bytes
+};
+BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
+  const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
+  auto slices = [](long long blocks, long long len) {
+    long long n = blocks >= 384 ? 1 : cdiv(512, blocks);
+    n = n < len / 128 ? n : len / 128;
+    return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
+  };
+  BwdSplit s;
+  s.q = slices(bg * cdiv(R, 128), p.Nk);
+  s.k = slices(bg * cdiv(p.Nk, 128), R);
+  s.rowdata = bg * ROWDATA * ((R + 63) / 64 * 64) * 4;
+  const long long q = s.q > 1 ? s.q * (long long)p.B * p.Nq * p.heads * 2 * p.d * 4 : 0, k = s.k > 1 ? 2ll * s.k * p.B * p.Nk * p.kv_heads * 2 * p.d * 4 : 0;
+  s.total = s.rowdata + (q > k ? q : k);
+  return s;
+}
+inline int sum_grid(long long n) { return (int)(n / 1024 + 1 < 2048 ? n / 1024 + 1 : 2048); }
 
 int check(const ff3d_diff_attention_t* p) {
   FF3D_REQUIRE(p && p->q && p->k && p->v && p->lam, FF3D_ERR_NULL);
@@ -746,23 +820,32 @@ int fwd(const ff3d_diff_attention_t& p, Args a, hipStream_t st) {
   if (blocks > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
   if (s.waves == 4) fwd_kernel<T, D, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
   else fwd_kernel<T, D, 1><<<(unsigned)blocks, 64, 0, st>>>(a);
-  if (s.splits > 1) join_kernel<T><<<(unsigned)cdiv((long long)a.B * a.G * a.R, 4), 256, 0, st>>>(a);
+  if (s.splits > 1) join_kernel<T><<<(unsigned)((long long)a.B * a.G * a.R), 256, 0, st>>>(a);
   return ff3d_launch_status();
 }
 
 template <typename T, int D>
 int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
-  const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128), kb = bg * cdiv(a.Nk, 128);
+  const BwdSplit s = bwd_split_of(p);
+  const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128) * s.q, kb = bg * cdiv(a.Nk, 128) * s.k;
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
+  a.part = a.rowdata + s.rowdata / 4;
   rows_kernel<T><<<(unsigned)cdiv(rows, 16), 256, 0, st>>>(a);
   if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
   if (a.dk) {
-    a.tiles = cdiv(a.Nk, 128);
+    const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;
+    a.tiles = cdiv(a.Nk, 128), a.splits = s.k;
     dkv_kernel<T, D><<<(unsigned)kb, 256, 0, st>>>(a);
+    if (s.k > 1) {
+      sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dk, n, 2 * n, s.k);
+      sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part + n, (T*)a.dv, n, 2 * n, s.k);
+    }
   }
   if (a.dq) {
-    a.tiles = cdiv(a.R, 128);
+    const long long n = (long long)a.B * a.Nq * a.H * 2 * a.d;
+    a.tiles = cdiv(a.R, 128), a.splits = s.q;
     dq_kernel<T, D><<<(unsigned)qb, 256, 0, st>>>(a);
+    if (s.q > 1) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, n, n, s.q);
   }
   return ff3d_launch_status();
 }
@@ -781,7 +864,7 @@ int bwd_d(const ff3d_diff_attention_t& p, const Args& a, void* dlam, hipStream_t
 extern "C" int64_t ff3d_diff_attention_workspace_bytes(const ff3d_diff_attention_t* p, int backward) {
   if (!p || p->B <= 0 || p->Nq <= 0 || p->Nk <= 0 || p->heads <= 0 || p->kv_heads <= 0 || p->heads % p->kv_heads) return 0;
   const long long bg = (long long)p->B * p->kv_heads, R = (long long)p->Nq * (p->heads / p->kv_heads);
-  if (backward) return bg * ROWDATA * ((R + 63) / 64 * 64) * 4;
+  if (backward) return bwd_split_of(*p).total;
   const Split s = split_of(*p);
   return s.splits > 1 ? (long long)s.splits * bg * R * (4 * p->d + 4) * 4 : 0;
 }

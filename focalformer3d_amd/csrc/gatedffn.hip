@@ -130,7 +130,7 @@ struct Operand {
         off[i] = in ? (unsigned)row * (unsigned)(ld * sizeof(T)) + g * 16u : OUT;
       } else {
         constexpr int GR = ROWS / P;
-        const int k = at / GR, g = place<GR, true>(k, at % GR);
+        const int k = at / GR, g = place<GR>(k, at % GR);
         kk[i] = k;
         off[i] = row0 + g * P < nrows ? (unsigned)k * (unsigned)(ld * sizeof(T)) + g * 16u : OUT;
       }
@@ -192,12 +192,12 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
         if constexpr (AROW) fa[s & 1][j] = row_frag<T, 8>(cur, (wm * TM + j) * 32 + (lane & 31), 16 * s, half);
-        else fa[s & 1][j] = col_frag<T, BM / P, true>(cur, 16 * s, (wm * TM + j) * 32, lane);
+        else fa[s & 1][j] = col_frag<T, BM / P>(cur, 16 * s, (wm * TM + j) * 32, lane);
       }
 #pragma unroll
       for (int i = 0; i < TN; ++i) {
         if constexpr (BROW) fb[s & 1][i] = row_frag<T, 8>(cur + ABYTES, (wn * TN + i) * 32 + (lane & 31), 16 * s, half);
-        else fb[s & 1][i] = col_frag<T, BN / P, true>(cur + ABYTES, 16 * s, (wn * TN + i) * 32, lane);
+        else fb[s & 1][i] = col_frag<T, BN / P>(cur + ABYTES, 16 * s, (wn * TN + i) * 32, lane);
       }
     };
     read(0);
