@@ -177,16 +177,16 @@ __device__ __forceinline__ void exclude_cols_q(const Args& a, const uint8_t* mro
 }
 
 template <typename T, int D, int KT>
-__device__ __forceinline__ f32x16 scores(const char* tile, int kb, int map, const vec8<T>* other, int lane) {
+__device__ __forceinline__ f32x16 scores(const char* tile, int kb, int map, const Op<T>* other, int lane) {
   constexpr int GR = 2 * D / Type<T>::PER16;
   f32x16 s = (f32x16)(0.f);
 #pragma unroll
-  for (int st = 0; st < D / 16; ++st) s = mfma16(row_frag<T, GR>(tile, kb * 32 + (lane & 31), map * D + 16 * st, lane >> 5), other[st], s);
+  for (int st = 0; st < D / 16; ++st) s = mfma_step<T>(op<T>(row_frag<T, GR>(tile, kb * 32 + (lane & 31), map * D + 16 * st, lane >> 5)), other[st], s);
   return s;
 }
 
 // waves per SIMD that the registers are cut for: 2 where they fit (two waves hide each other's waits)
-constexpr int waves_of(int D, int size, bool fits64) { return D <= 32 || (size == 2 && fits64) ? 2 : 1; }
+constexpr int waves_of(int D, int size, bool fits64) { return size == 4 ? (D <= 16 ? 2 : 1) : (D <= 32 || fits64 ? 2 : 1); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
 template <typename T, int D, int NW>
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
   const bool in = row < a.R;
   const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
 
-  vec8<T> q[2][ST];
+  Op<T> q[2][ST];
   {
     const char* p = a.q + (b * a.q_b + (long long)i * a.q_r + (long long)h * 2 * a.d) * (long long)sizeof(T);
 #pragma unroll
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
         const int e = 16 * st + 8 * half;
-        q[m][st] = load8<T>(p + (m * a.d + e) * (int)sizeof(T), in && e < a.d);
+        q[m][st] = op<T>(load8<T>(p + (m * a.d + e) * (int)sizeof(T), in && e < a.d));
       }
   }
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
 #pragma unroll
       for (int m = 0; m < 2; ++m) s[m] = scores<T, D, KT>(kt, kb, m, q[m], lane);
       if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
-      vec8<T> p[2][2];
+      Op<T> p[2][2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         float x = s[m][0];
@@ -283,16 +283,16 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
           sum += s[m][e];
         }
         l[m] += sum;
-        p[m][0] = acc_frag<T>(s[m], 0);
-        p[m][1] = acc_frag<T>(s[m], 1);
+        p[m][0] = op<T>(acc_frag<T>(s[m], 0));
+        p[m][1] = op<T>(acc_frag<T>(s[m], 1));
       }
 #pragma unroll
       for (int st = 0; st < 2; ++st)
 #pragma unroll
         for (int v = 0; v < VT; ++v) {
-          const vec8<T> f = col_frag_acc<T, GR>(vt, kb * 32 + 16 * st, v * 32, lane);
-          o[0][v] = mfma16(f, p[0][st], o[0][v]);
-          o[1][v] = mfma16(f, p[1][st], o[1][v]);
+          const Op<T> f = op<T>(col_frag_acc<T, GR>(vt, kb * 32 + 16 * st, v * 32, lane));
+          o[0][v] = mfma_step<T>(f, p[0][st], o[0][v]);
+          o[1][v] = mfma_step<T>(f, p[1][st], o[1][v]);
         }
     }
   }
@@ -453,7 +453,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   const bool in = row < a.R;
   const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
 
-  vec8<T> q[2][ST], go[VS];
+  Op<T> q[2][ST], go[VS];
   {
     const char* p = a.q + (b * a.q_b + (long long)i * a.q_r + (long long)h * 2 * a.d) * (long long)sizeof(T);
     const char* po = a.dout + (b * a.do_b + (long long)i * a.do_r + (long long)h * 2 * a.d) * (long long)sizeof(T);
@@ -462,12 +462,12 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
         const int e = 16 * st + 8 * half;
-        q[m][st] = load8<T>(p + (m * a.d + e) * (int)sizeof(T), in && e < a.d);
+        q[m][st] = op<T>(load8<T>(p + (m * a.d + e) * (int)sizeof(T), in && e < a.d));
       }
 #pragma unroll
     for (int st = 0; st < VS; ++st) {
       const int e = 16 * st + 8 * half;
-      go[st] = load8<T>(po + e * (int)sizeof(T), in && e < 2 * a.d);
+      go[st] = op<T>(load8<T>(po + e * (int)sizeof(T), in && e < 2 * a.d));
     }
   }
   float rd[ROWDATA];
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
       if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
-      for (int st = 0; st < VS; ++st) dp = mfma16(row_frag<T, GR>(vt, kb * 32 + (lane & 31), 16 * st, half), go[st], dp);
+      for (int st = 0; st < VS; ++st) dp = mfma_step<T>(op<T>(row_frag<T, GR>(vt, kb * 32 + (lane & 31), 16 * st, half)), go[st], dp);
       float top[2] = {0.f, 0.f};
 #pragma unroll
       for (int m = 0; m < 2; ++m)
@@ -539,10 +539,10 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
         sc[m].template see<QT>(top[m], acc[m]);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          const vec8<T> f = scaled_frag<T>(s[m], st, sc[m].mul());
+          const Op<T> f = op<T>(scaled_frag<T>(s[m], st, sc[m].mul()));
 #pragma unroll
           for (int x = 0; x < QT; ++x)
-            acc[m][x] = mfma16(col_frag_acc<T, GR>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, acc[m][x]);
+            acc[m][x] = mfma_step<T>(op<T>(col_frag_acc<T, GR>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane)), f, acc[m][x]);
         }
       }
     }
@@ -583,18 +583,18 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
 
   const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
   const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
-  vec8<T> k[2][ST], v[VS];
+  Op<T> k[2][ST], v[VS];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int st = 0; st < ST; ++st) {
       const int e = 16 * st + 8 * half;
-      k[m][st] = load8<T>(kbase + ((long long)j * a.k_r + m * a.d + e) * (long long)sizeof(T), in && e < a.d);
+      k[m][st] = op<T>(load8<T>(kbase + ((long long)j * a.k_r + m * a.d + e) * (long long)sizeof(T), in && e < a.d));
     }
 #pragma unroll
   for (int st = 0; st < VS; ++st) {
     const int e = 16 * st + 8 * half;
-    v[st] = load8<T>(vbase + ((long long)j * a.v_r + e) * (long long)sizeof(T), in && e < 2 * a.d);
+    v[st] = op<T>(load8<T>(vbase + ((long long)j * a.v_r + e) * (long long)sizeof(T), in && e < 2 * a.d));
   }
 
   f32x16 dv[VT], dk[2][QT];
@@ -655,7 +655,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
       }
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
-      for (int st = 0; st < VS; ++st) dp = mfma16(row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * st, half), v[st], dp);
+      for (int st = 0; st < VS; ++st) dp = mfma_step<T>(op<T>(row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * st, half)), v[st], dp);
       f32x16 w;
       float top[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -677,18 +677,18 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
       sv.template see<VT>(top[0], dv);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const vec8<T> f = scaled_frag<T>(w, st, sv.mul());
+        const Op<T> f = op<T>(scaled_frag<T>(w, st, sv.mul()));
 #pragma unroll
-        for (int x = 0; x < VT; ++x) dv[x] = mfma16(col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, x * 32, lane), f, dv[x]);
+        for (int x = 0; x < VT; ++x) dv[x] = mfma_step<T>(op<T>(col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, x * 32, lane)), f, dv[x]);
       }
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         sk[m].template see<QT>(top[1 + m], dk[m]);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          const vec8<T> f = scaled_frag<T>(s[m], st, sk[m].mul());
+          const Op<T> f = op<T>(scaled_frag<T>(s[m], st, sk[m].mul()));
 #pragma unroll
-          for (int x = 0; x < QT; ++x) dk[m][x] = mfma16(col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane), f, dk[m][x]);
+          for (int x = 0; x < QT; ++x) dk[m][x] = mfma_step<T>(op<T>(col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane)), f, dk[m][x]);
         }
       }
     }

@@ -2,8 +2,11 @@
 //
 // One step multiplies 32 x 16 by 16 x 32.  A lane l holds 8 elements of each operand, element e being
 //   A[l % 32][8 * (l / 32) + e]   and   B[8 * (l / 32) + e][l % 32],
-// in every type: 16-bit types feed them to one v_mfma_f32_32x32x16, fp32 feeds element e of all lanes to the e-th of eight
-// v_mfma_f32_32x32x2 (which pairs the k = e of the lower half with the k = 8 + e of the upper).  The order of k inside a step
+// in every type: 16-bit types feed them to one v_mfma_f32_32x32x16; an fp32 number is the sum of three bf16 numbers (hi, mid, lo, each
+// the rest rounded to nearest: 8 bits and a sign more every time, so 24 bits and more in all, over the whole range of exponents) and the
+// step is six bf16 products, all but mid * lo, lo * mid and lo * lo, which together are at most 2^-23 of the product and of either
+// sign.  Six times 32 cycles against eight v_mfma_f32_32x32x2 of 64, and the vector unit, which splits, works beside the matrix unit.
+// (Infinities split into NaN; numbers above 3.39e38 round to infinity.)  The order of k inside a step
 // is free as long as both operands agree, which the callers use: the accumulator layout
 //   reg r of lane l  =  C[8 * (r / 4) + 4 * (l / 32) + r % 4][l % 32]
 // read as the operand of a following product has element e of step s = reg 8 s + e, i.e. k = 16 s + 8 (e / 4) + 4 (l / 32) + e % 4
@@ -31,10 +34,54 @@ __device__ __forceinline__ f32x16 mfma16(vec8<__bf16> a, vec8<__bf16> b, f32x16 
 __device__ __forceinline__ f32x16 mfma16(vec8<_Float16> a, vec8<_Float16> b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mfma16(vec8<float> a, vec8<float> b, f32x16 c) {
+
+// An operand of a step, ready for the matrix unit: itself, or the three parts of fp32.
+template <typename T>
+struct Op {
+  vec8<T> v;
+};
+template <>
+struct Op<float> {
+  vec8<__bf16> h, m, l;
+};
+template <typename T>
+__device__ __forceinline__ Op<T> op(vec8<T> x) {
+  if constexpr (sizeof(T) == 2) {
+    return {x};
+  } else {
+    Op<float> o;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
-  return c;
+    for (int e = 0; e < 8; ++e) {
+      const __bf16 h = (__bf16)x[e];
+      const float r = x[e] - (float)h;               // exact
+      const __bf16 m = (__bf16)r;
+      o.h[e] = h, o.m[e] = m, o.l[e] = (__bf16)(r - (float)m);
+    }
+    return o;
+  }
+}
+// part 0 .. PARTS - 1 of a step, the smallest terms first; the caller may run the parts of several tiles in turn
+template <typename T>
+constexpr int PARTS = sizeof(T) == 4 ? 6 : 1;
+template <int PART, typename T>
+__device__ __forceinline__ f32x16 mfma_part(const Op<T>& a, const Op<T>& b, f32x16 c) {
+  if constexpr (sizeof(T) == 2) return mfma16(a.v, b.v, c);
+  else if constexpr (PART == 0) return mfma16(a.l, b.h, c);
+  else if constexpr (PART == 1) return mfma16(a.h, b.l, c);
+  else if constexpr (PART == 2) return mfma16(a.m, b.m, c);
+  else if constexpr (PART == 3) return mfma16(a.m, b.h, c);
+  else if constexpr (PART == 4) return mfma16(a.h, b.m, c);
+  else return mfma16(a.h, b.h, c);
+}
+template <typename T>
+__device__ __forceinline__ f32x16 mfma_step(const Op<T>& a, const Op<T>& b, f32x16 c) {
+  if constexpr (sizeof(T) == 4) {
+    c = mfma_part<0>(a, b, c), c = mfma_part<1>(a, b, c), c = mfma_part<2>(a, b, c);
+    c = mfma_part<3>(a, b, c), c = mfma_part<4>(a, b, c), c = mfma_part<5>(a, b, c);
+    return c;
+  } else {
+    return mfma16(a.v, b.v, c);
+  }
 }
 
 __device__ __forceinline__ int acc_row(int r, int half) { return 8 * (r / 4) + 4 * half + r % 4; }
@@ -126,6 +173,12 @@ __device__ __forceinline__ rsrc_t make_rsrc(const void* p, long long bytes) {
 }
 __device__ __forceinline__ void load_lds16(rsrc_t r, char* lds, unsigned off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
+}
+
+// Waits until at most N of this wave's loads are outstanding and its LDS reads are done, then for the other waves.
+template <int N>
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");
 }
 
 }  // namespace mma

@@ -12,6 +12,8 @@
 //   plain      dx and, with its row sum cut into slices that a second kernel adds in order, dW: results do not depend on timing
 // A block computes C^T tiles: the n side (features of W, columns of the output) is the row operand, so a lane holds 4 consecutive
 // columns of one output row and stores them together.
+#include <type_traits>
+
 #include "ff3d_mma.h"
 
 namespace {
@@ -32,7 +34,7 @@ struct GemmArgs {
   int M, N, K;                  // output rows and columns (F for EPI_GATED*), length of the sums
   int acols, bcols;             // column tiles: width of the operand, padded to whole granules
   int F, act, mt, nt, slices, kslice;
-  int vec_out, vec_dh;          // 4-element accesses of out / dh are aligned
+  int vec_out, vec_out2, vec_dh;     // 16-byte accesses of rows of out, of its second half (EPI_GATED_BWD) and of dh are aligned
   int out_pad;                  // EPI_GATED_BWD: zero columns behind the 2 F
 };
 
@@ -44,10 +46,16 @@ __device__ __forceinline__ float exp_t(float x) {
 }
 
 template <typename T>
+__device__ __forceinline__ float sigmoid_t(float x) {
+  if constexpr (sizeof(T) == 4) return 1.f / (1.f + expf(-x));
+  else return __builtin_amdgcn_rcpf(1.f + __expf(-x));         // 1 ulp of fp32, far below the output's rounding
+}
+
+template <typename T>
 __device__ __forceinline__ float act_f(float g, int act) {
   if (act == ACT_RELU) return g < 0.f ? 0.f : g;               // a NaN stays one
   if (act == ACT_GELU) return g * (0.5f * (1.f + erff(g * 0.70710678118654752f)));
-  const float s = 1.f / (1.f + exp_t<T>(-g));
+  const float s = sigmoid_t<T>(g);
   return act == ACT_SIGMOID ? s : g * s;
 }
 template <typename T>
@@ -58,7 +66,7 @@ __device__ __forceinline__ void act_both(float g, int act, float& a, float& da) 
     const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     a = g * cdf, da = cdf + g * exp_t<T>(-0.5f * g * g) * 0.39894228040143268f;
   } else {
-    const float s = 1.f / (1.f + exp_t<T>(-g));
+    const float s = sigmoid_t<T>(g);
     if (act == ACT_SIGMOID) a = s, da = s * (1.f - s);
     else a = g * s, da = s * (1.f + g * (1.f - s));
   }
@@ -94,12 +102,21 @@ __device__ __forceinline__ void load4(const T* p, float* v, int left, bool vec) 
   }
 }
 
+// The loop over the long sum.  Blocks of 8 waves (256 x 256): steps of 64 bytes of k in a ring of four; the two waves of a SIMD work
+// half a step apart, one reading its operands and asking for the step after next but one while the other multiplies, so the matrix
+// unit of the SIMD is fed without a pause (d W at 16384 x 5472 x 1024 in bf16: 182 us, against 217 with two steps of 128 bytes that
+// all waves read, multiply and wait for together).  Blocks of 4 waves: two or more share a CU and fill each other's waits; two steps
+// of 128 bytes (128 x 128, the same product: 221 us, 250 with the ring).
+constexpr int step_bytes_of(int waves) { return waves == 8 ? 64 : 128; }
+constexpr int stages_of(int waves) { return waves == 8 ? 4 : 2; }
+
 // One operand of a block: ROWS rows (or columns) of it, BK of k per step, DMA-ed into LDS.
 // ROW: k is contiguous in memory (row tile), else the rows are (column tile).  DUAL: rows come in blocks of 32 alternating between
 // the gate and the value half of the weight.
 template <typename T, bool ROW, bool DUAL, int ROWS, int NT>
 struct Operand {
-  static constexpr int P = Type<T>::PER16, BK = 128 / (int)sizeof(T), N = ROWS * 8 / NT;
+  static constexpr int STEP = step_bytes_of(NT / 64), P = Type<T>::PER16, BK = STEP / (int)sizeof(T), GK = STEP / 16, N = ROWS * GK / NT;
+  static_assert(ROWS * GK % NT == 0, "whole granules per thread");
   const char *base, *end;
   long long step_bytes;
   unsigned off[N];
@@ -109,7 +126,7 @@ struct Operand {
     end = p + bytes;
     if constexpr (ROW) {
       base = p + (DUAL ? 0 : (long long)row0 * ld * sizeof(T)) + k0 * (long long)sizeof(T);
-      step_bytes = 128;
+      step_bytes = STEP;
     } else {
       base = p + k0 * ld * (long long)sizeof(T) + (long long)row0 * sizeof(T);
       step_bytes = (long long)BK * ld * sizeof(T);
@@ -118,7 +135,7 @@ struct Operand {
     for (int i = 0; i < N; ++i) {
       const int at = i * NT + tid;
       if constexpr (ROW) {
-        const int r = at >> 3, g = place<8>(r, at & 7);
+        const int r = at / GK, g = place<GK>(r, at % GK);
         int row = r;
         bool in = row0 + r < nrows;
         if constexpr (DUAL) {
@@ -149,8 +166,8 @@ template <typename T, bool AROW, bool BROW, int WM, int WN, int TM, int TN, int 
 __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
   constexpr bool DUAL = EPI == EPI_GATED || EPI == EPI_GATED_BWD;
   constexpr int NT = WM * WN * 64, BM = WM * TM * 32, BN = WN * TN * 32, BNO = DUAL ? BN / 2 : BN;
-  constexpr int BK = 128 / (int)sizeof(T), STEPS = BK / 16, P = Type<T>::PER16;
-  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  constexpr int STEP = step_bytes_of(WM * WN), STAGES = stages_of(WM * WN), BK = STEP / (int)sizeof(T), STEPS = BK / 16, P = Type<T>::PER16, GK = STEP / 16;
+  constexpr int ABYTES = BM * STEP, STAGE = (BM + BN) * STEP;
   extern __shared__ __attribute__((aligned(16))) char lds[];
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
@@ -176,99 +193,209 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
     for (int j = 0; j < TM; ++j) acc[i][j] = (f32x16)(0.f);
 
   const int nk = (kn + BK - 1) / BK;
-  A.stage(lds, wave, kn);
-  B.stage(lds + ABYTES, wave, kn);
-  for (int t = 0; t < nk; ++t) {
-    char* cur = lds + (t & 1) * STAGE;
-    __syncthreads();               // step t has arrived, and nobody reads the other half any more
-    if (t + 1 < nk) {
-      char* nxt = lds + ((t + 1) & 1) * STAGE;
-      A.stage(nxt, wave, kn - (t + 1) * BK);
-      B.stage(nxt + ABYTES, wave, kn - (t + 1) * BK);
+  auto stage = [&](int t) {
+    char* to = lds + (t % STAGES) * STAGE;
+    A.stage(to, wave, kn - t * BK);
+    B.stage(to + ABYTES, wave, kn - t * BK);
+  };
+  vec8<T> fa[2][TM], fb[2][TN];
+  auto read = [&](const char* cur, int s) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+      if constexpr (AROW) fa[s & 1][j] = row_frag<T, GK>(cur, (wm * TM + j) * 32 + (lane & 31), 16 * s, half);
+      else fa[s & 1][j] = col_frag<T, BM / P>(cur, 16 * s, (wm * TM + j) * 32, lane);
     }
-    // operands of step s + 1 are read while the matrix unit works on step s
-    vec8<T> fa[2][TM], fb[2][TN];
-    auto read = [&](int s) {
 #pragma unroll
-      for (int j = 0; j < TM; ++j) {
-        if constexpr (AROW) fa[s & 1][j] = row_frag<T, 8>(cur, (wm * TM + j) * 32 + (lane & 31), 16 * s, half);
-        else fa[s & 1][j] = col_frag<T, BM / P>(cur, 16 * s, (wm * TM + j) * 32, lane);
-      }
+    for (int i = 0; i < TN; ++i) {
+      if constexpr (BROW) fb[s & 1][i] = row_frag<T, GK>(cur + ABYTES, (wn * TN + i) * 32 + (lane & 31), 16 * s, half);
+      else fb[s & 1][i] = col_frag<T, BN / P>(cur + ABYTES, 16 * s, (wn * TN + i) * 32, lane);
+    }
+  };
+  auto multiply = [&](int s) {
+    Op<T> oa[TM], ob[TN];
 #pragma unroll
-      for (int i = 0; i < TN; ++i) {
-        if constexpr (BROW) fb[s & 1][i] = row_frag<T, 8>(cur + ABYTES, (wn * TN + i) * 32 + (lane & 31), 16 * s, half);
-        else fb[s & 1][i] = col_frag<T, BN / P>(cur + ABYTES, 16 * s, (wn * TN + i) * 32, lane);
-      }
-    };
-    read(0);
+    for (int j = 0; j < TM; ++j) oa[j] = op<T>(fa[s & 1][j]);
 #pragma unroll
-    for (int s = 0; s < STEPS; ++s) {
-      if (s + 1 < STEPS) read(s + 1);
-      __builtin_amdgcn_sched_barrier(0);
+    for (int i = 0; i < TN; ++i) ob[i] = op<T>(fb[s & 1][i]);
+    auto all = [&](auto part) {
 #pragma unroll
       for (int i = 0; i < TN; ++i)
 #pragma unroll
-        for (int j = 0; j < TM; ++j) acc[i][j] = mfma16(fb[s & 1][i], fa[s & 1][j], acc[i][j]);
-      __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < TM; ++j) acc[i][j] = mfma_part<decltype(part)::value>(ob[i], oa[j], acc[i][j]);
+    };
+    all(std::integral_constant<int, 0>{});
+    if constexpr (PARTS<T> == 6) {
+      all(std::integral_constant<int, 1>{}), all(std::integral_constant<int, 2>{}), all(std::integral_constant<int, 3>{});
+      all(std::integral_constant<int, 4>{}), all(std::integral_constant<int, 5>{});
     }
+  };
+  if constexpr (WM * WN == 8) {
+    // Barriers are numbered; the late half of the waves meets one before it starts.  Early waves read step t between barriers 2 t and
+    // 2 t + 1 and multiply it until 2 t + 2, late ones are one barrier behind.  At the end of its reading of step t a wave has waited
+    // for its own loads of step t + 1: the early waves' first look at that step comes behind two barriers, the late ones' behind
+    // one.  The load of step t + 3 takes the place of step t - 1, which the late waves have read (lgkmcnt 0) before barrier 2 t.
+    static_assert(STEPS == 2 && STAGES == 4, "the schedule above");
+    constexpr int LOADS = Operand<T, AROW, false, BM, NT>::N + Operand<T, BROW, DUAL, BN, NT>::N;     // of a wave per step
+#pragma unroll
+    for (int t = 0; t < 3; ++t)
+      if (t < nk) stage(t);
+    if (nk > 2) wait_barrier<2 * LOADS>();
+    else wait_barrier<0>();
+    const bool late = wave >= 4;
+    if (late) asm volatile("s_barrier" ::: "memory");
+    for (int t = 0; t < nk; ++t) {
+      const char* cur = lds + (t % STAGES) * STAGE;
+      read(cur, 0);
+      read(cur, 1);
+      if (t + 3 < nk) {
+        stage(t + 3);
+        wait_barrier<2 * LOADS>();
+      } else if (t + 2 < nk) {
+        wait_barrier<LOADS>();
+      } else {
+        wait_barrier<0>();
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
+      multiply(0);
+      multiply(1);
+      __builtin_amdgcn_s_setprio(0);
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("s_barrier" ::: "memory");
+    }
+    if (!late) asm volatile("s_barrier" ::: "memory");
+  } else {
+    stage(0);
+    for (int t = 0; t < nk; ++t) {
+      const char* cur = lds + (t % STAGES) * STAGE;
+      __syncthreads();             // step t has arrived, and nobody reads the other half any more
+      if (t + 1 < nk) stage(t + 1);
+      read(cur, 0);
+#pragma unroll
+      for (int s = 0; s < STEPS; ++s) {      // operands of the next 16 k are read while the matrix unit works on these
+        if (s + 1 < STEPS) read(cur, s + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(s);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    __syncthreads();
   }
+  // Nobody reads operands any more: LDS now takes the output tile, so that it leaves (and dh arrives) in whole rows.  A lane holds 4
+  // columns of a row; granule and half of the granule are swizzled by the row.
+
+  constexpr int GO = BNO * (int)sizeof(T) / 16;      // granules of an output row
+  auto out_at = [](int r, int n) {                   // byte of columns n .. n + 3 (n a multiple of 4) of row r in the tile
+    if constexpr (sizeof(T) == 4) return (r * GO + place<GO>(r, n / 4)) * 16;
+    else return (r * GO + place<GO>(r, n / 8)) * 16 + (((n >> 2) ^ (r >> 4)) & 1) * 8;
+  };
+  // rows of the tile at `tile` to out + row * ldo + n0 (or fp16 / bf16 halves of a granule put back in order first)
+  auto store_tile = [&](const char* tile, T* out, long long ldo, int n_end, bool vec) {
+    constexpr int ITEMS = BM * GO / NT;
+#pragma unroll 4
+    for (int it = 0; it < ITEMS; ++it) {
+      const int at = it * NT + tid, r = at / GO, g = at % GO, m = m0 + r, n = n0 + g * P, left = n_end - n;
+      if (m >= p.M || left <= 0) continue;
+      u32x4 v = *(const u32x4*)(tile + (r * GO + place<GO>(r, g)) * 16);
+      if constexpr (sizeof(T) == 2)
+        if ((r >> 4) & 1) v = (u32x4){v[2], v[3], v[0], v[1]};
+      T* to = out + (long long)m * ldo + n;
+      if (vec && left >= P) {
+        *(u32x4*)to = v;
+      } else {
+        const T* e = (const T*)&v;
+#pragma unroll
+        for (int i = 0; i < P; ++i)
+          if (i < left) to[i] = e[i];
+      }
+    }
+  };
 
   if constexpr (DUAL) {
+    constexpr int TILE = BM * GO * 16;
+    static_assert((EPI == EPI_GATED ? 1 : 2) * TILE <= STAGES * STAGE, "the tiles fit where the operands were");
     const T* bias = (const T*)p.bias;
-    float* sums = (float*)lds;     // EPI_GATED_BWD: column sums of the waves, [WM][2][BNO]
-    if constexpr (EPI == EPI_GATED_BWD) __syncthreads();
+    float* sums = (float*)lds;     // EPI_GATED_BWD: column sums of the waves, [WM][2][BNO], once the tiles have left
+    if constexpr (EPI == EPI_GATED_BWD) {
+      constexpr int ITEMS = BM * GO / NT;
+#pragma unroll 4
+      for (int it = 0; it < ITEMS; ++it) {           // dh, in the layout of the output tile
+        const int at = it * NT + tid, r = at / GO, g = at % GO, m = m0 + r, n = n0 + g * P, left = p.N - n;
+        u32x4 v = (u32x4)(0u);
+        if (m < p.M && left > 0) {
+          const T* from = (const T*)p.dh + (long long)m * p.lddh + n;
+          if (p.vec_dh && left >= P) {
+            v = *(const u32x4*)from;
+          } else {
+            T* e = (T*)&v;
+#pragma unroll
+            for (int i = 0; i < P; ++i)
+              if (i < left) e[i] = from[i];
+          }
+        }
+        if constexpr (sizeof(T) == 2)
+          if ((r >> 4) & 1) v = (u32x4){v[2], v[3], v[0], v[1]};
+        *(u32x4*)(lds + (r * GO + place<GO>(r, g)) * 16) = v;
+      }
+      __syncthreads();
+    }
+    float sg[TN / 2][4][4] = {}, su[TN / 2][4][4] = {};
 #pragma unroll
     for (int pr = 0; pr < TN / 2; ++pr)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int nl = (wn * (TN / 2) + pr) * 32 + 8 * q + 4 * half, n = n0 + nl, left = p.N - n;
-        float bg[4] = {}, bu[4] = {}, sg[4] = {}, su[4] = {};
+        const int nl = (wn * (TN / 2) + pr) * 32 + 8 * q + 4 * half, left = p.N - n0 - nl;
+        float bg[4] = {}, bu[4] = {};
         if (bias && left > 0) {
-          load4(bias + n, bg, left, false);
-          load4(bias + p.F + n, bu, left, false);
+          load4(bias + n0 + nl, bg, left, false);
+          load4(bias + p.F + n0 + nl, bu, left, false);
         }
 #pragma unroll
         for (int j = 0; j < TM; ++j) {
-          const int m = m0 + (wm * TM + j) * 32 + (lane & 31);
-          if (m < p.M && left > 0) {
-            float g[4], u[4], o[4], o2[4];
+          const int r = (wm * TM + j) * 32 + (lane & 31);
+          char* at = lds + out_at(r, nl);
+          float g[4], u[4], o[4], o2[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) g[i] = acc[2 * pr][j][4 * q + i] + bg[i], u[i] = acc[2 * pr + 1][j][4 * q + i] + bu[i];
-            if constexpr (EPI == EPI_GATED) {
+          for (int i = 0; i < 4; ++i) g[i] = acc[2 * pr][j][4 * q + i] + bg[i], u[i] = acc[2 * pr + 1][j][4 * q + i] + bu[i];
+          if constexpr (EPI == EPI_GATED) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[i] = act_f<T>(g[i], p.act) * u[i];
-              store4((T*)p.out + (long long)m * p.ldo + n, o, left, p.vec_out);
-            } else {
-              float d[4];
-              load4((const T*)p.dh + (long long)m * p.lddh + n, d, left, p.vec_dh);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                float a, da;
-                act_both<T>(g[i], p.act, a, da);
-                o[i] = d[i] * u[i] * da, o2[i] = d[i] * a;
-                if (i < left) sg[i] += o[i], su[i] += o2[i];
-              }
-              T* row = (T*)p.out + (long long)m * p.ldo;
-              store4(row + n, o, left, p.vec_out);
-              store4(row + p.F + n, o2, left, p.vec_out);
-              if (left <= 4)       // the operand of the next products is whole granules wide: zeros behind the 2 F
-                for (int i = 0; i < p.out_pad; ++i) row[2 * p.F + i] = from_f<T>(0.f);
-            }
-          }
-        }
-        if constexpr (EPI == EPI_GATED_BWD) {
-          if (p.colsum) {
+            for (int i = 0; i < 4; ++i) o[i] = act_f<T>(g[i], p.act) * u[i];
+          } else {
+            float d[4];
+            load4((const T*)at, d, 4, true);         // zeros outside the matrix
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-#pragma unroll
-              for (int x = 1; x < 32; x <<= 1) sg[i] += __shfl_xor(sg[i], x), su[i] += __shfl_xor(su[i], x);
-              if ((lane & 31) == 0) sums[(wm * 2 + 0) * BNO + nl + i] = sg[i], sums[(wm * 2 + 1) * BNO + nl + i] = su[i];
+              float a, da;
+              act_both<T>(g[i], p.act, a, da);
+              o[i] = d[i] * u[i] * da, o2[i] = d[i] * a;
+              sg[pr][q][i] += o[i], su[pr][q][i] += o2[i];
             }
+            store4((T*)(at + TILE), o2, 4, true);
           }
+          store4((T*)at, o, 4, true);                // a lane's own place, also where it held dh
         }
       }
+    __syncthreads();
+    store_tile(lds, (T*)p.out, p.ldo, p.N, p.vec_out);
     if constexpr (EPI == EPI_GATED_BWD) {
+      store_tile(lds + TILE, (T*)p.out + p.F, p.ldo, p.N, p.vec_out2);
+      if (p.out_pad && n0 + BNO >= p.N)              // the operand of the next products is whole granules wide: zeros behind the 2 F
+        for (int r = tid; r < BM; r += NT)
+          if (m0 + r < p.M)
+            for (int i = 0; i < p.out_pad; ++i) ((T*)p.out)[(long long)(m0 + r) * p.ldo + 2 * p.F + i] = from_f<T>(0.f);
       if (p.colsum) {
+        __syncthreads();
+#pragma unroll
+        for (int pr = 0; pr < TN / 2; ++pr)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int nl = (wn * (TN / 2) + pr) * 32 + 8 * q + 4 * half + i;
+#pragma unroll
+              for (int x = 1; x < 32; x <<= 1) sg[pr][q][i] += __shfl_xor(sg[pr][q][i], x), su[pr][q][i] += __shfl_xor(su[pr][q][i], x);
+              if ((lane & 31) == 0) sums[(wm * 2 + 0) * BNO + nl] = sg[pr][q][i], sums[(wm * 2 + 1) * BNO + nl] = su[pr][q][i];
+            }
         __syncthreads();
         for (int i = tid; i < 2 * BNO; i += NT) {
           const int part = i / BNO, nl = i % BNO;
@@ -279,6 +406,21 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
         }
       }
     }
+  } else if constexpr (EPI == EPI_PLAIN) {
+    static_assert(BM * GO * 16 <= STAGES * STAGE, "the tile fits where the operands were");
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          float o[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = acc[i][j][4 * q + e];
+          store4((T*)(lds + out_at((wm * TM + j) * 32 + (lane & 31), (wn * TN + i) * 32 + 8 * q + 4 * half)), o, 4, true);
+        }
+    __syncthreads();
+    store_tile(lds, (T*)p.out, p.ldo, p.N, p.vec_out);
   } else {
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -292,22 +434,37 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
             float o[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[e] = acc[i][j][4 * q + e];
-            if constexpr (EPI == EPI_PARTIAL) store4((float*)p.out + ((long long)slice * p.M + m) * p.ldo + n, o, left, p.vec_out);
-            else store4((T*)p.out + (long long)m * p.ldo + n, o, left, p.vec_out);
+            store4((float*)p.out + ((long long)slice * p.M + m) * p.ldo + n, o, left, p.vec_out);
           }
         }
       }
   }
 }
 
-// out[i] = sum of the slices in order
-template <typename T>
+// out[i] = sum of the slices in order, W elements per thread (n a multiple of W)
+template <typename T, int W>
 __global__ __launch_bounds__(256) void sum_slices_kernel(const float* parts, T* out, int slices, long long n) {
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    float s = 0.f;
-    for (int k = 0; k < slices; ++k) s += parts[k * n + i];
-    out[i] = from_f<T>(s);
+  struct alignas(4 * W) In { float v[W]; };
+  struct alignas(W * sizeof(T)) Out { T v[W]; };
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n / W; i += (long long)gridDim.x * 256) {
+    float s[W] = {};
+#pragma unroll 8
+    for (int k = 0; k < slices; ++k) {
+      const In v = ((const In*)(parts + k * n))[i];
+#pragma unroll
+      for (int e = 0; e < W; ++e) s[e] += v.v[e];
+    }
+    Out o;
+#pragma unroll
+    for (int e = 0; e < W; ++e) o.v[e] = from_f<T>(s[e]);
+    ((Out*)out)[i] = o;
   }
+}
+template <typename T>
+void sum_slices(const float* parts, T* out, int slices, long long n, hipStream_t st) {
+  const unsigned grid = (unsigned)(n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096);
+  if (n % 4 == 0 && ff3d_aligned16(out)) sum_slices_kernel<T, 4><<<grid, 256, 0, st>>>(parts, out, slices, n);
+  else sum_slices_kernel<T, 1><<<grid, 256, 0, st>>>(parts, out, slices, n);
 }
 
 // rows of `cols` elements with stride ld into rows of whole granules, zeros behind
@@ -328,7 +485,7 @@ inline int grid_for(long long n) { return (int)(n < 1024ll * 256 ? (n + 255) / 2
 template <typename T, bool AROW, bool BROW, int WM, int WN, int TM, int TN, int EPI>
 int launch(GemmArgs a, hipStream_t st) {
   constexpr int BM = WM * TM * 32, BN = WN * TN * 32, BNO = (EPI == EPI_GATED || EPI == EPI_GATED_BWD) ? BN / 2 : BN;
-  constexpr int LDS = 2 * (BM + BN) * 128;
+  constexpr int LDS = stages_of(WM * WN) * (BM + BN) * step_bytes_of(WM * WN);
   auto k = gemm_kernel<T, AROW, BROW, WM, WN, TM, TN, EPI>;
   if (LDS > 64 * 1024) (void)hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   a.mt = cdiv(a.M, BM), a.nt = cdiv(a.N, BNO);
@@ -338,17 +495,26 @@ int launch(GemmArgs a, hipStream_t st) {
   return ff3d_launch_status();
 }
 
-// m rows per block of the gated kernel at these sizes (also the number of partial column sums)
+// Which tile, and into how many slices a long sum is cut: the least of an estimate in microseconds.  The most loaded CU runs `deep`
+// blocks, each (K / slices + 256) * per_k long (256 for filling and draining; per_k measured in bf16 on dx of 16384 x 1024 x 5472, one
+// 256 x 256 block or two 128 x 128 on each CU; fp32 runs at a quarter of that); slices cost their fp32 sums, written and read at 5 TB/s.
 struct Tile {
-  int id, bm, bn;
+  int id, bm, bn, slices;
 };
 template <typename T>
-Tile pick(long long M, long long N, bool dual, int slices = 1) {
-  const int bn_div = dual ? 2 : 1;
-  const Tile t[3] = {{0, 256, 256 / bn_div}, {1, 128, 128 / bn_div}, {2, 64, 128 / bn_div}};
-  for (int i = sizeof(T) == 4 ? 1 : 0; i < 2; ++i)
-    if ((long long)cdiv(M, t[i].bm) * cdiv(N, t[i].bn) * slices >= 224) return t[i];
-  return t[2];
+Tile pick(long long M, long long N, long long K, bool dual, bool cut) {
+  const int half = dual ? 2 : 1;
+  const struct { int bm, bn, per_cu; double per_k; } t[3] = {{256, 256 / half, 1, 0.033}, {128, 128 / half, 2, 0.020}, {64, 128 / half, 3, 0.013}};
+  Tile best = {2, t[2].bm, t[2].bn, 1};
+  double least = 1e300;
+  for (int i = sizeof(T) == 4 ? 1 : 0; i < 3; ++i)
+    for (int s = 1; s <= (cut ? 16 : 1) && (s == 1 || K / s >= 512); ++s) {
+      const long long blocks = (long long)cdiv(M, t[i].bm) * cdiv(N, t[i].bn) * s, slots = 256ll * t[i].per_cu;
+      const double deep = (double)(blocks / slots * t[i].per_cu + cdiv(blocks % slots, 256));
+      const double cost = deep * ((double)K / s + 256) * t[i].per_k * (sizeof(T) == 4 ? 4 : 1) + (s > 1 ? 5 + s * (double)M * N * 8 / 5e6 : 0);
+      if (cost < least) least = cost, best = {i, t[i].bm, t[i].bn, s};
+    }
+  return best;
 }
 
 template <typename T, bool AROW, bool BROW, int EPI>
@@ -376,15 +542,9 @@ Plan plan(long long M, int C, int F, int pack, bool bwd) {
   p.slices = 1, p.kslice = (int)M, p.mblocks = 0, p.d = p.part = p.colsum = 0;
   if (bwd) {
     p.d = take(M * p.ldd * sizeof(T));
-    p.mblocks = cdiv(M, pick<T>(M, F, true).bm);
+    p.mblocks = cdiv(M, pick<T>(M, F, p.Cp, true, false).bm);
     p.colsum = take((long long)p.mblocks * 2 * F * 4);
-    // dW has few tiles and long sums: cut them until the chip is full, but no shorter than 512 rows
-    const int bk = 128 / (int)sizeof(T);
-    const long long tiles = (long long)cdiv(2ll * F, 128) * cdiv(C, 128);
-    long long s = tiles >= 512 ? 1 : cdiv(512, tiles);
-    if (s > M / 512) s = M / 512;
-    if (s < 1) s = 1;
-    p.kslice = (int)align_up(cdiv(M, s), bk);
+    p.kslice = (int)align_up(cdiv(M, pick<T>(2ll * F, C, M, false, true).slices), 64);
     p.slices = cdiv(M, p.kslice);
     p.part = p.slices > 1 ? take((long long)p.slices * 2 * F * C * 4) : 0;
   }
@@ -413,7 +573,8 @@ GemmArgs gated_args(const T* x, long long ldx, const T* w, long long ldw, const 
   return a;
 }
 
-inline bool vec_ok(const void* p, long long ld, int size) { return ld % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (4 * size) == 0; }
+// rows of stride ld (elements) at p may be accessed 16 bytes at a time
+inline bool vec_ok(const void* p, long long ld, int size) { return ld * size % 16 == 0 && ff3d_aligned16(p); }
 
 template <typename T>
 int fwd(const T* x, long long ldx, const T* w, const T* bias, T* h, int M, int C, int F, int act, int pack, char* ws, hipStream_t st) {
@@ -422,7 +583,7 @@ int fwd(const T* x, long long ldx, const T* w, const T* bias, T* h, int M, int C
   pack_operands<T>(pl, pack, x, ldx, w, ldw, M, C, F, ws, st);
   GemmArgs a = gated_args<T>(x, ldx, w, ldw, bias, M, C, pl.Cp, F, act);
   a.out = h, a.ldo = F, a.vec_out = vec_ok(h, F, sizeof(T));
-  return dispatch<T, true, true, EPI_GATED>(pick<T>(M, F, true), a, st);
+  return dispatch<T, true, true, EPI_GATED>(pick<T>(M, F, pl.Cp, true, false), a, st);
 }
 
 template <typename T>
@@ -435,8 +596,8 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
   {
     GemmArgs a = gated_args<T>(x, ldx, w, ldw, bias, M, C, pl.Cp, F, act);
     a.out = d, a.ldo = pl.ldd, a.dh = dh, a.lddh = lddh, a.colsum = db ? (float*)(ws + pl.colsum) : nullptr;
-    a.out_pad = pl.ldd - 2 * F, a.vec_out = F % 4 == 0, a.vec_dh = vec_ok(dh, lddh, sizeof(T));
-    const int s = dispatch<T, true, true, EPI_GATED_BWD>(pick<T>(M, F, true), a, st);
+    a.out_pad = pl.ldd - 2 * F, a.vec_out = 1, a.vec_out2 = F * sizeof(T) % 16 == 0, a.vec_dh = vec_ok(dh, lddh, sizeof(T));
+    const int s = dispatch<T, true, true, EPI_GATED_BWD>(pick<T>(M, F, pl.Cp, true, false), a, st);
     if (s != FF3D_OK) return s;
   }
   const long long d_bytes = (long long)M * pl.ldd * sizeof(T);
@@ -446,7 +607,7 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
     a.b = (const char*)w, a.ldb = ldw, a.b_bytes = ((2ll * F - 1) * ldw + pl.Cp) * (long long)sizeof(T), a.bcols = pl.Cp;
     a.M = M, a.N = C, a.K = 2 * F, a.F = 0, a.slices = 1, a.kslice = (int)align_up(2ll * F, 64);
     a.out = dx, a.ldo = C, a.vec_out = vec_ok(dx, C, sizeof(T));
-    const int s = dispatch<T, true, false, EPI_PLAIN>(pick<T>(M, C, false), a, st);
+    const int s = dispatch<T, true, false, EPI_PLAIN>(pick<T>(M, C, 2ll * F, false, false), a, st);
     if (s != FF3D_OK) return s;
   }
   if (dw) {
@@ -454,19 +615,19 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
     a.a = (const char*)d, a.lda = pl.ldd, a.a_bytes = d_bytes, a.acols = pl.ldd;
     a.b = (const char*)x, a.ldb = ldx, a.b_bytes = ((M - 1) * ldx + pl.Cp) * (long long)sizeof(T), a.bcols = pl.Cp;
     a.M = 2 * F, a.N = C, a.K = M, a.slices = pl.slices, a.kslice = pl.kslice, a.ldo = C;
-    const Tile t = pick<T>(2ll * F, C, false, pl.slices);
+    const Tile t = pick<T>(2ll * F, C, M, false, true);
     int s;
     if (pl.slices > 1) {
-      a.out = ws + pl.part, a.vec_out = C % 4 == 0;
+      a.out = ws + pl.part, a.vec_out = C % 4 == 0;      // fp32
       s = dispatch<T, false, false, EPI_PARTIAL>(t, a, st);
-      if (s == FF3D_OK) sum_slices_kernel<T><<<grid_for(2ll * F * C), 256, 0, st>>>((const float*)(ws + pl.part), dw, pl.slices, 2ll * F * C);
+      if (s == FF3D_OK) sum_slices<T>((const float*)(ws + pl.part), dw, pl.slices, 2ll * F * C, st);
     } else {
       a.out = dw, a.vec_out = vec_ok(dw, C, sizeof(T));
       s = dispatch<T, false, false, EPI_PLAIN>(t, a, st);
     }
     if (s != FF3D_OK) return s;
   }
-  if (db) sum_slices_kernel<T><<<grid_for(2ll * F), 256, 0, st>>>((const float*)(ws + pl.colsum), db, pl.mblocks, 2ll * F);
+  if (db) sum_slices<T>((const float*)(ws + pl.colsum), db, pl.mblocks, 2ll * F, st);
   return ff3d_launch_status();
 }
 
