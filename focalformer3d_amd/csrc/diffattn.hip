@@ -24,7 +24,6 @@ using namespace mma;
 
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int JOIN = 1024;         // most slices of the keys
-constexpr float SLACK = 8.f;      // 2^8 above the largest term: far inside fp16's range for the rounded probabilities
 constexpr int ROWDATA = 6;        // fp32 values per row of the backward pass: reference 1, 2 of the exponentials (log2 units), D1, D2, 1 / sum 1, lam / sum 2
 
 struct Args {
@@ -35,7 +34,7 @@ struct Args {
   long long q_b, q_r, k_b, k_r, v_b, v_r, do_b, do_r;     // elements
   long long m_b, m_r;                                     // bytes
   char *out, *dq, *dk, *dv;
-  float *out2, *stat, *part, *rowdata;
+  float *out2, *stat, *part, *rowdata, *d2;
   int B, Nq, Nk, H, G, r, d, R, Rp, causal, mask4, splits, split_len, tiles;
   float scale, c;                 // c = scale * log2(e)
 };
@@ -176,7 +175,7 @@ __device__ __forceinline__ void exclude_cols_q(const Args& a, const uint8_t* mro
   }
 }
 
-template <typename T, int D, int KT>
+template <typename T, int D>
 __device__ __forceinline__ f32x16 scores(const char* tile, int kb, int map, const Op<T>* other, int lane) {
   constexpr int GR = 2 * D / Type<T>::PER16;
   f32x16 s = (f32x16)(0.f);
@@ -196,10 +195,10 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
   __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
 
-  int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
-  const int split = bid % a.splits;
-  bid /= a.splits;
-  const int tile = a.tiles - 1 - bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;   // causal: the long ones first
+  // Blocks go round the 8 XCDs: with the key head running fastest, an XCD works on few of them (their keys and values stay in its L2)
+  // and, under the causal order, on long and short tiles alike.
+  const int bgs = a.B * a.G, bg = blockIdx.x % bgs, b = bg / a.G, g = bg % a.G, split = blockIdx.x / bgs % a.splits;
+  const int tile = a.tiles - 1 - (int)(blockIdx.x / bgs / a.splits);       // causal: the long ones first
   const int row = tile * NW * 32 + wave * 32 + (lane & 31);
   const bool in = row < a.R;
   const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
@@ -257,7 +256,7 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
       if (jb >= kend) break;
       f32x16 s[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) s[m] = scores<T, D, KT>(kt, kb, m, q[m], lane);
+      for (int m = 0; m < 2; ++m) s[m] = scores<T, D>(kt, kb, m, q[m], lane);
       if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
       Op<T> p[2][2];
 #pragma unroll
@@ -266,9 +265,9 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
 #pragma unroll
         for (int e = 1; e < 16; ++e) x = fmaxf(x, s[m][e]);
         x = fmaxf(x, __shfl_xor(x, 32)) * a.c;
-        // the reference of the exponentials follows the maximum only when it lies 2^SLACK behind: what is kept in fp32 does not care,
-        // and the 2 D / 32 accumulators are rescaled a few times per row instead of at most steps
-        if (__any(x > ref[m] + SLACK)) {
+        // the reference of the exponentials is the running maximum: the largest probabilities are then just below 1, where rounding them
+        // costs least (a reference that lags by up to 2^8 saves 2 % of the time and makes the rounding error 15 % larger)
+        if (__any(x > ref[m])) {
           const float n = fmaxf(ref[m], x), f = exp2_(ref[m] - (n == -INFINITY ? 0.f : n));
           ref[m] = n;
           l[m] *= f;
@@ -417,15 +416,23 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
     for (int k = 0; k < ROWDATA; ++k) a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + row] = v[k];
 }
 
-// dlam[h] = -sum over batch and queries of D2: one block per head, fp64 sums in a fixed order
+// dlam[h] = -sum over batch and queries of P2 dP: D2 + (what the dq kernel found beyond it) / sum 2; one block per head, fp64 sums in
+// a fixed order
 template <typename T>
 __global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
   __shared__ double part[16];
   const int h = blockIdx.x, g = h / a.r, x = h % a.r;
   double s = 0.0;
   for (int b = 0; b < a.B; ++b) {
-    const float* p = a.rowdata + ((long long)(b * a.G + g) * ROWDATA + 3) * a.Rp + x;
-    for (int i = threadIdx.x; i < a.Nq; i += 1024) s += (double)p[(long long)i * a.r];
+    const int bg = b * a.G + g;
+    const float* d2 = a.rowdata + ((long long)bg * ROWDATA + 3) * a.Rp + x;
+    const float* inv = a.stat + ((long long)bg * 4 + 3) * a.R + x;
+    for (int i = threadIdx.x; i < a.Nq; i += 1024) {
+      const long long at = (long long)i * a.r;
+      double rest = 0.0;
+      for (int k = 0; k < a.splits; ++k) rest += (double)a.d2[((long long)k * a.B * a.G + bg) * a.Rp + x + at];
+      s += (double)d2[at] + rest * (double)inv[at];
+    }
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
@@ -445,10 +452,8 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1;
   __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
-  int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
-  const int split = bid % a.splits;
-  bid /= a.splits;
-  const int tile = a.tiles - 1 - bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;
+  const int bgs = a.B * a.G, bg = blockIdx.x % bgs, b = bg / a.G, g = bg % a.G, split = blockIdx.x / bgs % a.splits;
+  const int tile = a.tiles - 1 - (int)(blockIdx.x / bgs / a.splits);
   const int row = tile * 128 + wave * 32 + (lane & 31);
   const bool in = row < a.R;
   const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
@@ -470,7 +475,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
       go[st] = op<T>(load8<T>(po + e * (int)sizeof(T), in && e < 2 * a.d));
     }
   }
-  float rd[ROWDATA];
+  float rd[ROWDATA], rest = 0.f;
 #pragma unroll
   for (int k = 0; k < ROWDATA; ++k) rd[k] = a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + rowc];
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
@@ -519,7 +524,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
       if (jb >= kend) break;
       f32x16 s[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) s[m] = scores<T, D, KT>(kt, kb, m, q[m], lane);
+      for (int m = 0; m < 2; ++m) s[m] = scores<T, D>(kt, kb, m, q[m], lane);
       if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
@@ -532,6 +537,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
           // 1 / sum and -lam are factors of the whole column: they wait for the end
           const float ds = exp2_(fmaf(s[m][e], a.c, -rd[m])) * (dp[e] - rd[2 + m]);
           s[m][e] = ds;
+          if (m == 1) rest += ds;
           top[m] = fmaxf(top[m], fabsf(ds));
         }
 #pragma unroll
@@ -548,6 +554,12 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
     }
   }
   if (!in) return;
+  if (a.d2) {
+    // sum_j P2 dP in fp32 = D2 + sum_j P2 (dP - D2): dlam does not carry the rounding of the probabilities that O2 was made of
+    rest += __shfl_xor(rest, 32);
+    if (half == 0) a.d2[((long long)split * bgs + bg) * a.Rp + row] = rest;
+  }
+  if (!a.dq) return;
   const long long at = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d, all = (long long)a.B * a.Nq * a.H * 2 * a.d;
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
@@ -566,36 +578,60 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   }
 }
 
+// d = 64 in 16 bits (WIDE): the accumulators of 32 keys take 128 registers, and with the keys and values as operands beside them one wave
+// would fill a SIMD alone, its vector and matrix work in turn.  There the block's keys and values stay in LDS, 8 waves share them in
+// pairs - one takes the even, one the odd tiles of 32 rows - and the pair's sums are joined at the end.
 template <typename T, int D>
-__global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel(Args a) {
-  constexpr int NT = 256, QR = (sizeof(T) == 2 && D == 16) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = QR * GR * 16;
+constexpr bool wide_v = D == 64 && sizeof(T) == 2;
+
+template <typename T, int D>
+__global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : waves_of(D, sizeof(T), false))) void dkv_kernel(Args a) {
+  constexpr bool WIDE = wide_v<T, D>;
+  constexpr int NT = WIDE ? 512 : 256, QR = (sizeof(T) == 2 && D != 32) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = QR * GR * 16;
   constexpr int RG = ROWDATA * QR / 4, STAGE = 2 * BYTES + (RG + 63) / 64 * 1024;      // RG granules of row values
   constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1, VT = 2 * D / 32;
-  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE];
+  constexpr int KBYTES = WIDE ? 128 * GR * 16 : 0;   // keys, and values, of the block
+  __shared__ __attribute__((aligned(16))) char lds[2 * STAGE + 2 * KBYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
-  int bid = (int)ff3d_xcd_remap(blockIdx.x, gridDim.x);
-  const int split = bid % a.splits;
-  bid /= a.splits;
-  const int tile = bid % a.tiles, bg = bid / a.tiles, b = bg / a.G, g = bg % a.G;
+  const int bgs = a.B * a.G, bg = blockIdx.x % bgs, b = bg / a.G, g = bg % a.G, split = blockIdx.x / bgs % a.splits;
+  const int tile = blockIdx.x / bgs / a.splits;
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
-  const int jw = tile * 128 + wave * 32, j = jw + (lane & 31);
+  const int kw = wave & 3, jw = tile * 128 + kw * 32, j = jw + (lane & 31);
   const bool in = j < limit;
 
   const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
   const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
-  Op<T> k[2][ST], v[VS];
-#pragma unroll
-  for (int m = 0; m < 2; ++m)
-#pragma unroll
-    for (int st = 0; st < ST; ++st) {
-      const int e = 16 * st + 8 * half;
-      k[m][st] = op<T>(load8<T>(kbase + ((long long)j * a.k_r + m * a.d + e) * (long long)sizeof(T), in && e < a.d));
+  const long long kld = a.k_r * (long long)sizeof(T), vld = a.v_r * (long long)sizeof(T);
+  char* kt = lds + 2 * STAGE;
+  char* vt = kt + KBYTES;
+  Op<T> k[2][WIDE ? 1 : ST], v[WIDE ? 1 : VS];
+  if constexpr (WIDE) {
+    if (tile * 128 < limit) {
+      Tile<T, D, 128, NT, true>::keys(kt, kbase, kld, tile * 128, limit, a.d, tid, wave);
+      Tile<T, D, 128, NT, false>::keys(vt, vbase, vld, tile * 128, limit, a.d, tid, wave);
     }
+  } else {
 #pragma unroll
-  for (int st = 0; st < VS; ++st) {
-    const int e = 16 * st + 8 * half;
-    v[st] = op<T>(load8<T>(vbase + ((long long)j * a.v_r + e) * (long long)sizeof(T), in && e < 2 * a.d));
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int st = 0; st < ST; ++st) {
+        const int e = 16 * st + 8 * half;
+        k[m][st] = op<T>(load8<T>(kbase + ((long long)j * a.k_r + m * a.d + e) * (long long)sizeof(T), in && e < a.d));
+      }
+#pragma unroll
+    for (int st = 0; st < VS; ++st) {
+      const int e = 16 * st + 8 * half;
+      v[st] = op<T>(load8<T>(vbase + ((long long)j * a.v_r + e) * (long long)sizeof(T), in && e < 2 * a.d));
+    }
   }
+  auto key = [&](int m, int st) {
+    if constexpr (WIDE) return op<T>(row_frag<T, GR>(kt, kw * 32 + (lane & 31), m * D + 16 * st, half));
+    else return k[m][st];
+  };
+  auto value = [&](int st) {
+    if constexpr (WIDE) return op<T>(row_frag<T, GR>(vt, kw * 32 + (lane & 31), 16 * st, half));
+    else return v[st];
+  };
 
   f32x16 dv[VT], dk[2][QT];
 #pragma unroll
@@ -638,10 +674,16 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
     __syncthreads();
     if (t + 1 < nt) stage(lds + ((t + 1) & 1) * STAGE, row0 + QR);
 #pragma unroll
-    for (int rb = 0; rb < QR / 32; ++rb) {
+    for (int rb_ = 0; rb_ < (WIDE ? 1 : QR / 32); ++rb_) {
+      const int rb = WIDE ? wave >> 2 : rb_;
       f32x16 s[2];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) s[m] = scores<T, D, QR>(qt, rb, m, k[m], lane);
+      for (int m = 0; m < 2; ++m) {
+        s[m] = (f32x16)(0.f);
+#pragma unroll
+        for (int st = 0; st < ST; ++st)
+          s[m] = mfma_step<T>(op<T>(row_frag<T, GR>(qt, rb * 32 + (lane & 31), m * D + 16 * st, half)), key(m, st), s[m]);
+      }
       // (row, key) pairs to leave out: keys past the limit, the causal order, the mask
       const bool some = a.mask || jw + 31 >= limit || (a.causal && jw + 31 > (row0 + rb * 32) / a.r + shift);
       if (some) {
@@ -655,7 +697,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
       }
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
-      for (int st = 0; st < VS; ++st) dp = mfma_step<T>(op<T>(row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * st, half)), v[st], dp);
+      for (int st = 0; st < VS; ++st) dp = mfma_step<T>(op<T>(row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * st, half)), value(st), dp);
       f32x16 w;
       float top[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -693,6 +735,38 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
       }
     }
   }
+  const float fv = sv.undo(), fk[2] = {a.scale * sk[0].undo(), a.scale * sk[1].undo()};
+#pragma unroll
+  for (int x = 0; x < VT; ++x) dv[x] *= fv;
+#pragma unroll
+  for (int m = 0; m < 2; ++m)
+#pragma unroll
+    for (int x = 0; x < QT; ++x) dk[m][x] *= fk[m];
+  if constexpr (WIDE) {            // join the pairs
+    float* p = (float*)lds + (kw * (VT + 2 * QT) * 16) * 64 + lane;
+    static_assert(4 * (VT + 2 * QT) * 16 * 256 <= (int)sizeof(lds), "the odd waves' sums");
+    __syncthreads();
+    if (wave >= 4) {
+#pragma unroll
+      for (int x = 0; x < VT; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[(x * 16 + e) * 64] = dv[x][e];
+#pragma unroll
+      for (int x = 0; x < 2 * QT; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[((VT + x) * 16 + e) * 64] = dk[x / QT][x % QT][e];
+    }
+    __syncthreads();
+    if (wave >= 4) return;
+#pragma unroll
+    for (int x = 0; x < VT; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dv[x][e] += p[(x * 16 + e) * 64];
+#pragma unroll
+    for (int x = 0; x < 2 * QT; ++x)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dk[x / QT][x % QT][e] += p[((VT + x) * 16 + e) * 64];
+  }
   if (j >= a.Nk) return;           // keys past their sequence's length get zeros
   const long long at = (((long long)b * a.Nk + j) * a.G + g) * 2 * a.d, all = (long long)a.B * a.Nk * a.G * 2 * a.d;
 #pragma unroll
@@ -700,22 +774,20 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), false)) void dkv_kernel
 #pragma unroll
     for (int y = 0; y < 4; ++y) {
       const int e = x * 32 + 8 * y + 4 * half;
-      const float f = sv.undo();
       if (e < 2 * a.d) {
-        if (a.splits > 1) put4(a.part + (2ll * split + 1) * all + at + e, dv[x][4 * y] * f, dv[x][4 * y + 1] * f, dv[x][4 * y + 2] * f, dv[x][4 * y + 3] * f);
-        else put4((T*)a.dv + at + e, dv[x][4 * y] * f, dv[x][4 * y + 1] * f, dv[x][4 * y + 2] * f, dv[x][4 * y + 3] * f);
+        if (a.splits > 1) put4(a.part + (2ll * split + 1) * all + at + e, dv[x][4 * y], dv[x][4 * y + 1], dv[x][4 * y + 2], dv[x][4 * y + 3]);
+        else put4((T*)a.dv + at + e, dv[x][4 * y], dv[x][4 * y + 1], dv[x][4 * y + 2], dv[x][4 * y + 3]);
       }
     }
 #pragma unroll
   for (int m = 0; m < 2; ++m) {
-    const float f = a.scale * sk[m].undo();
 #pragma unroll
     for (int x = 0; x < QT; ++x)
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         const int col = (D >= 32 ? m * D : 0) + x * 32 + 8 * y + 4 * half, w = col % D;
         if (col / D == m && w < a.d) {
-          const float o0 = dk[m][x][4 * y] * f, o1 = dk[m][x][4 * y + 1] * f, o2 = dk[m][x][4 * y + 2] * f, o3 = dk[m][x][4 * y + 3] * f;
+          const float o0 = dk[m][x][4 * y], o1 = dk[m][x][4 * y + 1], o2 = dk[m][x][4 * y + 2], o3 = dk[m][x][4 * y + 3];
           if (a.splits > 1) put4(a.part + 2ll * split * all + at + m * a.d + w, o0, o1, o2, o3);
           else put4((T*)a.dk + at + m * a.d + w, o0, o1, o2, o3);
         }
@@ -764,7 +836,7 @@ Split split_of(const ff3d_diff_attention_t& p) {
 // blocks, to slices of at least 128 rows or keys; the slices' fp32 sums are added in order.  Both kernels use one place for them.
 struct BwdSplit {
   int q, k;
-  long long rowdata, total;        // bytes
+  long long rowdata, d2, total;    // bytes
 };
 BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
@@ -778,7 +850,8 @@ BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   s.k = slices(bg * cdiv(p.Nk, 128), R);
   s.rowdata = bg * ROWDATA * ((R + 63) / 64 * 64) * 4;
   const long long q = s.q > 1 ? s.q * (long long)p.B * p.Nq * p.heads * 2 * p.d * 4 : 0, k = s.k > 1 ? 2ll * s.k * p.B * p.Nk * p.kv_heads * 2 * p.d * 4 : 0;
-  s.total = s.rowdata + (q > k ? q : k);
+  s.d2 = s.q * bg * ((R + 63) / 64 * 64) * 4;
+  s.total = s.rowdata + s.d2 + (q > k ? q : k);
   return s;
 }
 inline int sum_grid(long long n) { return (int)(n / 1024 + 1 < 2048 ? n / 1024 + 1 : 2048); }
@@ -829,23 +902,24 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   const BwdSplit s = bwd_split_of(p);
   const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128) * s.q, kb = bg * cdiv(a.Nk, 128) * s.k;
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
-  a.part = a.rowdata + s.rowdata / 4;
+  a.d2 = dlam ? a.rowdata + s.rowdata / 4 : nullptr;
+  a.part = a.rowdata + (s.rowdata + s.d2) / 4;
   rows_kernel<T><<<(unsigned)cdiv(rows, 16), 256, 0, st>>>(a);
-  if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
   if (a.dk) {
     const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;
     a.tiles = cdiv(a.Nk, 128), a.splits = s.k;
-    dkv_kernel<T, D><<<(unsigned)kb, 256, 0, st>>>(a);
+    dkv_kernel<T, D><<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
     if (s.k > 1) {
       sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dk, n, 2 * n, s.k);
       sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part + n, (T*)a.dv, n, 2 * n, s.k);
     }
   }
-  if (a.dq) {
+  if (a.dq || dlam) {
     const long long n = (long long)a.B * a.Nq * a.H * 2 * a.d;
     a.tiles = cdiv(a.R, 128), a.splits = s.q;
     dq_kernel<T, D><<<(unsigned)qb, 256, 0, st>>>(a);
-    if (s.q > 1) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, n, n, s.q);
+    if (s.q > 1 && a.dq) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, n, n, s.q);
+    if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
   }
   return ff3d_launch_status();
 }

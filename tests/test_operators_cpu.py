@@ -86,7 +86,7 @@ def test_diff_attention_entry_checks_its_arguments():
     p = _lib.DiffAttention(**{**ok, 'Nq': 1, 'Nk': 2048})
     assert lib.ff3d_diff_attention_workspace_bytes(p, 0) == 8 * 4 * 1 * (4 * 16 + 4) * 4          # 8 slices of 256 keys, 4 rows
     assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 0) == 0
-    assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 1) == 4 * 6 * 64 * 4  # rows rounded up to 64
+    assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 1) == 4 * (6 + 1) * 64 * 4  # rows rounded up to 64
 
     def bwd(out=P, out2=P, lse=P, dout=P, db=320, dr=64, dq=P, dk=P, dv=P, dlam=P, ws=P, **k):
         return lib.ff3d_diff_attention_bwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, dout, db, dr, dq, dk, dv, dlam, ws, None)
