@@ -49,7 +49,7 @@ struct Scaled {
   template <int N>
   __device__ __forceinline__ void see(float mx, f32x16* acc) {
     if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
-      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      mx = max_halves(mx);
       const bool need = mx * s > 32768.f || (s == 0.f && mx > 0.f);
       if (__any(need)) {
         if (need) {
@@ -142,36 +142,47 @@ __device__ __forceinline__ void put4(T* p, float a, float b, float c, float d) {
   *(Four<T>*)p = f;
 }
 
+// The n-th row tile to start.  Under the causal order the last tiles are the longest: they come first, and where all blocks start at
+// once, two on a CU, the second of a CU's pair is as short as the first is long.
+__device__ __forceinline__ int row_tile(const Args& a, int n) {
+  const int first = (int)(gridDim.x <= 512 ? 256 / (gridDim.x / a.tiles) : a.tiles);     // tiles of the first block of every CU
+  return n < first ? a.tiles - 1 - n : n - first;
+}
+
 __device__ __forceinline__ int key_limit(const Args& a, int b) {
   int n = a.Nk;
   if (a.lens) n = max(0, min(n, a.lens[b]));
   return n;
 }
 
-// whether keys j .. j + 3 are blocked for a row of the mask, as 4 bits
-__device__ __forceinline__ unsigned blocked4(const Args& a, const uint8_t* mrow, int j) {
-  unsigned bits = 0;
-  if (a.mask4 && j + 3 < a.Nk) {
-    const unsigned w = *(const unsigned*)(mrow + j);
+// The mask bytes of a row for a half column of a tile of 32 keys: word q holds keys j0 + 8 q + 4 half .. + 3, as the accumulator does.
+struct MaskWords {
+  unsigned w[4];
+  __device__ __forceinline__ void load(const Args& a, const uint8_t* mrow, int j0, int half) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) bits |= (((w >> (8 * e)) & 0xff) ? 1u : 0u) << e;
-  } else {
+    for (int q = 0; q < 4; ++q) {
+      const int j = j0 + 8 * q + 4 * half;
+      if (a.mask4 && j + 3 < a.Nk) {
+        w[q] = *(const unsigned*)(mrow + j);
+      } else {
+        w[q] = 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (j + e < a.Nk && mrow[j + e]) bits |= 1u << e;
+        for (int e = 0; e < 4; ++e)
+          if (j + e < a.Nk) w[q] |= (unsigned)mrow[j + e] << (8 * e);
+      }
+    }
   }
-  return bits;
-}
+};
 
 // Excludes keys from a 32 x 32 tile with queries as columns: both maps' scores become -inf.
-__device__ __forceinline__ void exclude_cols_q(const Args& a, const uint8_t* mrow, f32x16& s1, f32x16& s2, int j0, int jlast, int half, bool use_mask) {
+__device__ __forceinline__ void exclude_cols_q(const MaskWords& mask, bool use_mask, f32x16& s1, f32x16& s2, int j0, int jlast, int half) {
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int j = j0 + 8 * q + 4 * half;
-    const unsigned m = use_mask ? blocked4(a, mrow, j) : 0u;
+    const unsigned m = use_mask ? mask.w[q] : 0u;
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (j + e > jlast || (m >> e & 1)) s1[4 * q + e] = -INFINITY, s2[4 * q + e] = -INFINITY;
+      if (j + e > jlast || (m >> (8 * e) & 0xff)) s1[4 * q + e] = -INFINITY, s2[4 * q + e] = -INFINITY;
   }
 }
 
@@ -188,18 +199,29 @@ __device__ __forceinline__ f32x16 scores(const char* tile, int kb, int map, cons
 constexpr int waves_of(int D, int size, bool fits64) { return size == 4 ? (D <= 16 ? 2 : 1) : (D <= 32 || fits64 ? 2 : 1); }
 
 // ---- forward ------------------------------------------------------------------------------------------------------------------
-template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_kernel(Args a) {
-  constexpr int NT = NW * 64, KT = (sizeof(T) == 2 && NW > 1) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
-  constexpr int VT = 2 * D / 32, ST = D / 16;
-  __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
+// ROWS: the 4 waves of a block take 32 rows each and share the keys and values.  Otherwise, where there are few rows, they take the
+// same 32 rows and every NW-th tile of 32 keys, with LDS of their own and no barrier, and join what they found at the end.
+template <typename T, int D, bool ROWS>
+struct FwdShape {
+  static constexpr int NW = !ROWS && D == 64 && sizeof(T) == 4 ? 2 : 4, KT = ROWS && sizeof(T) == 2 ? 64 : 32;
+  static constexpr int BYTES = KT * (2 * D / Type<T>::PER16) * 16, LDS = (ROWS ? 4 : 4 * NW) * BYTES;
+};
+
+template <typename T, int D, bool ROWS, bool MASK>
+__global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeof(T), ROWS))) void fwd_kernel(Args a) {
+  typedef FwdShape<T, D, ROWS> Shape;
+  constexpr int NW = Shape::NW, NT = ROWS ? NW * 64 : 64, KT = Shape::KT, GR = 2 * D / Type<T>::PER16, BYTES = Shape::BYTES;
+  constexpr int VT = 2 * D / 32, ST = D / 16, BLOCK_ROWS = ROWS ? NW * 32 : 32;
+  __shared__ __attribute__((aligned(16))) char lds[Shape::LDS];
+  __shared__ float found[ROWS ? 1 : NW][4][64];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
+  const int tid = ROWS ? threadIdx.x : lane, lwave = ROWS ? wave : 0;        // of the waves that load a tile together
 
   // Blocks go round the 8 XCDs: with the key head running fastest, an XCD works on few of them (their keys and values stay in its L2)
   // and, under the causal order, on long and short tiles alike.
   const int bgs = a.B * a.G, bg = blockIdx.x % bgs, b = bg / a.G, g = bg % a.G, split = blockIdx.x / bgs % a.splits;
-  const int tile = a.tiles - 1 - (int)(blockIdx.x / bgs / a.splits);       // causal: the long ones first
-  const int row = tile * NW * 32 + wave * 32 + (lane & 31);
+  const int tile = row_tile(a, blockIdx.x / bgs / a.splits);
+  const int row0 = tile * BLOCK_ROWS + (ROWS ? wave * 32 : 0), row = row0 + (lane & 31);
   const bool in = row < a.R;
   const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
 
@@ -216,19 +238,20 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
   }
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
   int kend = limit;
-  if (a.causal) kend = min(kend, min(a.R - 1, tile * NW * 32 + NW * 32 - 1) / a.r + shift + 1);
+  if (a.causal) kend = min(kend, min(a.R - 1, tile * BLOCK_ROWS + BLOCK_ROWS - 1) / a.r + shift + 1);
   const int kbeg = split * a.split_len;
   kend = min(kend, kbeg + a.split_len);
   const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;       // last key of this lane's row
-  const int wave_first = a.causal ? min(limit - 1, min(tile * NW * 32 + wave * 32, a.R - 1) / a.r + shift) : limit - 1;   // smallest in the wave
-  const uint8_t* mrow = a.mask ? a.mask + b * a.m_b + i * a.m_r : nullptr;
+  const int wave_first = a.causal ? min(limit - 1, min(row0, a.R - 1) / a.r + shift) : limit - 1;   // smallest in the wave
+  const uint8_t* mrow = MASK ? a.mask + b * a.m_b + i * a.m_r : nullptr;
 
   f32x16 o[2][VT];
 #pragma unroll
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int t = 0; t < VT; ++t) o[m][t] = (f32x16)(0.f);
-  float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  float ref[2] = {-INFINITY, -INFINITY}, top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  MaskWords mask_next;             // of the next 32 keys, asked for one step ahead
 
   const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
   const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
@@ -236,40 +259,49 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
   typedef Tile<T, D, KT, NT, true> KTile;
   typedef Tile<T, D, KT, NT, false> VTile;
   const int nt = kend > kbeg ? (kend - kbeg + KT - 1) / KT : 0;
-  if (nt > 0) {
-    KTile::keys(lds, kbase, kld, kbeg, limit, a.d, tid, wave);
-    VTile::keys(lds + BYTES, vbase, vld, kbeg, limit, a.d, tid, wave);
+  constexpr int STRIDE = ROWS ? 1 : NW;
+  char* my = lds + (ROWS ? 0 : wave * 4 * BYTES);
+  auto stage = [&](int n, int j) {
+    KTile::keys(my + (n & 1) * 2 * BYTES, kbase, kld, j, limit, a.d, tid, lwave);
+    VTile::keys(my + (n & 1) * 2 * BYTES + BYTES, vbase, vld, j, limit, a.d, tid, lwave);
+  };
+  const int t0 = ROWS ? 0 : wave;
+  if (t0 < nt) {
+    stage(0, kbeg + t0 * KT);
+    if (MASK) mask_next.load(a, mrow, kbeg + t0 * KT, half);
   }
-  for (int t = 0; t < nt; ++t) {
+  for (int t = t0, n = 0; t < nt; t += STRIDE, ++n) {
     const int j0 = kbeg + t * KT;
-    const char* kt = lds + (t & 1) * 2 * BYTES;
+    const char* kt = my + (n & 1) * 2 * BYTES;
     const char* vt = kt + BYTES;
-    __syncthreads();
-    if (t + 1 < nt) {
-      char* nx = lds + ((t + 1) & 1) * 2 * BYTES;
-      KTile::keys(nx, kbase, kld, j0 + KT, limit, a.d, tid, wave);
-      VTile::keys(nx + BYTES, vbase, vld, j0 + KT, limit, a.d, tid, wave);
-    }
+    if constexpr (ROWS) __syncthreads();
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");        // this wave's own loads, and its reads of the other half
+    if (t + STRIDE < nt) stage(n + 1, j0 + STRIDE * KT);
 #pragma unroll
     for (int kb = 0; kb < KT / 32; ++kb) {
       const int jb = j0 + kb * 32;
       if (jb >= kend) break;
+      const MaskWords mask = mask_next;
+      if (MASK) mask_next.load(a, mrow, jb + (ROWS ? 32 : STRIDE * KT), half);
       f32x16 s[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) s[m] = scores<T, D>(kt, kb, m, q[m], lane);
-      if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
+      if (MASK || jb + 31 > wave_first) exclude_cols_q(mask, MASK, s[0], s[1], jb, jlast, half);
+      const bool exact = !ROWS || (jb - kbeg) % 128 == 0;
       Op<T> p[2][2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
         float x = s[m][0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) x = fmaxf(x, s[m][e]);
-        x = fmaxf(x, __shfl_xor(x, 32)) * a.c;
-        // the reference of the exponentials is the running maximum: the largest probabilities are then just below 1, where rounding them
-        // costs least (a reference that lags by up to 2^8 saves 2 % of the time and makes the rounding error 15 % larger)
-        if (__any(x > ref[m])) {
-          const float n = fmaxf(ref[m], x), f = exp2_(ref[m] - (n == -INFINITY ? 0.f : n));
-          ref[m] = n;
+        x = max_halves(x) * a.c;
+        // The reference of the exponentials follows the running maximum every fourth step, and at once only where it lies more than 2^8
+        // behind.  Following it costs 2 D / 32 accumulators; letting it lag for good (only the 2^8) makes the rounding error of the
+        // probabilities 20 % larger, since the largest of them are then spread over a binade instead of sitting just below 1.
+        top[m] = fmaxf(top[m], x);
+        if (__any(top[m] > ref[m] + (exact ? 0.f : 8.f))) {
+          const float n2 = fmaxf(ref[m], top[m]), f = exp2_(ref[m] - (n2 == -INFINITY ? 0.f : n2));
+          ref[m] = n2;
           l[m] *= f;
 #pragma unroll
           for (int v = 0; v < VT; ++v) o[m][v] *= f;
@@ -295,45 +327,95 @@ __global__ __launch_bounds__(NW * 64, waves_of(D, sizeof(T), NW == 4)) void fwd_
         }
     }
   }
-  l[0] += __shfl_xor(l[0], 32);
-  l[1] += __shfl_xor(l[1], 32);
-  if (!in) return;
-  if (a.splits > 1) {              // [split][bg][row]: O1, O2 (2 d each), then maximum and sum of both maps
-    float* p = a.part + (((long long)split * a.B * a.G + bg) * a.R + row) * (4 * a.d + 4);
-    if (half == 0)
+  l[0] = sum_halves(l[0]), l[1] = sum_halves(l[1]);
+
+  // what leaves the block: columns e .. e + 3 of O1 and O2 of this lane's row
+  float inv[2];
+  const float lam = to_f(((const T*)a.lam)[h]);
+  const long long at = ((long long)b * a.Nq + i) * a.H + h;
+  float* part = a.part + (((long long)split * bgs + bg) * a.R + row) * (4 * a.d + 4);      // [split][bg][row]: O1, O2, references and sums
+  auto emit = [&](int e, const float* o1, const float* o2) {
+    if (!in || e >= 2 * a.d) return;
+    if (a.splits > 1) {
+      if (l[0] == 0.f && l[1] == 0.f) return;
+      put4(part + e, o1[0], o1[1], o1[2], o1[3]);
+      put4(part + 2 * a.d + e, o2[0], o2[1], o2[2], o2[3]);
+      return;
+    }
+    float y[4], z[4];
 #pragma unroll
-      for (int m = 0; m < 2; ++m) p[4 * a.d + 2 * m] = ref[m], p[4 * a.d + 2 * m + 1] = l[m];
-    if (l[0] == 0.f && l[1] == 0.f) return;
+    for (int k = 0; k < 4; ++k) z[k] = o2[k] * inv[1], y[k] = o1[k] * inv[0] - lam * z[k];
+    put4((T*)a.out + at * 2 * a.d + e, y[0], y[1], y[2], y[3]);
+    if (a.out2) put4(a.out2 + at * 2 * a.d + e, z[0], z[1], z[2], z[3]);
+  };
+  auto emit_row = [&] {
+    if (!in || half) return;
+    if (a.splits > 1) {
 #pragma unroll
-    for (int m = 0; m < 2; ++m)
+      for (int m = 0; m < 2; ++m) part[4 * a.d + 2 * m] = ref[m], part[4 * a.d + 2 * m + 1] = l[m];
+    } else if (a.stat) {
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        a.stat[((long long)bg * 4 + m) * a.R + row] = ref[m] == -INFINITY ? 0.f : ref[m];
+        a.stat[((long long)bg * 4 + 2 + m) * a.R + row] = inv[m];
+      }
+    }
+  };
+  if constexpr (ROWS) {
+#pragma unroll
+    for (int m = 0; m < 2; ++m) inv[m] = l[m] == 0.f ? 0.f : 1.f / l[m];
+#pragma unroll
+    for (int v = 0; v < VT; ++v)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        float o1[4], o2[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o1[k] = o[0][v][4 * x + k], o2[k] = o[1][v][4 * x + k];
+        emit(v * 32 + 8 * x + 4 * half, o1, o2);
+      }
+    emit_row();
+  } else {
+    // a wave's sums to LDS; then each takes a share of the elements, weighted by 2^(reference - the largest)
+    static_assert(NW * 2 * VT * 16 * 256 <= Shape::LDS, "the sums fit where the keys and values were");
+    __syncthreads();
+    float* sums = (float*)lds + lane;
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      found[wave][m][lane] = ref[m], found[wave][2 + m][lane] = l[m];
 #pragma unroll
       for (int v = 0; v < VT; ++v)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int e = v * 32 + 8 * x + 4 * half;
-          if (e < 2 * a.d) put4(p + m * 2 * a.d + e, o[m][v][4 * x], o[m][v][4 * x + 1], o[m][v][4 * x + 2], o[m][v][4 * x + 3]);
-        }
-    return;
-  }
-  const float i0 = l[0] == 0.f ? 0.f : 1.f / l[0], i1 = l[1] == 0.f ? 0.f : 1.f / l[1], lam = to_f(((const T*)a.lam)[h]);
-  const long long at = ((long long)b * a.Nq + i) * a.H + h;
-#pragma unroll
-  for (int v = 0; v < VT; ++v)
-#pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int e = v * 32 + 8 * x + 4 * half;
-      if (e < 2 * a.d) {
-        float y[4], z[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) z[k] = o[1][v][4 * x + k] * i1, y[k] = o[0][v][4 * x + k] * i0 - lam * z[k];
-        put4((T*)a.out + at * 2 * a.d + e, y[0], y[1], y[2], y[3]);
-        if (a.out2) put4(a.out2 + at * 2 * a.d + e, z[0], z[1], z[2], z[3]);
-      }
+        for (int e = 0; e < 16; ++e) sums[(((wave * 2 + m) * VT + v) * 16 + e) * 64] = o[m][v][e];
     }
-  if (a.stat && half == 0) {
+    __syncthreads();
+    float w[2][NW];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) a.stat[((long long)bg * 4 + m) * a.R + row] = ref[m] == -INFINITY ? 0.f : ref[m];
-    a.stat[((long long)bg * 4 + 2) * a.R + row] = i0, a.stat[((long long)bg * 4 + 3) * a.R + row] = i1;
+    for (int m = 0; m < 2; ++m) {
+      float r = -INFINITY;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) r = fmaxf(r, found[k][m][lane]);
+      l[m] = 0.f;
+#pragma unroll
+      for (int k = 0; k < NW; ++k) {
+        const float rk = found[k][m][lane];
+        w[m][k] = rk == -INFINITY ? 0.f : exp2_(rk - r);
+        l[m] += w[m][k] * found[k][2 + m][lane];
+      }
+      ref[m] = r;
+      inv[m] = l[m] == 0.f ? 0.f : 1.f / l[m];
+    }
+    for (int it = wave; it < VT * 4; it += NW) {
+      const int v = it >> 2, x = it & 3;
+      float y[2][4] = {};
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int k = 0; k < NW; ++k)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[m][e] = fmaf(w[m][k], sums[(((k * 2 + m) * VT + v) * 16 + 4 * x + e) * 64], y[m][e]);
+      emit(v * 32 + 8 * x + 4 * half, y[0], y[1]);
+    }
+    if (wave == 0) emit_row();
   }
 }
 
@@ -369,7 +451,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
   __syncthreads();
   const int w4 = 4 * a.d, e = tid % w4, groups = 256 / w4, m = e >= 2 * a.d;
   float acc = 0.f;
-#pragma unroll 4
+#pragma unroll 8
   for (int s = tid / w4; s < a.splits; s += groups) {
     const float w = wt[m][s];
     if (w != 0.f) acc = fmaf(w, p[s * step + e], acc);      // a slice without keys has written nothing
@@ -416,23 +498,20 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
     for (int k = 0; k < ROWDATA; ++k) a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + row] = v[k];
 }
 
-// dlam[h] = -sum over batch and queries of P2 dP: D2 + (what the dq kernel found beyond it) / sum 2; one block per head, fp64 sums in
-// a fixed order
+// dlam[h] = -sum over batch and queries of P2 dP: D2, in 16 bits + (what the dq kernel found beyond it) / sum 2; one block per head, fp64
+// sums in a fixed order
 template <typename T>
 __global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
   __shared__ double part[16];
   const int h = blockIdx.x, g = h / a.r, x = h % a.r;
   double s = 0.0;
-  for (int b = 0; b < a.B; ++b) {
-    const int bg = b * a.G + g;
-    const float* d2 = a.rowdata + ((long long)bg * ROWDATA + 3) * a.Rp + x;
-    const float* inv = a.stat + ((long long)bg * 4 + 3) * a.R + x;
-    for (int i = threadIdx.x; i < a.Nq; i += 1024) {
-      const long long at = (long long)i * a.r;
-      double rest = 0.0;
-      for (int k = 0; k < a.splits; ++k) rest += (double)a.d2[((long long)k * a.B * a.G + bg) * a.Rp + x + at];
-      s += (double)d2[at] + rest * (double)inv[at];
-    }
+  const int n = a.B * a.Nq, slices = a.d2 ? a.splits : 0;
+#pragma unroll 4
+  for (long long it = threadIdx.x; it < (long long)n * (slices + 1); it += 1024) {
+    const int k = (int)(it / n), bi = (int)(it - (long long)k * n), b = bi / a.Nq, bg = b * a.G + g;
+    const long long row = (long long)(bi - b * a.Nq) * a.r + x;
+    if (k == 0) s += (double)a.rowdata[((long long)bg * ROWDATA + 3) * a.Rp + row];
+    else s += (double)(a.d2[((long long)(k - 1) * a.B * a.G + bg) * a.Rp + row] * a.stat[((long long)bg * 4 + 3) * a.R + row]);
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
@@ -446,14 +525,14 @@ __global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
 }
 
 // Where there are few row tiles, the keys of a row tile are cut into a.splits slices, whose sums go to a.part in fp32
-template <typename T, int D>
+template <typename T, int D, bool MASK>
 __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(Args a) {
   constexpr int NT = 256, KT = sizeof(T) == 2 ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
   constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1;
   __shared__ __attribute__((aligned(16))) char lds[4 * BYTES];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, half = lane >> 5;
   const int bgs = a.B * a.G, bg = blockIdx.x % bgs, b = bg / a.G, g = bg % a.G, split = blockIdx.x / bgs % a.splits;
-  const int tile = a.tiles - 1 - (int)(blockIdx.x / bgs / a.splits);
+  const int tile = row_tile(a, blockIdx.x / bgs / a.splits);
   const int row = tile * 128 + wave * 32 + (lane & 31);
   const bool in = row < a.R;
   const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
@@ -489,7 +568,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   }
   const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;
   const int wave_first = a.causal ? min(limit - 1, min(tile * 128 + wave * 32, a.R - 1) / a.r + shift) : limit - 1;
-  const uint8_t* mrow = a.mask ? a.mask + b * a.m_b + i * a.m_r : nullptr;
+  const uint8_t* mrow = MASK ? a.mask + b * a.m_b + i * a.m_r : nullptr;
 
   f32x16 acc[2][QT];
 #pragma unroll
@@ -497,6 +576,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
 #pragma unroll
     for (int t = 0; t < QT; ++t) acc[m][t] = (f32x16)(0.f);
   Scaled<T> sc[2];
+  MaskWords mask_next;             // of the next 32 keys, asked for one step ahead
 
   const char* kbase = a.k + (b * a.k_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
   const char* vbase = a.v + (b * a.v_b + (long long)g * 2 * a.d) * (long long)sizeof(T);
@@ -507,6 +587,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   if (nt > 0) {
     KTile::keys(lds, kbase, kld, kbeg, limit, a.d, tid, wave);
     VTile::keys(lds + BYTES, vbase, vld, kbeg, limit, a.d, tid, wave);
+    if (MASK) mask_next.load(a, mrow, kbeg, half);
   }
   for (int t = 0; t < nt; ++t) {
     const int j0 = kbeg + t * KT;
@@ -522,10 +603,12 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
     for (int kb = 0; kb < KT / 32; ++kb) {
       const int jb = j0 + kb * 32;
       if (jb >= kend) break;
+      const MaskWords mask = mask_next;
+      if (MASK) mask_next.load(a, mrow, jb + 32, half);
       f32x16 s[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) s[m] = scores<T, D>(kt, kb, m, q[m], lane);
-      if (a.mask || jb + 31 > wave_first) exclude_cols_q(a, mrow, s[0], s[1], jb, jlast, half, a.mask != nullptr);
+      if (MASK || jb + 31 > wave_first) exclude_cols_q(mask, MASK, s[0], s[1], jb, jlast, half);
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
       for (int st = 0; st < VS; ++st) dp = mfma_step<T>(op<T>(row_frag<T, GR>(vt, kb * 32 + (lane & 31), 16 * st, half)), go[st], dp);
@@ -556,7 +639,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   if (!in) return;
   if (a.d2) {
     // sum_j P2 dP in fp32 = D2 + sum_j P2 (dP - D2): dlam does not carry the rounding of the probabilities that O2 was made of
-    rest += __shfl_xor(rest, 32);
+    rest = sum_halves(rest);
     if (half == 0) a.d2[((long long)split * bgs + bg) * a.Rp + row] = rest;
   }
   if (!a.dq) return;
@@ -584,7 +667,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
 template <typename T, int D>
 constexpr bool wide_v = D == 64 && sizeof(T) == 2;
 
-template <typename T, int D>
+template <typename T, int D, bool MASK>
 __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : waves_of(D, sizeof(T), false))) void dkv_kernel(Args a) {
   constexpr bool WIDE = wide_v<T, D>;
   constexpr int NT = WIDE ? 512 : 256, QR = (sizeof(T) == 2 && D != 32) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = QR * GR * 16;
@@ -676,6 +759,14 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
 #pragma unroll
     for (int rb_ = 0; rb_ < (WIDE ? 1 : QR / 32); ++rb_) {
       const int rb = WIDE ? wave >> 2 : rb_;
+      uint8_t mask[WIDE || !MASK ? 1 : 16]; // of this lane's key and its 16 rows, asked for before the products where registers allow
+      if constexpr (!WIDE && MASK) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int i = min(row0 + rb * 32 + acc_row(e, half), a.R - 1) / a.r;
+          mask[e] = in ? a.mask[b * a.m_b + i * a.m_r + j] : 0;
+        }
+      }
       f32x16 s[2];
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
@@ -685,13 +776,15 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
           s[m] = mfma_step<T>(op<T>(row_frag<T, GR>(qt, rb * 32 + (lane & 31), m * D + 16 * st, half)), key(m, st), s[m]);
       }
       // (row, key) pairs to leave out: keys past the limit, the causal order, the mask
-      const bool some = a.mask || jw + 31 >= limit || (a.causal && jw + 31 > (row0 + rb * 32) / a.r + shift);
+      const bool some = MASK || jw + 31 >= limit || (a.causal && jw + 31 > (row0 + rb * 32) / a.r + shift);
       if (some) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int row = min(row0 + rb * 32 + acc_row(e, half), a.R - 1), i = row / a.r;
           bool no = !in || (a.causal && j > i + shift);
-          if (a.mask && !no) no = a.mask[b * a.m_b + i * a.m_r + j] != 0;
+          if constexpr (MASK) {
+            if (!no) no = (WIDE ? a.mask[b * a.m_b + i * a.m_r + j] : mask[WIDE ? 0 : e]) != 0;
+          }
           if (no) s[0][e] = -INFINITY, s[1][e] = -INFINITY;
         }
       }
@@ -813,21 +906,21 @@ __global__ __launch_bounds__(256) void sum_kernel(const float* part, T* out, lon
 inline int cdiv(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 struct Split {
-  int waves, tiles, splits, len;
+  int rows, tiles, splits, len;
 };
-// Blocks of 4 waves (128 rows) share keys and values among more rows; blocks of one wave fill the chip where there are few rows.
-// Where even those leave most of it idle, the keys are cut into slices of at least 256.
+// Blocks of 128 rows share keys and values among more rows; blocks of 32 rows, whose waves divide the keys, fill the chip where there
+// are few.  Where even those leave most of it idle, the keys are cut into slices of at least 512 that a second kernel joins.
 Split split_of(const ff3d_diff_attention_t& p) {
   const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
   Split s;
-  s.waves = bg * cdiv(R, 128) >= 256 ? 4 : 1;
-  s.tiles = cdiv(R, 32 * s.waves);
+  s.rows = bg * cdiv(R, 128) >= 256 ? 128 : 32;
+  s.tiles = cdiv(R, s.rows);
   const long long blocks = bg * s.tiles;
-  long long n = blocks >= 512 ? 1 : cdiv(1024, blocks);
-  n = n < p.Nk / 256 ? n : p.Nk / 256;
+  long long n = blocks >= 128 ? 1 : cdiv(256, blocks);
+  n = n < p.Nk / 512 ? n : p.Nk / 512;
   if (n > JOIN) n = JOIN;
   if (n < 1) n = 1;
-  s.len = (int)((cdiv(p.Nk, n) + 63) / 64 * 64);
+  s.len = (int)((cdiv(p.Nk, n) + 127) / 128 * 128);
   s.splits = cdiv(p.Nk, s.len);
   return s;
 }
@@ -891,8 +984,9 @@ int fwd(const ff3d_diff_attention_t& p, Args a, hipStream_t st) {
   a.tiles = s.tiles, a.splits = s.splits, a.split_len = s.len;
   const long long blocks = (long long)a.B * a.G * s.tiles * s.splits;
   if (blocks > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
-  if (s.waves == 4) fwd_kernel<T, D, 4><<<(unsigned)blocks, 256, 0, st>>>(a);
-  else fwd_kernel<T, D, 1><<<(unsigned)blocks, 64, 0, st>>>(a);
+  auto kernel = s.rows == 128 ? (a.mask ? fwd_kernel<T, D, true, true> : fwd_kernel<T, D, true, false>)
+                              : (a.mask ? fwd_kernel<T, D, false, true> : fwd_kernel<T, D, false, false>);
+  kernel<<<(unsigned)blocks, s.rows == 128 ? 256 : FwdShape<T, D, false>::NW * 64, 0, st>>>(a);
   if (s.splits > 1) join_kernel<T><<<(unsigned)((long long)a.B * a.G * a.R), 256, 0, st>>>(a);
   return ff3d_launch_status();
 }
@@ -902,25 +996,25 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   const BwdSplit s = bwd_split_of(p);
   const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128) * s.q, kb = bg * cdiv(a.Nk, 128) * s.k;
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
-  a.d2 = dlam ? a.rowdata + s.rowdata / 4 : nullptr;
+  a.d2 = dlam && sizeof(T) == 2 ? a.rowdata + s.rowdata / 4 : nullptr;
   a.part = a.rowdata + (s.rowdata + s.d2) / 4;
   rows_kernel<T><<<(unsigned)cdiv(rows, 16), 256, 0, st>>>(a);
   if (a.dk) {
     const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;
     a.tiles = cdiv(a.Nk, 128), a.splits = s.k;
-    dkv_kernel<T, D><<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
+    (a.mask ? dkv_kernel<T, D, true> : dkv_kernel<T, D, false>)<<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
     if (s.k > 1) {
       sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dk, n, 2 * n, s.k);
       sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part + n, (T*)a.dv, n, 2 * n, s.k);
     }
   }
-  if (a.dq || dlam) {
+  if (a.dq || a.d2) {
     const long long n = (long long)a.B * a.Nq * a.H * 2 * a.d;
     a.tiles = cdiv(a.R, 128), a.splits = s.q;
-    dq_kernel<T, D><<<(unsigned)qb, 256, 0, st>>>(a);
+    (a.mask ? dq_kernel<T, D, true> : dq_kernel<T, D, false>)<<<(unsigned)qb, 256, 0, st>>>(a);
     if (s.q > 1 && a.dq) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, n, n, s.q);
-    if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
   }
+  if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
   return ff3d_launch_status();
 }
 

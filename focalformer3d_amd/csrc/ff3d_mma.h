@@ -175,6 +175,16 @@ __device__ __forceinline__ void load_lds16(rsrc_t r, char* lds, unsigned off) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void*)lds, 16, (int)off, 0, 0, 0);
 }
 
+// the other half's value of the same column (lane ^ 32), by a register swap: no trip through LDS and no wait for the reads before it
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float sum_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
 // Waits until at most N of this wave's loads are outstanding and its LDS reads are done, then for the other waves.
 template <int N>
 __device__ __forceinline__ void wait_barrier() {

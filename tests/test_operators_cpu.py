@@ -84,7 +84,7 @@ def test_diff_attention_entry_checks_its_arguments():
     # few rows over long keys need a place for the slices
     assert run(Nq=1, Nk=2048, heads=2) == -4
     p = _lib.DiffAttention(**{**ok, 'Nq': 1, 'Nk': 2048})
-    assert lib.ff3d_diff_attention_workspace_bytes(p, 0) == 8 * 4 * 1 * (4 * 16 + 4) * 4          # 8 slices of 256 keys, 4 rows
+    assert lib.ff3d_diff_attention_workspace_bytes(p, 0) == 4 * 4 * 1 * (4 * 16 + 4) * 4          # 4 slices of 512 keys, 4 rows
     assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 0) == 0
     assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 1) == 4 * (6 + 1) * 64 * 4  # rows rounded up to 64
 
