@@ -767,13 +767,17 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
           mask[e] = in ? a.mask[b * a.m_b + i * a.m_r + j] : 0;
         }
       }
-      f32x16 s[2];
+      // operands are read in groups ahead of the products that use them (a group is waited for once), as far as registers go
+      f32x16 s[2] = {(f32x16)(0.f), (f32x16)(0.f)};
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        s[m] = (f32x16)(0.f);
+        vec8<T> x[ST];
+        Op<T> y[ST];
 #pragma unroll
-        for (int st = 0; st < ST; ++st)
-          s[m] = mfma_step<T>(op<T>(row_frag<T, GR>(qt, rb * 32 + (lane & 31), m * D + 16 * st, half)), key(m, st), s[m]);
+        for (int st = 0; st < ST; ++st) x[st] = row_frag<T, GR>(qt, rb * 32 + (lane & 31), m * D + 16 * st, half), y[st] = key(m, st);
+        if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < ST; ++st) s[m] = mfma_step<T>(op<T>(x[st]), y[st], s[m]);
       }
       // (row, key) pairs to leave out: keys past the limit, the causal order, the mask
       const bool some = MASK || jw + 31 >= limit || (a.causal && jw + 31 > (row0 + rb * 32) / a.r + shift);
@@ -790,7 +794,16 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
       }
       f32x16 dp = (f32x16)(0.f);
 #pragma unroll
-      for (int st = 0; st < VS; ++st) dp = mfma_step<T>(op<T>(row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * st, half)), value(st), dp);
+      for (int st0 = 0; st0 < VS; st0 += 4) {
+        constexpr int G = VS < 4 ? VS : 4;
+        vec8<T> x[G];
+        Op<T> y[G];
+#pragma unroll
+        for (int st = 0; st < G; ++st) x[st] = row_frag<T, GR>(ot, rb * 32 + (lane & 31), 16 * (st0 + st), half), y[st] = value(st0 + st);
+        if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int st = 0; st < G; ++st) dp = mfma_step<T>(op<T>(x[st]), y[st], dp);
+      }
       f32x16 w;
       float top[3] = {0.f, 0.f, 0.f};
 #pragma unroll
@@ -813,18 +826,28 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         const Op<T> f = op<T>(scaled_frag<T>(w, st, sv.mul()));
+        vec8<T> x[VT];
 #pragma unroll
-        for (int x = 0; x < VT; ++x) dv[x] = mfma_step<T>(op<T>(col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, x * 32, lane)), f, dv[x]);
+        for (int t = 0; t < VT; ++t) x[t] = col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, t * 32, lane);
+        if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), f, dv[t]);
       }
+      sk[0].template see<QT>(top[1], dk[0]);
+      sk[1].template see<QT>(top[2], dk[1]);
 #pragma unroll
-      for (int m = 0; m < 2; ++m) {
-        sk[m].template see<QT>(top[1 + m], dk[m]);
+      for (int st = 0; st < 2; ++st) {
+        const Op<T> f[2] = {op<T>(scaled_frag<T>(s[0], st, sk[0].mul())), op<T>(scaled_frag<T>(s[1], st, sk[1].mul()))};
+        vec8<T> x[2][QT];          // d = 16: both maps share the columns of one tile
 #pragma unroll
-        for (int st = 0; st < 2; ++st) {
-          const Op<T> f = op<T>(scaled_frag<T>(s[m], st, sk[m].mul()));
+        for (int m = 0; m < (D >= 32 ? 2 : 1); ++m)
 #pragma unroll
-          for (int x = 0; x < QT; ++x) dk[m][x] = mfma_step<T>(op<T>(col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane)), f, dk[m][x]);
-        }
+          for (int t = 0; t < QT; ++t) x[m][t] = col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + t * 32, lane);
+        if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), f[m], dk[m][t]);
       }
     }
   }
