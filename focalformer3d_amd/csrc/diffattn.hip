@@ -35,9 +35,12 @@ struct Args {
   long long m_b, m_r;                                     // bytes
   char *out, *dq, *dk, *dv;
   float *out2, *stat, *part, *rowdata, *d2;
-  int B, Nq, Nk, H, G, r, d, R, Rp, causal, mask4, splits, split_len, tiles;
+  int B, Nq, Nk, H, G, r, rlog, d, R, Rp, causal, mask4, splits, split_len, tiles;     // rlog: log2 r, or -1
   float scale, c;                 // c = scale * log2(e)
 };
+
+// the query of a packed row (an integer division costs 25 instructions, and some loops need 32 of them)
+__device__ __forceinline__ int query_of(const Args& a, int row) { return a.rlog >= 0 ? row >> a.rlog : row / a.r; }
 
 __device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -108,16 +111,16 @@ struct Tile {
     }
   }
   // packed rows row0 ..: row = i r + h, at base + i * ld + h * head bytes
-  __device__ __forceinline__ static void rows(char* lds, const char* base, long long ld, int head, int row0, int R, int per, int d, int tid, int wave) {
-    const int i0 = row0 / per;
+  __device__ __forceinline__ static void rows(const Args& a, char* lds, const char* base, long long ld, int head, int row0, int d, int tid, int wave) {
+    const int i0 = query_of(a, row0);
     const char* p = base + i0 * ld;
     const rsrc_t rs = make_rsrc(p, 0x7fffffff);
 #pragma unroll
     for (int it = 0; it < N; ++it) {
       const int at = it * NT + tid, r = at / GR, g = place<GR>(r, at % GR), s = source(g, d);
-      const int row = row0 + r, i = row / per, h = row - i * per;
+      const int row = row0 + r, i = query_of(a, row), h = row - i * a.r;
       load_lds16(rs, lds + (it * NT + wave * 64) * 16,
-                 row < R && s >= 0 ? (unsigned)(i - i0) * (unsigned)ld + (unsigned)h * (unsigned)head + s * (unsigned)sizeof(T) : OUT);
+                 row < a.R && s >= 0 ? (unsigned)(i - i0) * (unsigned)ld + (unsigned)h * (unsigned)head + s * (unsigned)sizeof(T) : OUT);
     }
   }
 };
@@ -223,7 +226,7 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
   const int tile = row_tile(a, blockIdx.x / bgs / a.splits);
   const int row0 = tile * BLOCK_ROWS + (ROWS ? wave * 32 : 0), row = row0 + (lane & 31);
   const bool in = row < a.R;
-  const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
+  const int rowc = min(row, a.R - 1), i = query_of(a, rowc), h = g * a.r + (rowc - i * a.r);
 
   Op<T> q[2][ST];
   {
@@ -238,11 +241,11 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
   }
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
   int kend = limit;
-  if (a.causal) kend = min(kend, min(a.R - 1, tile * BLOCK_ROWS + BLOCK_ROWS - 1) / a.r + shift + 1);
+  if (a.causal) kend = min(kend, query_of(a, min(a.R - 1, tile * BLOCK_ROWS + BLOCK_ROWS - 1)) + shift + 1);
   const int kbeg = split * a.split_len;
   kend = min(kend, kbeg + a.split_len);
   const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;       // last key of this lane's row
-  const int wave_first = a.causal ? min(limit - 1, min(row0, a.R - 1) / a.r + shift) : limit - 1;   // smallest in the wave
+  const int wave_first = a.causal ? min(limit - 1, query_of(a, min(row0, a.R - 1)) + shift) : limit - 1;   // smallest in the wave
   const uint8_t* mrow = MASK ? a.mask + b * a.m_b + i * a.m_r : nullptr;
 
   f32x16 o[2][VT];
@@ -535,7 +538,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   const int tile = row_tile(a, blockIdx.x / bgs / a.splits);
   const int row = tile * 128 + wave * 32 + (lane & 31);
   const bool in = row < a.R;
-  const int rowc = min(row, a.R - 1), i = rowc / a.r, h = g * a.r + rowc % a.r;
+  const int rowc = min(row, a.R - 1), i = query_of(a, rowc), h = g * a.r + (rowc - i * a.r);
 
   Op<T> q[2][ST], go[VS];
   {
@@ -559,7 +562,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
   for (int k = 0; k < ROWDATA; ++k) rd[k] = a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + rowc];
   const int limit = key_limit(a, b), shift = a.Nk - a.Nq;
   int kend = limit;
-  if (a.causal) kend = min(kend, min(a.R - 1, tile * 128 + 127) / a.r + shift + 1);
+  if (a.causal) kend = min(kend, query_of(a, min(a.R - 1, tile * 128 + 127)) + shift + 1);
   int kbeg = 0;
   if (a.splits > 1) {              // whole tiles of the keys that the rows attend
     const int n = kend > 0 ? (kend + KT - 1) / KT : 0;
@@ -567,7 +570,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
     kend = min(kend, (int)((long long)n * (split + 1) / a.splits) * KT);
   }
   const int jlast = a.causal ? min(limit - 1, i + shift) : limit - 1;
-  const int wave_first = a.causal ? min(limit - 1, min(tile * 128 + wave * 32, a.R - 1) / a.r + shift) : limit - 1;
+  const int wave_first = a.causal ? min(limit - 1, query_of(a, min(tile * 128 + wave * 32, a.R - 1)) + shift) : limit - 1;
   const uint8_t* mrow = MASK ? a.mask + b * a.m_b + i * a.m_r : nullptr;
 
   f32x16 acc[2][QT];
@@ -741,8 +744,8 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
   }
 
   auto stage = [&](char* to, int row0) {
-    QTile::rows(to, qbase, qld, head, row0, a.R, a.r, a.d, tid, wave);
-    OTile::rows(to + BYTES, obase, old_, head, row0, a.R, a.r, a.d, tid, wave);
+    QTile::rows(a, to, qbase, qld, head, row0, a.d, tid, wave);
+    OTile::rows(a, to + BYTES, obase, old_, head, row0, a.d, tid, wave);
     if (wave * 64 < RG) {          // QR / 4 granules of each of the arrays
       const rsrc_t rs = make_rsrc(rdata + row0, ((long long)ROWDATA * a.Rp - row0) * 4);
       load_lds16(rs, to + 2 * BYTES + wave * 1024, tid < RG ? (unsigned)(tid / (QR / 4)) * (unsigned)a.Rp * 4u + (tid % (QR / 4)) * 16u : OUT);
@@ -763,7 +766,7 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
       if constexpr (!WIDE && MASK) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int i = min(row0 + rb * 32 + acc_row(e, half), a.R - 1) / a.r;
+          const int i = query_of(a, min(row0 + rb * 32 + acc_row(e, half), a.R - 1));
           mask[e] = in ? a.mask[b * a.m_b + i * a.m_r + j] : 0;
         }
       }
@@ -780,11 +783,11 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
         for (int st = 0; st < ST; ++st) s[m] = mfma_step<T>(op<T>(x[st]), y[st], s[m]);
       }
       // (row, key) pairs to leave out: keys past the limit, the causal order, the mask
-      const bool some = MASK || jw + 31 >= limit || (a.causal && jw + 31 > (row0 + rb * 32) / a.r + shift);
+      const bool some = MASK || jw + 31 >= limit || (a.causal && jw + 31 > query_of(a, row0 + rb * 32) + shift);
       if (some) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int row = min(row0 + rb * 32 + acc_row(e, half), a.R - 1), i = row / a.r;
+          const int i = query_of(a, min(row0 + rb * 32 + acc_row(e, half), a.R - 1));
           bool no = !in || (a.causal && j > i + shift);
           if constexpr (MASK) {
             if (!no) no = (WIDE ? a.mask[b * a.m_b + i * a.m_r + j] : mask[WIDE ? 0 : e]) != 0;
@@ -957,7 +960,7 @@ struct BwdSplit {
 BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
   auto slices = [](long long blocks, long long len) {
-    long long n = blocks >= 384 ? 1 : cdiv(512, blocks);
+    long long n = blocks >= 384 ? 1 : 512 / blocks;        // two blocks on a CU, and no second round
     n = n < len / 128 ? n : len / 128;
     return (int)(n < 1 ? 1 : n > 64 ? 64 : n);
   };
@@ -996,6 +999,9 @@ Args args_of(const ff3d_diff_attention_t& p) {
   a.m_b = p.mask_batch, a.m_r = p.mask_row;
   a.mask4 = p.mask && ((p.mask_batch | p.mask_row | (long long)reinterpret_cast<uintptr_t>(p.mask)) & 3) == 0;
   a.B = p.B, a.Nq = p.Nq, a.Nk = p.Nk, a.H = p.heads, a.G = p.kv_heads, a.r = p.heads / p.kv_heads, a.d = p.d, a.causal = p.causal;
+  a.rlog = -1;
+  for (int k = 0; k < 31; ++k)
+    if (a.r == 1 << k) a.rlog = k;
   a.R = a.Nq * a.r, a.Rp = (a.R + 63) / 64 * 64;
   a.scale = p.scale, a.c = p.scale * LOG2E, a.splits = 1, a.split_len = p.Nk;
   return a;

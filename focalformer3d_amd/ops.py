@@ -5,6 +5,7 @@ Every wrapper validates device / dtype / contiguity and raises - there is no fal
 Reference call sites are cited per function (FD = focal_decoder.py, EU = encoder_utils.py,
 UT = utils.py, BC = transfusion_bbox_coder.py of the reference plugin).
 """
+import array
 import ctypes as C
 import functools
 import os
@@ -1797,25 +1798,28 @@ def _ptr(t):
 
 
 def _gated_args(x, weight, bias, act):
-    if x.dtype not in _DTYPE:
+    """Checked operands -> (x as rows, weight, bias, F, C, which operands have to be packed, dtype code, activation code)."""
+    code, acode = _DTYPE.get(x.dtype), _ACTS.get(act)
+    if code is None:
         raise RuntimeError(f'gated_linear: expected fp32, bf16 or fp16 tensors, got {x.dtype}')
-    if act not in _ACTS:
+    if acode is None:
         raise ValueError(f'gated_linear: unknown activation {act!r} (one of {", ".join(_ACTS)})')
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[0] % 2 or weight.shape[0] == 0 or weight.shape[1] == 0:
+    if x.dim() < 1 or weight.dim() != 2 or weight.shape[0] % 2 or 0 in weight.shape:
         raise RuntimeError(f'gated_linear: expected x (..., C) and weight (2 F, C), got {tuple(x.shape)} and {tuple(weight.shape)}')
     F2, C_ = weight.shape
     _same(weight, x, 'weight')
-    _same(x, x, 'x', (*x.shape[:-1], C_))
+    if x.shape[-1] != C_:
+        raise RuntimeError(f'x: expected rows of {C_}, got {tuple(x.shape)}')
     if bias is not None:
         _same(bias, x, 'bias', (F2,))
         bias = bias.contiguous()
-    x2 = x.reshape(-1, C_)
+    x2 = x if x.dim() == 2 else x.reshape(-1, C_)
     if x2.stride(1) != 1 or x2.stride(0) < C_:
         x2 = x2.contiguous()
     weight = weight.contiguous()
-    per = 16 // x.element_size()
-    pack = (1 if C_ % per or x2.stride(0) % per or x2.data_ptr() % 16 else 0) | (2 if C_ % per or weight.data_ptr() % 16 else 0)
-    return x2, weight, bias, F2 // 2, C_, pack
+    per = 4 if code == 0 else 8
+    pack = 3 if C_ % per else (1 if x2.stride(0) % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
+    return x2, weight, bias, F2 // 2, C_, pack, code, acode
 
 
 @_on_device_of('x')
@@ -1823,24 +1827,27 @@ def gated_linear(x, weight, bias=None, act='silu'):
     """h = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel (ff3d_gated_linear_fwd): x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F)
     or None, all fp32, bf16 or fp16 -> (..., F).  act: 'silu', 'gelu' (erf form), 'relu' or 'sigmoid'.  Sums in fp32, one rounding.
     The differentiable form is ``autograd.gated_linear``."""
-    x2, weight, bias, F_, C_, pack = _gated_args(x, weight, bias, act)
-    M, code = x2.shape[0], _DTYPE[x.dtype]
-    h = torch.empty(*x.shape[:-1], F_, dtype=x.dtype, device=x.device)
+    x2, weight, bias, F_, C_, pack, code, acode = _gated_args(x, weight, bias, act)
+    M = x2.shape[0]
+    h = torch.empty((*x.shape[:-1], F_), dtype=x.dtype, device=x.device)
     if M == 0:
         return h
     lib = _lib.load()
-    n = lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 0)
-    ws = torch.empty(n, dtype=torch.uint8, device=x.device) if n else None
-    _lib.check(lib.ff3d_gated_linear_fwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(h), M, C_, F_, _ACTS[act], code, pack, _ptr(ws),
-                                         _stream()), 'ff3d_gated_linear_fwd')
+    ws = None
+    if pack:
+        ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 0), dtype=torch.uint8, device=x.device)
+    st = lib.ff3d_gated_linear_fwd(x2.data_ptr(), x2.stride(0), weight.data_ptr(), None if bias is None else bias.data_ptr(), h.data_ptr(), M, C_, F_,
+                                   acode, code, pack, None if ws is None else ws.data_ptr(), _stream())
+    if st:
+        _lib.check(st, 'ff3d_gated_linear_fwd')
     return h
 
 
 @_on_device_of('x')
 def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     """Gradients of ``gated_linear`` for dh (..., F) -> (dx, dweight, dbias); None where ``want`` is false (or there is no bias)."""
-    x2, weight, bias, F_, C_, pack = _gated_args(x, weight, bias, act)
-    M, code = x2.shape[0], _DTYPE[x.dtype]
+    x2, weight, bias, F_, C_, pack, code, acode = _gated_args(x, weight, bias, act)
+    M = x2.shape[0]
     _same(dh, x, 'dh', (*x.shape[:-1], F_))
     want_b = want[2] and bias is not None
     new = torch.zeros if M == 0 else torch.empty
@@ -1855,7 +1862,7 @@ def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     lib = _lib.load()
     ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 1), dtype=torch.uint8, device=x.device)
     _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh2.stride(0), _ptr(dx), _ptr(dw), _ptr(db),
-                                         M, C_, F_, _ACTS[act], code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
+                                         M, C_, F_, acode, code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
     return dx, dw, db
 
 
@@ -1970,17 +1977,26 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None
 _NORM_KINDS = {2: 2, 1: 1, float('inf'): 0}
 
 
-def _grad_list(tensors, name):
-    """Host arrays (pointers, element counts, dtype codes) of a list of dense CUDA tensors on one device."""
-    dev = tensors[0].device
-    for i, t in enumerate(tensors):
-        if not isinstance(t, torch.Tensor) or t.device != dev or t.dtype not in _DTYPE or t.layout != torch.strided:
-            raise RuntimeError(f'{name}[{i}]: expected a dense fp32, bf16 or fp16 tensor on {dev}')
-        if not _dense(t):
-            raise RuntimeError(f'{name}[{i}]: expected a tensor without gaps or overlaps, got shape {tuple(t.shape)}, strides {t.stride()}')
-    n = len(tensors)
-    return ((C.c_void_p * n)(*[t.data_ptr() for t in tensors]), (C.c_int64 * n)(*[t.numel() for t in tensors]),
-            (C.c_int32 * n)(*[_DTYPE[t.dtype] for t in tensors]))
+def _grad_list(tensors, name, numel=None):
+    """Host arrays (pointers, element counts, dtype codes) of a list of dense CUDA tensors on one device, and whether all are contiguous.
+    (A call's time on many small tensors is this function's: one pass per property, no per-tensor Python beyond it.)"""
+    dev = tensors[0].get_device()
+    codes = [_DTYPE.get(t.dtype) for t in tensors]
+    plain = False not in [t.is_contiguous() for t in tensors]
+    if not plain or None in codes or [t.get_device() for t in tensors] != [dev] * len(tensors):
+        for i, t in enumerate(tensors):
+            if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype not in _DTYPE or t.layout != torch.strided:
+                raise RuntimeError(f'{name}[{i}]: expected a dense fp32, bf16 or fp16 tensor on cuda:{dev}')
+            if not _dense(t):
+                raise RuntimeError(f'{name}[{i}]: expected a tensor without gaps or overlaps, got shape {tuple(t.shape)}, strides {t.stride()}')
+    ptrs = array.array('Q', [t.data_ptr() for t in tensors])
+    if numel is None:
+        numel = array.array('q', [t.numel() for t in tensors])
+    return ptrs, numel, array.array('i', codes), plain
+
+
+def _addr(a):
+    return a.buffer_info()[0]
 
 
 def _dense(t):
@@ -2007,12 +2023,13 @@ def grad_norm(grads, norm_type=2.0):
     """Norm (2, 1 or inf) over all elements of a list of dense fp32 / bf16 / fp16 tensors of one device -> fp32 scalar on the device
     (ff3d_grad_norm; sums in fp64, no host synchronisation)."""
     kind = _norm_kind(norm_type)
-    ptrs, numel, codes = _grad_list(grads, 'grads')
+    grads = list(grads)
+    ptrs, numel, codes, _ = _grad_list(grads, 'grads')
     lib = _lib.load()
-    dev = grads[0].device
+    dev, n = grads[0].device, len(grads)
     norm = torch.empty((), device=dev)
-    ws = torch.empty(lib.ff3d_grad_norm_workspace_bytes(numel, len(grads)), dtype=torch.uint8, device=dev)
-    _lib.check(lib.ff3d_grad_norm(ptrs, numel, codes, len(grads), kind, _ptr(ws), _ptr(norm), _stream()), 'ff3d_grad_norm')
+    ws = torch.empty(lib.ff3d_grad_norm_workspace_bytes(_addr(numel), n), dtype=torch.uint8, device=dev)
+    _lib.check(lib.ff3d_grad_norm(_addr(ptrs), _addr(numel), _addr(codes), n, kind, _ptr(ws), _ptr(norm), _stream()), 'ff3d_grad_norm')
     return norm
 
 
@@ -2025,23 +2042,25 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f'max_norm {max_norm}: expected a number >= 0')
-    ptrs, numel, codes = _grad_list(grads, 'grads')
+    grads = list(grads)
+    ptrs, numel, codes, plain = _grad_list(grads, 'grads')
     optrs, ocodes = ptrs, codes
+    dev, n = grads[0].device, len(grads)
     if out is not None:
-        if len(out) != len(grads) or any(o.shape != g.shape or (o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()))
-                                         for o, g in zip(out, grads)):
-            raise RuntimeError('out: expected one tensor per gradient, of its shape and strides')
-        if out[0].device != grads[0].device:
-            raise RuntimeError(f'out: expected tensors on {grads[0].device}')
-        optrs, _, ocodes = _grad_list(out, 'out')
+        out = list(out)
+        if [o.shape for o in out] != [g.shape for g in grads] or out[0].get_device() != grads[0].get_device():
+            raise RuntimeError(f'out: expected one tensor per gradient, of its shape and on {dev}')
+        optrs, _, ocodes, out_plain = _grad_list(out, 'out', numel)
+        if not (plain and out_plain):
+            for o, g in zip(out, grads):
+                if o.stride() != g.stride() and not (o.is_contiguous() and g.is_contiguous()):
+                    raise RuntimeError('out: expected the strides of the gradients')
     lib = _lib.load()
-    dev = grads[0].device
     norm = torch.empty((), device=dev)
-    ws = torch.empty(lib.ff3d_grad_norm_workspace_bytes(numel, len(grads)), dtype=torch.uint8, device=dev)
-    st = lib.ff3d_clip_grads(ptrs, optrs, numel, codes, ocodes, len(grads), kind, max_norm, _ptr(ws), _ptr(norm), _stream())
+    ws = torch.empty(lib.ff3d_grad_norm_workspace_bytes(_addr(numel), n), dtype=torch.uint8, device=dev)
+    st = lib.ff3d_clip_grads(_addr(ptrs), _addr(optrs), _addr(numel), _addr(codes), _addr(ocodes), n, kind, max_norm, _ptr(ws), _ptr(norm), _stream())
     if st == -5:
         raise RuntimeError('clip_grads: two outputs share memory, or an output overlaps a gradient that is not its own')
     _lib.check(st, 'ff3d_clip_grads')
-    for t in (grads if out is None else out):           # written through raw pointers: tell autograd
-        torch.autograd.graph.increment_version(t)
+    torch.autograd.graph.increment_version(grads if out is None else out)           # written through raw pointers: tell autograd
     return norm
