@@ -51,25 +51,33 @@ __device__ __forceinline__ float sigmoid_t(float x) {
   else return __builtin_amdgcn_rcpf(1.f + __expf(-x));         // 1 ulp of fp32, far below the output's rounding
 }
 
-template <typename T>
-__device__ __forceinline__ float act_f(float g, int act) {
-  if (act == ACT_RELU) return g < 0.f ? 0.f : g;               // a NaN stays one
-  if (act == ACT_GELU) return g * (0.5f * (1.f + erff(g * 0.70710678118654752f)));
+template <typename T, int ACT>
+__device__ __forceinline__ float act_f(float g) {
+  if constexpr (ACT == ACT_RELU) return g < 0.f ? 0.f : g;               // a NaN stays one
+  if constexpr (ACT == ACT_GELU) return g * (0.5f * (1.f + erff(g * 0.70710678118654752f)));
   const float s = sigmoid_t<T>(g);
-  return act == ACT_SIGMOID ? s : g * s;
+  return ACT == ACT_SIGMOID ? s : g * s;
 }
-template <typename T>
-__device__ __forceinline__ void act_both(float g, int act, float& a, float& da) {
-  if (act == ACT_RELU) {
+template <typename T, int ACT>
+__device__ __forceinline__ void act_both(float g, float& a, float& da) {
+  if constexpr (ACT == ACT_RELU) {
     a = g < 0.f ? 0.f : g, da = g > 0.f ? 1.f : 0.f;
-  } else if (act == ACT_GELU) {
+  } else if constexpr (ACT == ACT_GELU) {
     const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     a = g * cdf, da = cdf + g * exp_t<T>(-0.5f * g * g) * 0.39894228040143268f;
   } else {
     const float s = sigmoid_t<T>(g);
-    if (act == ACT_SIGMOID) a = s, da = s * (1.f - s);
+    if constexpr (ACT == ACT_SIGMOID) a = s, da = s * (1.f - s);
     else a = g * s, da = s * (1.f + g * (1.f - s));
   }
+}
+
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  if (act == ACT_SILU) f(std::integral_constant<int, ACT_SILU>{});
+  else if (act == ACT_GELU) f(std::integral_constant<int, ACT_GELU>{});
+  else if (act == ACT_RELU) f(std::integral_constant<int, ACT_RELU>{});
+  else f(std::integral_constant<int, ACT_SIGMOID>{});
 }
 
 template <typename T>
@@ -340,6 +348,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
       __syncthreads();
     }
     float sg[TN / 2][4][4] = {}, su[TN / 2][4][4] = {};
+    with_act(p.act, [&](auto act) {                  // outside the loops: the elements' chains run beside each other
+    constexpr int ACT = decltype(act)::value;
 #pragma unroll
     for (int pr = 0; pr < TN / 2; ++pr)
 #pragma unroll
@@ -359,14 +369,14 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
           for (int i = 0; i < 4; ++i) g[i] = acc[2 * pr][j][4 * q + i] + bg[i], u[i] = acc[2 * pr + 1][j][4 * q + i] + bu[i];
           if constexpr (EPI == EPI_GATED) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = act_f<T>(g[i], p.act) * u[i];
+            for (int i = 0; i < 4; ++i) o[i] = act_f<T, ACT>(g[i]) * u[i];
           } else {
             float d[4];
             load4((const T*)at, d, 4, true);         // zeros outside the matrix
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               float a, da;
-              act_both<T>(g[i], p.act, a, da);
+              act_both<T, ACT>(g[i], a, da);
               o[i] = d[i] * u[i] * da, o2[i] = d[i] * a;
               sg[pr][q][i] += o[i], su[pr][q][i] += o2[i];
             }
@@ -375,6 +385,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
           store4((T*)at, o, 4, true);                // a lane's own place, also where it held dh
         }
       }
+    });
     __syncthreads();
     store_tile(lds, (T*)p.out, p.ldo, p.N, p.vec_out);
     if constexpr (EPI == EPI_GATED_BWD) {
@@ -480,14 +491,17 @@ __global__ __launch_bounds__(NW * 64) void gated_rows_kernel(GemmArgs p) {
     for (int e = 0; e < 16; ++e) sums[wave][t][e][lane] = acc[t][e];
   __syncthreads();
   const T* bias = (const T*)p.bias;
+  with_act(p.act, [&](auto act) {
+  constexpr int ACT = decltype(act)::value;
   for (int it = threadIdx.x; it < 1024; it += NW * 64) {         // (row, column) pairs, columns running fastest
     const int nl = it & 31, ml = it >> 5, e = 4 * (nl >> 3) + (nl & 3), at = ml + 32 * ((nl >> 2) & 1);
     if (n0 + nl >= p.N || m0 + ml >= p.M) continue;
     float g = bias ? to_f(bias[n0 + nl]) : 0.f, u = bias ? to_f(bias[p.F + n0 + nl]) : 0.f;
 #pragma unroll
     for (int w = 0; w < NW; ++w) g += sums[w][0][e][at], u += sums[w][1][e][at];
-    ((T*)p.out)[(long long)(m0 + ml) * p.ldo + n0 + nl] = from_f<T>(act_f<T>(g, p.act) * u);
+    ((T*)p.out)[(long long)(m0 + ml) * p.ldo + n0 + nl] = from_f<T>(act_f<T, ACT>(g) * u);
   }
+  });
 }
 
 // out[i] = sum of the slices in order, W elements per thread (n a multiple of W)
