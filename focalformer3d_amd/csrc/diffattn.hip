@@ -35,7 +35,7 @@ struct Args {
   long long m_b, m_r;                                     // bytes
   char *out, *dq, *dk, *dv;
   float *out2, *stat, *part, *rowdata, *d2;
-  int B, Nq, Nk, H, G, r, rlog, d, R, Rp, causal, mask4, splits, split_len, tiles;     // rlog: log2 r, or -1
+  int B, Nq, Nk, H, G, r, rlog, d, R, Rp, causal, splits, split_len, tiles;     // rlog: log2 r, or -1
   float scale, c;                 // c = scale * log2(e)
 };
 
@@ -165,8 +165,8 @@ struct MaskWords {
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int j = j0 + 8 * q + 4 * half;
-      if (a.mask4 && j + 3 < a.Nk) {
-        w[q] = *(const unsigned*)(mrow + j);
+      if (j + 3 < a.Nk) {
+        __builtin_memcpy(&w[q], mrow + j, 4);        // one load, whatever its alignment
       } else {
         w[q] = 0;
 #pragma unroll
@@ -509,12 +509,13 @@ __global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
   const int h = blockIdx.x, g = h / a.r, x = h % a.r;
   double s = 0.0;
   const int n = a.B * a.Nq, slices = a.d2 ? a.splits : 0;
-#pragma unroll 4
-  for (long long it = threadIdx.x; it < (long long)n * (slices + 1); it += 1024) {
-    const int k = (int)(it / n), bi = (int)(it - (long long)k * n), b = bi / a.Nq, bg = b * a.G + g;
+  for (int bi = threadIdx.x; bi < n; bi += 1024) {
+    const int b = bi / a.Nq, bg = b * a.G + g;
     const long long row = (long long)(bi - b * a.Nq) * a.r + x;
-    if (k == 0) s += (double)a.rowdata[((long long)bg * ROWDATA + 3) * a.Rp + row];
-    else s += (double)(a.d2[((long long)(k - 1) * a.B * a.G + bg) * a.Rp + row] * a.stat[((long long)bg * 4 + 3) * a.R + row]);
+    float rest = 0.f;
+#pragma unroll 16
+    for (int k = 0; k < slices; ++k) rest += a.d2[((long long)k * a.B * a.G + bg) * a.Rp + row];
+    s += (double)a.rowdata[((long long)bg * ROWDATA + 3) * a.Rp + row] + (double)(slices ? rest * a.stat[((long long)bg * 4 + 3) * a.R + row] : 0.f);
   }
 #pragma unroll
   for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
@@ -914,11 +915,13 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
   }
 }
 
-// out[i] = sum over the slices of part[slice * step + i], in order
+// out[i] = sum over the slices of part[slice * step + i], in order; the second half of the grid, if any, does the same for out2
 template <typename T>
-__global__ __launch_bounds__(256) void sum_kernel(const float* part, T* out, long long n, long long step, int slices) {
+__global__ __launch_bounds__(256) void sum_kernel(const float* part, T* out, T* out2, long long n, long long step, int slices) {
+  if (blockIdx.y) part += n, out = out2;
   for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
     float s[4] = {};
+#pragma unroll 8
     for (int k = 0; k < slices; ++k) {
       const Four<float> v = *(const Four<float>*)(part + k * step + i);
 #pragma unroll
@@ -997,7 +1000,6 @@ Args args_of(const ff3d_diff_attention_t& p) {
   a.q = (const char*)p.q, a.k = (const char*)p.k, a.v = (const char*)p.v, a.lam = p.lam, a.mask = p.mask, a.lens = p.kv_lens;
   a.q_b = p.q_batch, a.q_r = p.q_row, a.k_b = p.k_batch, a.k_r = p.k_row, a.v_b = p.v_batch, a.v_r = p.v_row;
   a.m_b = p.mask_batch, a.m_r = p.mask_row;
-  a.mask4 = p.mask && ((p.mask_batch | p.mask_row | (long long)reinterpret_cast<uintptr_t>(p.mask)) & 3) == 0;
   a.B = p.B, a.Nq = p.Nq, a.Nk = p.Nk, a.H = p.heads, a.G = p.kv_heads, a.r = p.heads / p.kv_heads, a.d = p.d, a.causal = p.causal;
   a.rlog = -1;
   for (int k = 0; k < 31; ++k)
@@ -1032,16 +1034,13 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
     const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;
     a.tiles = cdiv(a.Nk, 128), a.splits = s.k;
     (a.mask ? dkv_kernel<T, D, true> : dkv_kernel<T, D, false>)<<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
-    if (s.k > 1) {
-      sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dk, n, 2 * n, s.k);
-      sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part + n, (T*)a.dv, n, 2 * n, s.k);
-    }
+    if (s.k > 1) sum_kernel<T><<<dim3(sum_grid(n), 2), 256, 0, st>>>(a.part, (T*)a.dk, (T*)a.dv, n, 2 * n, s.k);
   }
   if (a.dq || a.d2) {
     const long long n = (long long)a.B * a.Nq * a.H * 2 * a.d;
     a.tiles = cdiv(a.R, 128), a.splits = s.q;
     (a.mask ? dq_kernel<T, D, true> : dq_kernel<T, D, false>)<<<(unsigned)qb, 256, 0, st>>>(a);
-    if (s.q > 1 && a.dq) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, n, n, s.q);
+    if (s.q > 1 && a.dq) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, nullptr, n, n, s.q);
   }
   if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
   return ff3d_launch_status();
