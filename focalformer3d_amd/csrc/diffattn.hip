@@ -277,7 +277,7 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
     const int j0 = kbeg + t * KT;
     const char* kt = my + (n & 1) * 2 * BYTES;
     const char* vt = kt + BYTES;
-    if constexpr (ROWS) __syncthreads();
+    if constexpr (ROWS) wait_barrier<0>();
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");        // this wave's own loads, and its reads of the other half
     if (t + STRIDE < nt) stage(n + 1, j0 + STRIDE * KT);
 #pragma unroll
@@ -597,7 +597,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
     const int j0 = kbeg + t * KT;
     const char* kt = lds + (t & 1) * 2 * BYTES;
     const char* vt = kt + BYTES;
-    __syncthreads();
+    wait_barrier<0>();
     if (t + 1 < nt) {
       char* nx = lds + ((t + 1) & 1) * 2 * BYTES;
       KTile::keys(nx, kbase, kld, j0 + KT, limit, a.d, tid, wave);
@@ -758,7 +758,7 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
     const char* qt = lds + (t & 1) * STAGE;
     const char* ot = qt + BYTES;
     const float* rd = (const float*)(qt + 2 * BYTES);
-    __syncthreads();
+    wait_barrier<0>();
     if (t + 1 < nt) stage(lds + ((t + 1) & 1) * STAGE, row0 + QR);
 #pragma unroll
     for (int rb_ = 0; rb_ < (WIDE ? 1 : QR / 32); ++rb_) {
@@ -865,7 +865,7 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
   if constexpr (WIDE) {            // join the pairs
     float* p = (float*)lds + (kw * (VT + 2 * QT) * 16) * 64 + lane;
     static_assert(4 * (VT + 2 * QT) * 16 * 256 <= (int)sizeof(lds), "the odd waves' sums");
-    __syncthreads();
+    wait_barrier<0>();             // a block without rows still has its keys on the way to LDS
     if (wave >= 4) {
 #pragma unroll
       for (int x = 0; x < VT; ++x)

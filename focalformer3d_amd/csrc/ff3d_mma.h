@@ -186,6 +186,8 @@ __device__ __forceinline__ float sum_halves(float x) {
 }
 
 // Waits until at most N of this wave's loads are outstanding and its LDS reads are done, then for the other waves.
+// What load_lds16 fetched is read only behind this: a plain __syncthreads() waits for LDS accesses, and whether it also waits for loads on
+// their way to LDS is left to where the compiler puts its own waits - behind the barrier or before a loop, as well.
 template <int N>
 __device__ __forceinline__ void wait_barrier() {
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(N) : "memory");

@@ -276,7 +276,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
     stage(0);
     for (int t = 0; t < nk; ++t) {
       const char* cur = lds + (t % STAGES) * STAGE;
-      __syncthreads();             // step t has arrived, and nobody reads the other half any more
+      wait_barrier<0>();           // step t has arrived, and nobody reads the other half any more
       if (t + 1 < nk) stage(t + 1);
       read(cur, 0);
 #pragma unroll
