@@ -31,8 +31,9 @@ struct Args {
   const void* lam;
   const uint8_t* mask;
   const int32_t* lens;
+  unsigned* bits;                 // backward: the mask by keys, word (b, i / 32, j) bit i % 32
   long long q_b, q_r, k_b, k_r, v_b, v_r, do_b, do_r;     // elements
-  long long m_b, m_r;                                     // bytes
+  long long m_b, m_r, bits_b;                             // bytes, words
   char *out, *dq, *dk, *dv;
   float *out2, *stat, *part, *rowdata, *d2;
   int B, Nq, Nk, H, G, r, rlog, d, R, Rp, causal, splits, split_len, tiles;     // rlog: log2 r, or -1
@@ -501,6 +502,21 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
     for (int k = 0; k < ROWDATA; ++k) a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + row] = v[k];
 }
 
+// The mask's bytes turned into words of 32 queries per key: the dk / dv kernel then needs one word per lane and step, and can ask for it
+// a step ahead (16 byte loads behind the step's DMA, in order, would make it wait for that).
+__global__ __launch_bounds__(256) void bits_kernel(Args a, int words) {
+  const int j = blockIdx.x * 256 + threadIdx.x, w = blockIdx.y, b = blockIdx.z;
+  if (j >= a.Nk) return;
+  const uint8_t* p = a.mask + b * a.m_b + j;
+  uint8_t v[32];                   // all asked for before the first is looked at
+#pragma unroll
+  for (int k = 0; k < 32; ++k) v[k] = p[min(w * 32 + k, a.Nq - 1) * a.m_r];
+  unsigned bits = 0;
+#pragma unroll
+  for (int k = 0; k < 32; ++k) bits |= v[k] ? 1u << k : 0u;
+  a.bits[((long long)b * words + w) * a.Nk + j] = bits;
+}
+
 // dlam[h] = -sum over batch and queries of P2 dP: D2, in 16 bits + (what the dq kernel found beyond it) / sum 2; one block per head, fp64
 // sums in a fixed order
 template <typename T>
@@ -752,25 +768,38 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
       load_lds16(rs, to + 2 * BYTES + wave * 1024, tid < RG ? (unsigned)(tid / (QR / 4)) * (unsigned)a.Rp * 4u + (tid % (QR / 4)) * 16u : OUT);
     }
   };
-  if (nt > 0) stage(lds, rbeg);
+  // words of the mask for this lane's key and the queries of a tile's 32 rows: two, since the first query may lie anywhere in a word
+  constexpr int SUBS = !MASK || WIDE ? 1 : QR / 32;
+  unsigned words[SUBS][2], words_next[SUBS][2];
+  const int nwords = (a.Nq + 31) / 32;
+  const unsigned* bits = MASK ? a.bits + b * a.bits_b + min(j, a.Nk - 1) : nullptr;
+  auto ask = [&](int row0) {
+#pragma unroll
+    for (int x = 0; x < SUBS; ++x) {
+      const int first = row0 + (WIDE ? wave >> 2 : x) * 32, w = query_of(a, min(first, a.R - 1)) >> 5;
+      words_next[x][0] = bits[(long long)w * a.Nk];
+      words_next[x][1] = bits[(long long)min(w + 1, nwords - 1) * a.Nk];
+    }
+  };
+  if (nt > 0) {
+    if constexpr (MASK) ask(rbeg);
+    stage(lds, rbeg);
+  }
   for (int t = 0; t < nt; ++t) {
     const int row0 = rbeg + t * QR;
     const char* qt = lds + (t & 1) * STAGE;
     const char* ot = qt + BYTES;
     const float* rd = (const float*)(qt + 2 * BYTES);
     wait_barrier<0>();
+    if constexpr (MASK) {
+#pragma unroll
+      for (int x = 0; x < SUBS; ++x) words[x][0] = words_next[x][0], words[x][1] = words_next[x][1];
+      if (t + 1 < nt) ask(row0 + QR);
+    }
     if (t + 1 < nt) stage(lds + ((t + 1) & 1) * STAGE, row0 + QR);
 #pragma unroll
     for (int rb_ = 0; rb_ < (WIDE ? 1 : QR / 32); ++rb_) {
       const int rb = WIDE ? wave >> 2 : rb_;
-      uint8_t mask[WIDE || !MASK ? 1 : 16]; // of this lane's key and its 16 rows, asked for before the products where registers allow
-      if constexpr (!WIDE && MASK) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int i = query_of(a, min(row0 + rb * 32 + acc_row(e, half), a.R - 1));
-          mask[e] = in ? a.mask[b * a.m_b + i * a.m_r + j] : 0;
-        }
-      }
       // operands are read in groups ahead of the products that use them (a group is waited for once), as far as registers go
       f32x16 s[2] = {(f32x16)(0.f), (f32x16)(0.f)};
 #pragma unroll
@@ -786,14 +815,16 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
       // (row, key) pairs to leave out: keys past the limit, the causal order, the mask
       const bool some = MASK || jw + 31 >= limit || (a.causal && jw + 31 > query_of(a, row0 + rb * 32) + shift);
       if (some) {
+        // one comparison and two selects each, without a branch: keys past the limit lie behind every query's last key
+        const int i0 = query_of(a, min(row0 + rb * 32, a.R - 1)), jc = in ? j : 0x7fffffff;
+        const unsigned blocked = MASK ? __builtin_amdgcn_alignbit(words[MASK ? rb_ : 0][1], words[MASK ? rb_ : 0][0], i0 & 31) : 0u;   // bit i - i0
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int i = query_of(a, min(row0 + rb * 32 + acc_row(e, half), a.R - 1));
-          bool no = !in || (a.causal && j > i + shift);
-          if constexpr (MASK) {
-            if (!no) no = (WIDE ? a.mask[b * a.m_b + i * a.m_r + j] : mask[WIDE ? 0 : e]) != 0;
-          }
-          if (no) s[0][e] = -INFINITY, s[1][e] = -INFINITY;
+          const int last = a.causal ? i + shift : 0x7ffffffe;
+          const bool no = (jc > last) | (MASK && (blocked >> (i - i0) & 1));
+          s[0][e] = no ? -INFINITY : s[0][e];
+          s[1][e] = no ? -INFINITY : s[1][e];
         }
       }
       f32x16 dp = (f32x16)(0.f);
@@ -958,7 +989,7 @@ Split split_of(const ff3d_diff_attention_t& p) {
 // blocks, to slices of at least 128 rows or keys; the slices' fp32 sums are added in order.  Both kernels use one place for them.
 struct BwdSplit {
   int q, k;
-  long long rowdata, d2, total;    // bytes
+  long long rowdata, d2, bits, total;      // bytes
 };
 BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
@@ -973,7 +1004,8 @@ BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   s.rowdata = bg * ROWDATA * ((R + 63) / 64 * 64) * 4;
   const long long q = s.q > 1 ? s.q * (long long)p.B * p.Nq * p.heads * 2 * p.d * 4 : 0, k = s.k > 1 ? 2ll * s.k * p.B * p.Nk * p.kv_heads * 2 * p.d * 4 : 0;
   s.d2 = s.q * bg * ((R + 63) / 64 * 64) * 4;
-  s.total = s.rowdata + s.d2 + (q > k ? q : k);
+  s.bits = p.mask ? ((p.mask_batch ? p.B : 1) * (long long)cdiv(p.Nq, 32) * p.Nk * 4 + 255) / 256 * 256 : 0;
+  s.total = s.rowdata + s.d2 + s.bits + (q > k ? q : k);
   return s;
 }
 inline int sum_grid(long long n) { return (int)(n / 1024 + 1 < 2048 ? n / 1024 + 1 : 2048); }
@@ -1028,7 +1060,14 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128) * s.q, kb = bg * cdiv(a.Nk, 128) * s.k;
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
   a.d2 = dlam && sizeof(T) == 2 ? a.rowdata + s.rowdata / 4 : nullptr;
-  a.part = a.rowdata + (s.rowdata + s.d2) / 4;
+  a.bits = (unsigned*)(a.rowdata + (s.rowdata + s.d2) / 4);
+  a.bits_b = a.m_b ? (long long)cdiv(a.Nq, 32) * a.Nk : 0;
+  a.part = a.rowdata + (s.rowdata + s.d2 + s.bits) / 4;
+  if (a.mask && a.dk) {
+    const int words = cdiv(a.Nq, 32);
+    if (words > 65535 || a.B > 65535) return FF3D_ERR_BAD_SHAPE;
+    bits_kernel<<<dim3(cdiv(a.Nk, 256), words, a.m_b ? a.B : 1), 256, 0, st>>>(a, words);
+  }
   rows_kernel<T><<<(unsigned)cdiv(rows, 16), 256, 0, st>>>(a);
   if (a.dk) {
     const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;

@@ -69,6 +69,16 @@ def test_diff_attention_masks_and_lengths(dtype, d):
     _check(q, k, v, lam, dout, H, G, kv_lens=torch.tensor([-5, 1, 92], dtype=torch.int32, device='cuda'))
 
 
+@pytest.mark.parametrize('B,Nq,H,G,d', [(2, 100, 6, 2, 16), (1, 45, 5, 1, 64), (1, 333, 4, 4, 32), (2, 70, 8, 1, 8)])
+@pytest.mark.parametrize('dtype', ['f32', 'f16'])
+def test_diff_attention_mask_words(dtype, B, Nq, H, G, d):
+    """Tiles of 32 packed rows that begin anywhere in a word of 32 queries: 3, 5, 1 and 8 heads per key head."""
+    q, k, v, lam, dout = _inputs(B, Nq, 131, H, G, d, DT[dtype], 19)
+    mask = torch.rand(B, Nq, 131, generator=torch.Generator(device='cuda').manual_seed(20), device='cuda') < 0.5
+    _check(q, k, v, lam, dout, H, G, mask=mask)
+    _check(q, k, v, lam, dout, H, G, mask=mask[0], causal=True)
+
+
 # few rows over long keys: slices that a second kernel joins, some of them without a key
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
 @pytest.mark.parametrize('B,Nq,Nk,H,G,d', [(1, 1, 5000, 1, 1, 64), (2, 1, 3001, 8, 2, 32), (3, 7, 1024, 4, 4, 16), (1, 2, 2050, 16, 1, 8)])
