@@ -98,11 +98,8 @@ __device__ __forceinline__ void transpose_tile_v4(const float* __restrict__ in, 
       const long long o = (long long)n * C + c;
       if (o1) *reinterpret_cast<float4*>(o1 + o) = v;
       if (o2) {
-        if (pe_reg) {                                        // the block's positional tile, read once for all of its frames
+        if (pe) {                                            // the block's positional tile, read once for all of its frames
           const float4 q = pe_reg[it];
-          v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
-        } else if (pe) {
-          const float4 q = *reinterpret_cast<const float4*>(pe + o);
           v.x += q.x; v.y += q.y; v.z += q.z; v.w += q.w;
         }
         if (split_plane < 0) {                               // one bf16 plane: 4 channels = one 8-byte store
@@ -159,7 +156,8 @@ __global__ __launch_bounds__(256) void bev_flatten_kernel(FlattenParams p) {
   // registers (4 float4 per value and thread in the 16-byte path).  Before, every frame's block read them again: Nv x C fp32 per
   // decoder stage - 2 x 43.5 MB at 180 x 180, 2 x 294 MB at 468 x 468, neither resident in an L2 across frames - 2.8 GB of the
   // 4.1 GB the kernel fetched per 32-frame launch (PMC FETCH_SIZE, profiles/r05_l_*), 4.7 of 7.1 GB at 468 x 468 x 8 frames.
-  const bool pe_regs = v4 && p.fb > 1;
+  // (For one frame too: a choice between the registers and the table's address puts the registers into scratch memory - the 32-frame
+  // launch at 180 x 180 then takes 1.72 ms.)
   float4 per0[TT / 16], per1[TT / 16], per2[TT / 16], per3[TT / 16];     // (four named arrays: indexed statically -> registers)
   auto load_pe = [&](int v, float4* pr) {
     const int l16 = threadIdx.x & 15, r16 = threadIdx.x >> 4;
@@ -167,7 +165,7 @@ __global__ __launch_bounds__(256) void bev_flatten_kernel(FlattenParams p) {
     for (int it = 0; it < TT / 16; ++it) {
       const int n = n0 + r16 + 16 * it, c = c0 + 4 * l16;
       pr[it] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (pe_regs && v < p.n_values && p.pos_embed[v] && n < HW && c < p.C)
+      if (v4 && v < p.n_values && p.pos_embed[v] && n < HW && c < p.C)
         pr[it] = *reinterpret_cast<const float4*>(p.pos_embed[v] + ((long long)p.lv.start[l] + n) * p.C + c);
     }
   };
@@ -195,7 +193,7 @@ __global__ __launch_bounds__(256) void bev_flatten_kernel(FlattenParams p) {
       }
       if (v4)
         transpose_tile_v4(in, HW, HW, p.C, n0, c0, pe, v == 0 ? o1 : nullptr, o2, tile, plane, split_scale, v == 0,
-                          (pe_regs && pe) ? pr : nullptr);
+                          pr);
       else
         transpose_tile(in, HW, HW, p.C, n0, c0, pe, v == 0 ? o1 : nullptr, o2, tile, plane, split_scale, v == 0);
     };
