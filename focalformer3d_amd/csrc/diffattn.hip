@@ -473,10 +473,29 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 }
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------
+// Before the products, in one launch: the first row_blocks blocks write the rows' values, the others the mask's words.
 // rowdata (B G, ROWDATA, Rp): maxima, D1 = <dO, out> + lam D2, D2 = <dO, O2>, 1 / sum 1, lam / sum 2; zeros behind R, whose
 // probabilities are therefore 0.  16 lanes per row.
+// Words: 32 queries' mask bytes of a key in one word.  The dk / dv kernel then needs a word or two per lane and step, and can ask for them
+// a step ahead (16 byte loads behind the step's DMA, in order, would make it wait for that: 93 instead of 122 us at 4 x 720 x 720, 8 heads
+// of 16, fp32, 27 instead of 48 at 3 x 333 x 1777, 4 heads of 32, fp16).
 template <typename T>
-__global__ __launch_bounds__(256) void rows_kernel(Args a) {
+__global__ __launch_bounds__(256) void prep_kernel(Args a, unsigned row_blocks) {
+  if (blockIdx.x >= row_blocks) {
+    const int words = (a.Nq + 31) / 32, jt = (a.Nk + 255) / 256;
+    const unsigned at = blockIdx.x - row_blocks;
+    const int j = (int)(at % jt) * 256 + threadIdx.x, w = (int)(at / jt % words), b = (int)(at / jt / words);
+    if (j >= a.Nk) return;
+    const uint8_t* p = a.mask + b * a.m_b + j;
+    uint8_t v[32];                 // all asked for before the first is looked at
+#pragma unroll
+    for (int k = 0; k < 32; ++k) v[k] = p[min(w * 32 + k, a.Nq - 1) * a.m_r];
+    unsigned bits = 0;
+#pragma unroll
+    for (int k = 0; k < 32; ++k) bits |= v[k] ? 1u << k : 0u;
+    a.bits[((long long)b * words + w) * a.Nk + j] = bits;
+    return;
+  }
   const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
   if (at >= (long long)a.B * a.G * a.Rp) return;
   const int bg = (int)(at / a.Rp), row = (int)(at % a.Rp), lane = threadIdx.x & 15;
@@ -500,48 +519,6 @@ __global__ __launch_bounds__(256) void rows_kernel(Args a) {
   if (lane == 0)
 #pragma unroll
     for (int k = 0; k < ROWDATA; ++k) a.rowdata[((long long)bg * ROWDATA + k) * a.Rp + row] = v[k];
-}
-
-// The mask's bytes turned into words of 32 queries per key: the dk / dv kernel then needs one word per lane and step, and can ask for it
-// a step ahead (16 byte loads behind the step's DMA, in order, would make it wait for that).
-__global__ __launch_bounds__(256) void bits_kernel(Args a, int words) {
-  const int j = blockIdx.x * 256 + threadIdx.x, w = blockIdx.y, b = blockIdx.z;
-  if (j >= a.Nk) return;
-  const uint8_t* p = a.mask + b * a.m_b + j;
-  uint8_t v[32];                   // all asked for before the first is looked at
-#pragma unroll
-  for (int k = 0; k < 32; ++k) v[k] = p[min(w * 32 + k, a.Nq - 1) * a.m_r];
-  unsigned bits = 0;
-#pragma unroll
-  for (int k = 0; k < 32; ++k) bits |= v[k] ? 1u << k : 0u;
-  a.bits[((long long)b * words + w) * a.Nk + j] = bits;
-}
-
-// dlam[h] = -sum over batch and queries of P2 dP: D2, in 16 bits + (what the dq kernel found beyond it) / sum 2; one block per head, fp64
-// sums in a fixed order
-template <typename T>
-__global__ __launch_bounds__(1024) void dlam_kernel(Args a, T* dlam) {
-  __shared__ double part[16];
-  const int h = blockIdx.x, g = h / a.r, x = h % a.r;
-  double s = 0.0;
-  const int n = a.B * a.Nq, slices = a.d2 ? a.splits : 0;
-  for (int bi = threadIdx.x; bi < n; bi += 1024) {
-    const int b = bi / a.Nq, bg = b * a.G + g;
-    const long long row = (long long)(bi - b * a.Nq) * a.r + x;
-    float rest = 0.f;
-#pragma unroll 16
-    for (int k = 0; k < slices; ++k) rest += a.d2[((long long)k * a.B * a.G + bg) * a.Rp + row];
-    s += (double)a.rowdata[((long long)bg * ROWDATA + 3) * a.Rp + row] + (double)(slices ? rest * a.stat[((long long)bg * 4 + 3) * a.R + row] : 0.f);
-  }
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s = 0.0;
-    for (int k = 0; k < 16; ++k) s += part[k];
-    dlam[h] = from_f<T>((float)-s);
-  }
 }
 
 // Where there are few row tiles, the keys of a row tile are cut into a.splits slices, whose sums go to a.part in fp32
@@ -946,19 +923,56 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
   }
 }
 
-// out[i] = sum over the slices of part[slice * step + i], in order; the second half of the grid, if any, does the same for out2
+// Behind the products, in one launch: the gradients' slices added in order, and dlam.
+// out[i] = sum over the slices of part[slice * step + i]
 template <typename T>
-__global__ __launch_bounds__(256) void sum_kernel(const float* part, T* out, T* out2, long long n, long long step, int slices) {
-  if (blockIdx.y) part += n, out = out2;
-  for (long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (long long)gridDim.x * 1024) {
-    float s[4] = {};
+struct SumJob {
+  const float* part;
+  T* out;
+  long long n, step;
+  int slices, blocks;
+};
+// dlam[h] = -sum over batch and queries of P2 dP: D2, in 16 bits + (what the dq kernel found beyond it) / sum 2; one block per head, fp64
+// sums in a fixed order
+template <typename T>
+__global__ __launch_bounds__(1024) void finish_kernel(Args a, T* dlam, SumJob<T> j0, SumJob<T> j1, SumJob<T> j2) {
+  int at = blockIdx.x - (dlam ? a.H : 0);
+  if (at >= 0) {
+    SumJob<T> j = j0;
+    if (at >= j0.blocks) at -= j0.blocks, j = j1;
+    if (at >= j.blocks) at -= j.blocks, j = j2;
+    for (long long i = ((long long)at * 1024 + threadIdx.x) * 4; i < j.n; i += (long long)j.blocks * 4096) {
+      float s[4] = {};
 #pragma unroll 8
-    for (int k = 0; k < slices; ++k) {
-      const Four<float> v = *(const Four<float>*)(part + k * step + i);
+      for (int k = 0; k < j.slices; ++k) {
+        const Four<float> v = *(const Four<float>*)(j.part + k * j.step + i);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] += v.v[e];
+        for (int e = 0; e < 4; ++e) s[e] += v.v[e];
+      }
+      put4(j.out + i, s[0], s[1], s[2], s[3]);
     }
-    put4(out + i, s[0], s[1], s[2], s[3]);
+    return;
+  }
+  __shared__ double part[16];
+  const int h = blockIdx.x, g = h / a.r, x = h % a.r;
+  double s = 0.0;
+  const int n = a.B * a.Nq, slices = a.d2 ? a.splits : 0;
+  for (int bi = threadIdx.x; bi < n; bi += 1024) {
+    const int b = bi / a.Nq, bg = b * a.G + g;
+    const long long row = (long long)(bi - b * a.Nq) * a.r + x;
+    float rest = 0.f;
+#pragma unroll 16
+    for (int k = 0; k < slices; ++k) rest += a.d2[((long long)k * a.B * a.G + bg) * a.Rp + row];
+    s += (double)a.rowdata[((long long)bg * ROWDATA + 3) * a.Rp + row] + (double)(slices ? rest * a.stat[((long long)bg * 4 + 3) * a.R + row] : 0.f);
+  }
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    for (int k = 0; k < 16; ++k) s += part[k];
+    dlam[h] = from_f<T>((float)-s);
   }
 }
 
@@ -986,10 +1000,10 @@ Split split_of(const ff3d_diff_attention_t& p) {
 }
 
 // Backward pass: the loop of a key tile (over rows) or of a row tile (over keys) is cut where the tiles alone leave the chip short of
-// blocks, to slices of at least 128 rows or keys; the slices' fp32 sums are added in order.  Both kernels use one place for them.
+// blocks, to slices of at least 128 rows or keys; the slices' fp32 sums are added in order.
 struct BwdSplit {
   int q, k;
-  long long rowdata, d2, bits, total;      // bytes
+  long long rowdata, d2, bits, dk, total;  // bytes
 };
 BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   const long long bg = (long long)p.B * p.kv_heads, R = (long long)p.Nq * (p.heads / p.kv_heads);
@@ -1002,13 +1016,14 @@ BwdSplit bwd_split_of(const ff3d_diff_attention_t& p) {
   s.q = slices(bg * cdiv(R, 128), p.Nk);
   s.k = slices(bg * cdiv(p.Nk, 128), R);
   s.rowdata = bg * ROWDATA * ((R + 63) / 64 * 64) * 4;
-  const long long q = s.q > 1 ? s.q * (long long)p.B * p.Nq * p.heads * 2 * p.d * 4 : 0, k = s.k > 1 ? 2ll * s.k * p.B * p.Nk * p.kv_heads * 2 * p.d * 4 : 0;
+  const long long q = s.q > 1 ? s.q * (long long)p.B * p.Nq * p.heads * 2 * p.d * 4 : 0;
+  s.dk = s.k > 1 ? 2ll * s.k * p.B * p.Nk * p.kv_heads * 2 * p.d * 4 : 0;
   s.d2 = s.q * bg * ((R + 63) / 64 * 64) * 4;
   s.bits = p.mask ? ((p.mask_batch ? p.B : 1) * (long long)cdiv(p.Nq, 32) * p.Nk * 4 + 255) / 256 * 256 : 0;
-  s.total = s.rowdata + s.d2 + s.bits + (q > k ? q : k);
+  s.total = s.rowdata + s.d2 + s.bits + s.dk + q;
   return s;
 }
-inline int sum_grid(long long n) { return (int)(n / 1024 + 1 < 2048 ? n / 1024 + 1 : 2048); }
+inline int sum_grid(long long n) { return (int)(n / 4096 + 1 < 1024 ? n / 4096 + 1 : 1024); }
 
 int check(const ff3d_diff_attention_t* p) {
   FF3D_REQUIRE(p && p->q && p->k && p->v && p->lam, FF3D_ERR_NULL);
@@ -1063,25 +1078,25 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   a.bits = (unsigned*)(a.rowdata + (s.rowdata + s.d2) / 4);
   a.bits_b = a.m_b ? (long long)cdiv(a.Nq, 32) * a.Nk : 0;
   a.part = a.rowdata + (s.rowdata + s.d2 + s.bits) / 4;
-  if (a.mask && a.dk) {
-    const int words = cdiv(a.Nq, 32);
-    if (words > 65535 || a.B > 65535) return FF3D_ERR_BAD_SHAPE;
-    bits_kernel<<<dim3(cdiv(a.Nk, 256), words, a.m_b ? a.B : 1), 256, 0, st>>>(a, words);
-  }
-  rows_kernel<T><<<(unsigned)cdiv(rows, 16), 256, 0, st>>>(a);
+  const long long row_blocks = cdiv(rows, 16), word_blocks = a.mask && a.dk ? (long long)cdiv(a.Nk, 256) * cdiv(a.Nq, 32) * (a.m_b ? a.B : 1) : 0;
+  if (row_blocks + word_blocks > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
+  prep_kernel<T><<<(unsigned)(row_blocks + word_blocks), 256, 0, st>>>(a, (unsigned)row_blocks);
+  SumJob<T> dk = {}, dv = {}, dq = {};
   if (a.dk) {
     const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;
     a.tiles = cdiv(a.Nk, 128), a.splits = s.k;
     (a.mask ? dkv_kernel<T, D, true> : dkv_kernel<T, D, false>)<<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
-    if (s.k > 1) sum_kernel<T><<<dim3(sum_grid(n), 2), 256, 0, st>>>(a.part, (T*)a.dk, (T*)a.dv, n, 2 * n, s.k);
+    if (s.k > 1) dk = {a.part, (T*)a.dk, n, 2 * n, s.k, sum_grid(n)}, dv = {a.part + n, (T*)a.dv, n, 2 * n, s.k, sum_grid(n)};
   }
+  a.part += s.dk / 4;
   if (a.dq || a.d2) {
     const long long n = (long long)a.B * a.Nq * a.H * 2 * a.d;
     a.tiles = cdiv(a.R, 128), a.splits = s.q;
     (a.mask ? dq_kernel<T, D, true> : dq_kernel<T, D, false>)<<<(unsigned)qb, 256, 0, st>>>(a);
-    if (s.q > 1 && a.dq) sum_kernel<T><<<sum_grid(n), 256, 0, st>>>(a.part, (T*)a.dq, nullptr, n, n, s.q);
+    if (s.q > 1 && a.dq) dq = {a.part, (T*)a.dq, n, n, s.q, sum_grid(n)};
   }
-  if (dlam) dlam_kernel<T><<<a.H, 1024, 0, st>>>(a, dlam);
+  const int blocks = (dlam ? a.H : 0) + dk.blocks + dv.blocks + dq.blocks;
+  if (blocks) finish_kernel<T><<<blocks, 1024, 0, st>>>(a, dlam, dk, dv, dq);
   return ff3d_launch_status();
 }
 
