@@ -9,6 +9,7 @@ import array
 import ctypes as C
 import functools
 import os
+import struct
 
 import torch
 
@@ -1866,19 +1867,27 @@ def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     return dx, dw, db
 
 
-def _attn_rows(t, name, like, B, N, width):
-    """t (B, N, width) of ``like``'s type and device -> itself, or a copy where its rows are not dense, aligned and in range."""
-    _same(t, like, name, (B, N, width))
-    per = 16 // t.element_size()
-    if (t.stride(2) != 1 or t.stride(0) % per or t.stride(1) % per or t.stride(1) < width or t.data_ptr() % 16
-            or t.stride(1) * t.element_size() >= 1 << 24):
+def _attn_rows(t, name, like, shape, per):
+    """t, of ``like``'s type and device and of ``shape`` -> (itself, or a copy where its rows are not dense, aligned and in range; its
+    address, batch and row stride).  A call's time on small inputs is what these checks take: each property is asked for once."""
+    if not isinstance(t, torch.Tensor) or t.dtype is not like.dtype or t.get_device() != like.get_device() or t.shape != shape:
+        _same(t, like, name, shape)
+    batch, row, col = t.stride()
+    p = t.data_ptr()
+    if col != 1 or (batch | row) % per or row < shape[2] or p % 16 or row * 16 >= per << 24:
         t = t.clone(memory_format=torch.contiguous_format)
-    return t
+        batch, row, col = t.stride()
+        p = t.data_ptr()
+    return t, p, batch, row
+
+
+_DIFF_ATTENTION = struct.Struct('6Q8q8if4x')            # the fields of _lib.DiffAttention
 
 
 def _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale):
-    """Checked arguments -> (struct, the tensors it points to)."""
-    if q.dtype not in _DTYPE:
+    """Checked arguments -> (struct, the tensors it points to, heads * 2 d and the other sizes)."""
+    code = _DTYPE.get(q.dtype)
+    if code is None:
         raise RuntimeError(f'diff_attention: expected fp32, bf16 or fp16 tensors, got {q.dtype}')
     kv_heads = heads if kv_heads is None else kv_heads
     if heads < 1 or kv_heads < 1 or heads % kv_heads:
@@ -1886,44 +1895,47 @@ def _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, s
     if q.dim() != 3 or k.dim() != 3 or q.shape[2] % (2 * heads) or q.shape[2] // (2 * heads) not in (8, 16, 32, 64):
         raise RuntimeError(f'diff_attention: expected q (B, Nq, heads * 2 d) and k (B, Nk, kv_heads * 2 d) with d = 8, 16, 32 or 64, got '
                            f'{tuple(q.shape)} and {tuple(k.shape)} for {heads} heads')
-    B, Nq, _ = q.shape
-    Nk, d = k.shape[1], q.shape[2] // (2 * heads)
-    q = _attn_rows(q, 'q', q, B, Nq, heads * 2 * d)
-    k = _attn_rows(k, 'k', q, B, Nk, kv_heads * 2 * d)
-    v = _attn_rows(v, 'v', q, B, Nk, kv_heads * 2 * d)
+    B, Nq, width = q.shape
+    Nk, d, per = k.shape[1], width // (2 * heads), 4 if code == 0 else 8
+    kshape = (B, Nk, kv_heads * 2 * d)
+    q, qp, qb, qr = _attn_rows(q, 'q', q, q.shape, per)
+    k, kp, kb, kr = _attn_rows(k, 'k', q, kshape, per)
+    v, vp, vb, vr = _attn_rows(v, 'v', q, kshape, per)
     _same(lam, q, 'lam', (heads,))
     lam = lam.contiguous()
-    mb = mr = 0
+    mp = mb = mr = lp = 0
     if mask is not None:
-        if not isinstance(mask, torch.Tensor) or mask.device != q.device or mask.dtype not in (torch.bool, torch.uint8):
+        if not isinstance(mask, torch.Tensor) or mask.get_device() != q.get_device() or mask.dtype not in (torch.bool, torch.uint8):
             raise RuntimeError(f'mask: expected a bool or uint8 tensor on {q.device} (True = not attended)')
-        if tuple(mask.shape) not in ((Nq, Nk), (1, Nq, Nk), (B, Nq, Nk)):
+        if mask.shape != (B, Nq, Nk) and tuple(mask.shape) not in ((Nq, Nk), (1, Nq, Nk)):
             raise RuntimeError(f'mask: expected shape {(Nq, Nk)} or {(B, Nq, Nk)}, got {tuple(mask.shape)}')
-        mask = (mask if mask.dim() == 3 else mask[None])
+        mask = mask if mask.dim() == 3 else mask[None]
         if Nk > 1 and mask.stride(2) != 1:
             mask = mask.contiguous()
-        mb, mr = mask.stride(0) if mask.shape[0] > 1 else 0, mask.stride(1)
+        mb, mr, _ = mask.stride()
+        mp, mb = mask.data_ptr(), mb if mask.shape[0] > 1 else 0
     if kv_lens is not None:
-        if not isinstance(kv_lens, torch.Tensor) or kv_lens.device != q.device or kv_lens.dtype != torch.int32 or tuple(kv_lens.shape) != (B,):
+        if (not isinstance(kv_lens, torch.Tensor) or kv_lens.get_device() != q.get_device() or kv_lens.dtype != torch.int32
+                or tuple(kv_lens.shape) != (B,)):
             raise RuntimeError(f'kv_lens: expected a ({B},) int32 tensor on {q.device}')
         kv_lens = kv_lens.contiguous()
+        lp = kv_lens.data_ptr()
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float('inf'):
         raise ValueError(f'diff_attention: scale {scale}: expected a positive number')
-    keep = (q, k, v, lam, mask, kv_lens)
-    p = _lib.DiffAttention(*[None if t is None else t.data_ptr() for t in keep], q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0),
-                           v.stride(1), mb, mr, B, Nq, Nk, heads, kv_heads, d, 1 if causal else 0, _DTYPE[q.dtype], scale)
-    return p, keep
+    p = _lib.DiffAttention.from_buffer_copy(_DIFF_ATTENTION.pack(qp, kp, vp, lam.data_ptr(), mp, lp, qb, qr, kb, kr, vb, vr, mb, mr,
+                                                                 B, Nq, Nk, heads, kv_heads, d, 1 if causal else 0, code, scale))
+    return p, (q, k, v, lam, mask, kv_lens), (B, Nq, Nk, kv_heads, per)
 
 
 def _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, save):
-    p, keep = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    p, keep, (B, Nq, Nk, kv_heads, _) = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
     dev, shape = q.device, q.shape
-    empty = p.B == 0 or p.Nq == 0 or p.Nk == 0
+    empty = 0 in (B, Nq, Nk)
     new = torch.zeros if empty else torch.empty
     out = new(shape, dtype=q.dtype, device=dev)
     out2 = new(shape, device=dev) if save else None
-    stat = new(p.B, p.kv_heads, 4, p.Nq * p.heads // p.kv_heads, device=dev) if save else None
+    stat = new((B, kv_heads, 4, Nq * heads // kv_heads), device=dev) if save else None
     if not empty:
         lib = _lib.load()
         n = lib.ff3d_diff_attention_workspace_bytes(p, 0)
@@ -1956,11 +1968,16 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None
                        want=(True, True, True, True)):
     """Gradients of ``diff_attention`` for dout (B, Nq, heads * 2 d) -> (dq, dk, dv, dlam); None where ``want`` is false (dk and dv are
     computed together)."""
-    p, keep = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    p, keep, (B, Nq, Nk, kv_heads, per) = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
     dev, dt = q.device, q.dtype
-    _same(out, q, 'out', q.shape)
-    dout = _attn_rows(dout, 'dout', q, p.B, p.Nq, q.shape[2])
-    empty = p.B == 0 or p.Nq == 0 or p.Nk == 0
+    stat_shape = (B, kv_heads, 4, Nq * heads // kv_heads)
+    if (out.dtype is not dt or out.shape != q.shape or out2.shape != q.shape or stat.shape != stat_shape
+            or not (out2.dtype is stat.dtype is torch.float32) or not (out.get_device() == out2.get_device() == stat.get_device() == q.get_device())
+            or not (out.is_contiguous() and out2.is_contiguous() and stat.is_contiguous())):
+        raise RuntimeError(f'diff_attention_bwd: out, out2, stat: expected what diff_attention_train_fwd gave: contiguous, {dt} and fp32, of '
+                           f'shapes {tuple(q.shape)}, {tuple(q.shape)} and {stat_shape}')
+    dout, dop, dob, dor = _attn_rows(dout, 'dout', q, q.shape, per)
+    empty = 0 in (B, Nq, Nk)
     new = torch.zeros if empty else torch.empty
     pair = want[1] or want[2]
     dq = new(q.shape, dtype=dt, device=dev) if want[0] else None
@@ -1969,7 +1986,7 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None
     if not empty and any(want):
         lib = _lib.load()
         ws = torch.empty(lib.ff3d_diff_attention_workspace_bytes(p, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.ff3d_diff_attention_bwd(p, _ptr(out), _ptr(out2), _ptr(stat), _ptr(dout), dout.stride(0), dout.stride(1), _ptr(dq), _ptr(dk),
+        _lib.check(lib.ff3d_diff_attention_bwd(p, out.data_ptr(), out2.data_ptr(), stat.data_ptr(), dop, dob, dor, _ptr(dq), _ptr(dk),
                                                _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), 'ff3d_diff_attention_bwd')
     return dq, dk if want[1] else None, dv if want[2] else None, dlam
 

@@ -250,3 +250,6 @@ def test_refusals_on_device():
     saved = ops.diff_attention_train_fwd(q, k, v, lam, 2)
     with pytest.raises(RuntimeError):
         ops.diff_attention_bwd(q, k, v, lam, 2, *saved, dout[:, :4])
+    for i, bad in ((0, saved[0][:, :4]), (0, saved[0].half()), (1, saved[1].half()), (1, saved[1].transpose(0, 1)), (2, saved[2][:, :1]), (2, saved[2].cpu())):
+        with pytest.raises(RuntimeError):
+            ops.diff_attention_bwd(q, k, v, lam, 2, *saved[:i], bad, *saved[i + 1:], dout)
