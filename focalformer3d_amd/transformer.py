@@ -392,10 +392,11 @@ class DifferentialAttention(nn.Module):
         if key_padding_mask is not None:
             pad = key_padding_mask.bool()[:, None, :].expand(B, N, N)
             mask = pad if mask is None else mask | pad
-        o = differential_attention(self._project(xp, self.q_proj), self._project(xp, self.k_proj), self._project(x, self.v_proj), self.lam(),
-                                   self.num_heads, kv_heads=self.kv_heads, mask=mask)
+        q = self._project(xp, self.q_proj)                 # (under autocast the projections' type is not the parameters')
+        o = differential_attention(q, self._project(xp, self.k_proj), self._project(x, self.v_proj), self.lam().to(q.dtype), self.num_heads,
+                                   kv_heads=self.kv_heads, mask=mask)
         heads = o.view(B, N, self.num_heads, -1)
-        o = F.rms_norm(heads, heads.shape[-1:], self.head_norm, self.eps) * (1.0 - self.lambda_init)
+        o = F.rms_norm(heads, heads.shape[-1:], self.head_norm.to(o.dtype), self.eps) * (1.0 - self.lambda_init)
         out = self._project(o.reshape(B, N, C), self.out_proj)
         return x + self.dropout_layer(self.proj_drop(out))
 
@@ -713,6 +714,8 @@ class GatedFFN(nn.Module):
         super().__init__()
         if num_fcs != 2:
             raise NotImplementedError('GatedFFN: one gated projection and one output projection (num_fcs=2)')
+        if dropout_layer and dropout_layer.get('drop_prob', 0.):
+            raise NotImplementedError('GatedFFN: ffn_drop is its dropout (dropout_layer)')
         self.act = act_cfg.get('type', 'SiLU').lower()
         if self.act not in ops._ACTS:
             raise NotImplementedError(f"act_cfg: type {act_cfg.get('type')!r} (SiLU, GELU, ReLU or Sigmoid)")

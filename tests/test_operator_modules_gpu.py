@@ -1,0 +1,207 @@
+"""The modules of the three-type operators - ``DifferentialAttention`` and ``GatedFFN`` in the places of ``MultiheadAttention`` and ``FFN``
+- and a training step of a head that uses both and clips its gradients.
+
+Module tolerances: a module is a chain of at most 6 sums of n <= 128 products (projections, scores, maps, norm, output), each of which
+adds n 2^-24 of its inputs' magnitude; the difference of two maps and the division by its norm enlarge what reaches them by at most
+(1 + lam) / |1 - lam| <= 9 at lam = 0.8: 6 * 128 * 9 * 2^-24 = 4.1e-4 relative to the result's norm (the kernels' own bounds are tested
+element by element elsewhere; here a wrong wiring has to show).  The backward pass doubles the chain."""
+import pytest
+import torch
+import torch.nn.functional as F
+
+pytestmark = pytest.mark.gpu
+REL = 6 * 128 * 9 * 2.0 ** -24
+
+
+def close(got, want, rel, what):
+    err = float((got.detach().double() - want.detach()).norm() / want.detach().norm().clamp_min(1e-30))
+    assert err <= rel, (what, err, rel)
+
+
+def plain_attention(m, P, x, pos, blocked):
+    """The module's formula in 64 bits; P: its parameters as doubles, blocked (B, N, N) or None."""
+    B, N, C = x.shape
+    H, G = m.num_heads, m.kv_heads
+    d = C // H // 2
+    lin = lambda t, n: F.linear(t, P[n + '.weight'], P[n + '.bias'])  # noqa: E731
+    xp = x if pos is None else x + pos
+    q = lin(xp, 'q_proj').view(B, N, H, 2, d).permute(0, 2, 3, 1, 4)
+    k = lin(xp, 'k_proj').view(B, N, G, 2, d).permute(0, 2, 3, 1, 4).repeat_interleave(H // G, 1)
+    v = lin(x, 'v_proj').view(B, N, G, 2 * d).transpose(1, 2).repeat_interleave(H // G, 1)
+    s = q @ k.transpose(-1, -2).contiguous() * d ** -0.5
+    if blocked is not None:
+        s = s.masked_fill(blocked[:, None, None], -1e300)
+    p = torch.softmax(s, -1)
+    if blocked is not None:
+        p = p * (~blocked)[:, None, None]
+    lam = torch.exp((P['lambda_q1'] * P['lambda_k1']).sum()) - torch.exp((P['lambda_q2'] * P['lambda_k2']).sum()) + m.lambda_init
+    o = (p[:, :, 0] - lam * p[:, :, 1]) @ v
+    o = o * torch.rsqrt(o.square().mean(-1, keepdim=True) + m.eps) * P['head_norm'] * (1 - m.lambda_init)
+    return x + lin(o.transpose(1, 2).reshape(B, N, C), 'out_proj')
+
+
+def plain_gated(m, P, x):
+    g, u = F.linear(x, P['in_proj.weight'], P['in_proj.bias']).chunk(2, -1)
+    a = {'silu': F.silu, 'gelu': F.gelu, 'relu': F.relu, 'sigmoid': torch.sigmoid}[m.act](g)
+    return x + F.linear(a * u, P['out_proj.weight'], P['out_proj.bias'])
+
+
+def doubles(m):
+    return {n: p.detach().double().requires_grad_(True) for n, p in m.named_parameters()}
+
+
+def attention_module(C, H, G, seed):
+    from focalformer3d_amd.registry import build_attention
+    import focalformer3d_amd.transformer  # noqa: F401
+    torch.manual_seed(seed)
+    m = build_attention(dict(type='DifferentialAttention', embed_dims=C, num_heads=H, kv_heads=G, dropout=0.0, batch_first=True)).cuda()
+    with torch.no_grad():
+        for n, p in m.named_parameters():
+            if n.endswith('bias') or n == 'head_norm':
+                p.add_(torch.randn_like(p) * 0.1)
+    return m
+
+
+@pytest.mark.parametrize('C,H,G,N,masked', [(64, 4, 4, 50, 'none'), (64, 2, 1, 50, 'frame'), (128, 8, 2, 33, 'all'), (128, 1, 1, 7, 'heads'),
+                                            (64, 4, 2, 40, 'padding'), (64, 4, 4, 1, 'none')])
+def test_differential_attention_module(C, H, G, N, masked):
+    B = 2
+    m = attention_module(C, H, G, 1)
+    gen = torch.Generator('cuda').manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=gen, device='cuda')  # noqa: E731
+    x, pos, dout = r(B, N, C), r(B, N, C), r(B, N, C)
+    holes = torch.rand(B, N, N, generator=gen, device='cuda') < 0.3
+    holes[:, N // 2] = True                                       # a query that sees nothing
+    pad = torch.zeros(B, N, dtype=torch.bool, device='cuda')
+    pad[1, N // 3:] = True
+    kw, blocked = dict(none=({}, None), frame=(dict(attn_mask=holes), holes), all=(dict(attn_mask=holes[0]), holes[:1].expand(B, N, N)),
+                       heads=(dict(attn_mask=torch.where(holes, -1e4, 0.0)), holes),
+                       padding=(dict(attn_mask=holes, key_padding_mask=pad), holes | pad[:, None]))[masked]
+    P, xd, pd = doubles(m), x.double().requires_grad_(True), pos.double().requires_grad_(True)
+    want = plain_attention(m, P, xd, pd, blocked)
+    names = list(P)
+    wg = torch.autograd.grad(want, [xd, pd, *P.values()], dout.double())
+    x.requires_grad_(True), pos.requires_grad_(True)
+    got = m.train()(x, query_pos=pos, **kw)
+    close(got, want, REL, 'training route')
+    gg = torch.autograd.grad(got, [x, pos, *m.parameters()], dout)
+    floor = 2 * REL * max(float(g.norm() / g.numel() ** 0.5) for g in wg)                # of gradients that cancel (a key's shift: 0)
+    for n, a, b in zip(['x', 'pos', *names], gg, wg):
+        err = float((a.double() - b).norm())
+        assert err <= 2 * REL * float(b.norm()) + floor * b.numel() ** 0.5, (n, err, float(b.norm()))
+    with torch.no_grad():
+        close(m.eval()(x, query_pos=pos, **kw), want, REL, 'inference route')
+        seq = attention_module(C, H, G, 1)
+        seq.batch_first = False
+        t = seq(x.transpose(0, 1), query_pos=pos.transpose(0, 1), **kw)
+        close(t.transpose(0, 1), want, REL, 'sequence first')
+
+
+@pytest.mark.parametrize('act', ['SiLU', 'GELU', 'ReLU', 'Sigmoid'])
+def test_gated_ffn_module(act):
+    from focalformer3d_amd.registry import build_feedforward_network
+    import focalformer3d_amd.transformer  # noqa: F401
+    torch.manual_seed(3)
+    m = build_feedforward_network(dict(type='GatedFFN', embed_dims=48, feedforward_channels=100, act_cfg=dict(type=act, inplace=True))).cuda()
+    x, dout = torch.randn(2, 3, 37, 48, device='cuda')
+    P, xd = doubles(m), x.double().requires_grad_(True)
+    want = plain_gated(m, P, xd)
+    wg = torch.autograd.grad(want, [xd, *P.values()], dout.double())
+    x.requires_grad_(True)
+    got = m.train()(x)
+    close(got, want, REL, 'training route')
+    for n, a, b in zip(['x', *P], torch.autograd.grad(got, [x, *m.parameters()], dout), wg):
+        close(a, b, 2 * REL, n)
+    with torch.no_grad():
+        close(m.eval()(x), want, REL, 'inference route')
+        m.gemm_dtype = torch.bfloat16
+        # bf16 operands and hidden row: four roundings of 2^-8, averaged over the sums they enter
+        close(m(x), want, 4 * 2.0 ** -8, 'bf16 mode')
+        w = m.in_proj.weight.clone()
+        m.in_proj.weight.mul_(2.0)                                # the bf16 weights follow the parameter
+        m.invalidate_cache()
+        P['in_proj.weight'] = 2.0 * w.double()
+        close(m(x), plain_gated(m, P, xd), 4 * 2.0 ** -8, 'bf16 mode, new weights')
+
+
+def test_modules_under_autocast():
+    """Activations in bf16, parameters in fp32: the operators run in the activations' type.  Roundings of 2^-8 at 6 places, enlarged 9 times
+    by the difference of the maps."""
+    m = attention_module(64, 4, 2, 5).train()
+    x = torch.randn(2, 20, 64, device='cuda', requires_grad=True)
+    want = plain_attention(m, doubles(m), x.detach().double(), None, None)
+    with torch.autocast('cuda', torch.bfloat16):
+        got = m(x)
+    close(got.float(), want, 6 * 9 * 2.0 ** -8, 'autocast')
+    got.float().square().sum().backward()
+    assert all(bool(torch.isfinite(p.grad).all()) and p.grad.dtype == torch.float32 for p in m.parameters())
+
+
+def _head(train_cfg):
+    from focalformer3d_amd.synthetic import build_head_from_cfg, focalformer3d_l_head_cfg
+    cfg = focalformer3d_l_head_cfg(C=128, grid=180, num_proposals=200, stages=3, decoder_stages=2)
+    cfg['add_gt_groups'] = 0
+    layer = cfg['decoder_cfg']['transformerlayers']
+    layer['attn_cfgs'][0] = dict(type='DifferentialAttention', embed_dims=128, num_heads=8, dropout=0.1)
+    layer['ffn_cfgs'] = dict(type='GatedFFN', embed_dims=128, num_fcs=2, act_cfg=dict(type='SiLU'))
+    if train_cfg:
+        cfg['train_cfg'] = dict(
+            dataset='nuScenes',
+            assigner=dict(type='HungarianAssigner3D', iou_calculator=dict(type='BboxOverlaps3D', coordinate='lidar'),
+                          cls_cost=dict(type='FocalLossCost', gamma=2, alpha=0.25, weight=0.15),
+                          reg_cost=dict(type='BBoxBEVL1Cost', weight=0.25), iou_cost=dict(type='IoU3DCost', weight=0.25)),
+            pos_weight=-1, gaussian_overlap=0.1, min_radius=2, grid_size=[1440, 1440, 40], voxel_size=[0.075, 0.075, 0.2],
+            out_size_factor=8, code_weights=[1.0] * 8 + [0.2, 0.2], point_cloud_range=[-54.0, -54.0, -5.0, 54.0, 54.0, 3.0])
+    return build_head_from_cfg(cfg, seed=0, device='cuda')
+
+
+def test_head_with_both_modules_routes_agree():
+    """Training and inference route of a head with both modules are two implementations of one function.  2e-4 of the largest value is what
+    the head with plain attention is held to; the difference of the maps enlarges an attention's share 9 times and (1 - lambda_init) = 0.2
+    scales it: 1.8 * 2e-4."""
+    from focalformer3d_amd.synthetic import stage_features
+    from tests.util import align_queries, permute_queries
+    head = _head(False)
+    inputs = stage_features(2, 128, 180, 3, seed=1, device='cuda')
+    ev = head.eval()(inputs, None, [{}] * 2)[0][0]
+    ev_labels = head.query_labels.clone()
+    head.train()
+    for m in head.modules():
+        if isinstance(m, (torch.nn.BatchNorm1d, torch.nn.BatchNorm2d, torch.nn.Dropout)):
+            m.eval()
+    with torch.no_grad():
+        tr = head(inputs, None, [{}] * 2)[0][0]
+    tr_labels = head.query_labels.clone()
+    nq = tr_labels.shape[1]
+    perm = align_queries({'center': tr['center'].detach()}, {'center': ev['center']}, tr_labels, ev_labels, nq, nq // 3, max_moved=12)
+    for key in ('center', 'height', 'dim', 'rot', 'vel', 'heatmap', 'query_heatmap_score'):
+        scale = max(1.0, float(ev[key].abs().max()))
+        assert float((tr[key].cpu() - permute_queries(ev[key].cpu(), perm, nq)).abs().max()) <= 1.8 * 2e-4 * scale, key
+
+
+def test_training_step_with_clipped_gradients():
+    """Forward, loss, backward, clipping and the optimizer's step of a head with both modules."""
+    from focalformer3d_amd import training
+    from focalformer3d_amd.synthetic import stage_features
+    head = _head(True).train()
+    inputs = stage_features(2, 128, 180, 3, seed=1, device='cuda')
+    gts = [torch.tensor([[5.0, 3.0, -1.0, 4.0, 2.0, 1.5, 0.3, 0.1, 0.2], [-20.0, 11.0, -1.0, 4.2, 1.9, 1.6, 1.2, 0.0, 0.0]], device='cuda')] * 2
+    labels = [torch.tensor([0, 3], device='cuda')] * 2
+    preds = head(inputs, None, [{}] * 2, gt_bboxes_3d=gts, gt_labels_3d=labels)
+    losses = head.loss(gts, labels, preds)
+    sum(v for k, v in losses.items() if 'loss' in k).backward()
+    layers = [layer for dec in head.decoder for layer in dec.layers]
+    for layer in layers:
+        for n, p in [*layer.attentions[0].named_parameters(), *layer.ffns[0].named_parameters()]:
+            assert p.grad is not None and bool(torch.isfinite(p.grad).all()) and float(p.grad.abs().max()) > 0.0, n
+    params = [p for p in head.parameters() if p.grad is not None]
+    before = [p.grad.double() for p in params]
+    norm = float(torch.stack([g.square().sum() for g in before]).sum().sqrt())
+    got = training.clip_grad_norm_(head.parameters(), 0.1)
+    assert abs(float(got) - norm) <= 2.0 ** -22 * norm                      # fp64 sums, one rounding; two more for the comparison
+    factor = min(1.0, 0.1 / (norm + 1e-6))
+    for p, g in zip(params, before):                                        # the factor and the product, each rounded to fp32
+        assert bool(((p.grad.double() - g * factor).abs() <= 2.0 ** -22 * (g * factor).abs() + 2.0 ** -149).all())
+    values = [p.detach().clone() for p in params]
+    torch.optim.SGD(params, lr=0.5).step()
+    assert sum(not torch.equal(p, v) for p, v in zip(params, values)) > len(params) // 2

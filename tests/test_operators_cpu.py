@@ -93,3 +93,32 @@ def test_diff_attention_entry_checks_its_arguments():
     for n in ('out', 'out2', 'lse', 'dout', 'ws', 'dk', 'dv'):
         assert bwd(**{n: None}) == -4, n
     assert bwd(dr=32) == -1 and bwd(dr=66) == -3 and bwd(dq=P + 4) == -3
+
+
+def test_modules_refuse_what_they_cannot_do():
+    import focalformer3d_amd.transformer  # noqa: F401
+    from focalformer3d_amd.registry import build_attention, build_feedforward_network
+    ok = dict(type='DifferentialAttention', embed_dims=64, num_heads=4)
+    m = build_attention(dict(ok, dropout=0.1, batch_first=True))
+    assert m.kv_heads == 4 and m.dropout_layer.p == 0.1 and tuple(m.lam().shape) == (4,)
+    assert tuple(build_attention(dict(ok, kv_heads=2)).k_proj.weight.shape) == (32, 64)
+    for bad in (dict(num_heads=3), dict(num_heads=8), dict(embed_dims=60), dict(kv_heads=3), dict(kv_heads=0), dict(embed_dims=1024)):
+        with pytest.raises(ValueError):
+            build_attention({**ok, **bad})
+    for bad in (dict(attn_drop=0.1), dict(dropout_layer=dict(type='DropPath', drop_prob=0.1))):
+        with pytest.raises(NotImplementedError):
+            build_attention({**ok, **bad})
+    x = torch.zeros(2, 5, 64)
+    for bad in (dict(key=x.clone()), dict(value=x.clone()), dict(identity=x), dict(query_pos=x, key_pos=x.clone())):
+        with pytest.raises(NotImplementedError):
+            m(x, **bad)
+    with pytest.raises(RuntimeError, match='CUDA'):
+        m(x)
+    ffn = dict(type='GatedFFN', embed_dims=64, feedforward_channels=96)
+    g = build_feedforward_network(ffn)
+    assert tuple(g.in_proj.weight.shape) == (192, 64) and g.act == 'silu'
+    for bad in (dict(num_fcs=3), dict(act_cfg=dict(type='Tanh')), dict(dropout_layer=dict(type='Dropout', drop_prob=0.5))):
+        with pytest.raises(NotImplementedError):
+            build_feedforward_network({**ffn, **bad})
+    with pytest.raises(RuntimeError, match='CUDA'):
+        g(x)
