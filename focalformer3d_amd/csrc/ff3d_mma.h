@@ -44,18 +44,27 @@ template <>
 struct Op<float> {
   vec8<__bf16> h, m, l;
 };
+// two values rounded to bf16 in one register, the first one in the low half
+__device__ __forceinline__ unsigned pack_bf16(float a, float b) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const bf16x2 v = __builtin_convertvector((f32x2){a, b}, bf16x2);
+  return __builtin_bit_cast(unsigned, v);
+}
 template <typename T>
 __device__ __forceinline__ Op<T> op(vec8<T> x) {
   if constexpr (sizeof(T) == 2) {
     return {x};
   } else {
     Op<float> o;
+    unsigned *h = (unsigned*)&o.h, *m = (unsigned*)&o.m, *l = (unsigned*)&o.l;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const __bf16 h = (__bf16)x[e];
-      const float r = x[e] - (float)h;               // exact
-      const __bf16 m = (__bf16)r;
-      o.h[e] = h, o.m[e] = m, o.l[e] = (__bf16)(r - (float)m);
+    for (int e = 0; e < 4; ++e) {                    // in pairs: one conversion per plane, 5.5 instructions per element instead of 7.5
+      const float x0 = x[2 * e], x1 = x[2 * e + 1];
+      h[e] = pack_bf16(x0, x1);
+      const float r0 = x0 - __uint_as_float(h[e] << 16), r1 = x1 - __uint_as_float(h[e] & 0xffff0000u);     // exact
+      m[e] = pack_bf16(r0, r1);
+      l[e] = pack_bf16(r0 - __uint_as_float(m[e] << 16), r1 - __uint_as_float(m[e] & 0xffff0000u));
     }
     return o;
   }
