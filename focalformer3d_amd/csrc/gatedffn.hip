@@ -112,7 +112,7 @@ __device__ __forceinline__ void load4(const T* p, float* v, int left, bool vec) 
 
 // The loop over the long sum.  Blocks of 8 waves (256 x 256): steps of 64 bytes of k in a ring of four; the two waves of a SIMD work
 // half a step apart, one reading its operands and asking for the step after next but one while the other multiplies, so the matrix
-// unit of the SIMD is fed without a pause (d W at 16384 x 5472 x 1024 in bf16: 182 us, against 217 with two steps of 128 bytes that
+// unit of the SIMD is fed without a pause (dx of 16384 x 1024 over 5472 in bf16: 182 us, against 217 with two steps of 128 bytes that
 // all waves read, multiply and wait for together).  Blocks of 4 waves: two or more share a CU and fill each other's waits; two steps
 // of 128 bytes (128 x 128, the same product: 221 us, 250 with the ring).
 constexpr int step_bytes_of(int waves) { return waves == 8 ? 64 : 128; }
@@ -558,23 +558,36 @@ int launch(GemmArgs a, hipStream_t st) {
   return ff3d_launch_status();
 }
 
-// Which tile, and into how many slices a long sum is cut: the least of an estimate in microseconds.  The most loaded CU runs `deep`
-// blocks, each (K / slices + 256) * per_k long (256 for filling and draining; per_k measured in bf16 on dx of 16384 x 1024 x 5472, one
-// 256 x 256 block or two 128 x 128 on each CU; fp32 runs at a quarter of that); slices cost their fp32 sums, written and read at 5 TB/s.
+// Which tile, and into how many slices a long sum is cut: the least of an estimate in microseconds.  Blocks run in rounds that fill the
+// chip's places; an element of k takes a round between `alone` (one block on a few CUs: latency) and `full` (every place taken), half by
+// how many places are taken and half by how many on the fullest CU, and the first round its filling and draining, which grow with it.  Slices cost their fp32 sums, written and read at 4.5 TB/s, and a launch.
+// Measured on 600 .. 16384 rows of 112 .. 1024 columns to 192 .. 2736 and both gradients: e.g. 1024 x 1024 -> 2736 forward in bf16 17 us
+// in 128 x 128 tiles, 27 in 256 x 256 ones; 2880 x 256 -> 1024 8 us in 64 x 128 tiles, 13 in 256 x 256 ones; 16384 x 5472 x 1024 190 us in
+// 256 x 256 tiles, 225 in 128 x 128 ones.
+inline long long slice_length(long long K, int slices) { return align_up(cdiv(K, slices), 64); }
+
 struct Tile {
   int id, bm, bn, slices;
 };
 template <typename T>
 Tile pick(long long M, long long N, long long K, bool dual, bool cut) {
   const int half = dual ? 2 : 1;
-  const struct { int bm, bn, per_cu; double per_k; } t[3] = {{256, 256 / half, 1, 0.033}, {128, 128 / half, 2, 0.020}, {64, 128 / half, 3, 0.013}};
+  constexpr bool F32 = sizeof(T) == 4;
+  const struct { int bm, bn, per_cu; double alone, full, fixed; } t[3] = {
+      {256, 256 / half, 1, 0.0184, 0.029, 6.0},
+      {128, 128 / half, 2, F32 ? 0.047 : 0.0113, F32 ? 0.075 : 0.0165, F32 ? 6.0 : 3.0},
+      {64, 128 / half, 3, F32 ? 0.033 : 0.0105, F32 ? 0.073 : 0.0155, F32 ? 5.0 : 2.5}};
   Tile best = {2, t[2].bm, t[2].bn, 1};
   double least = 1e300;
-  for (int i = sizeof(T) == 4 ? 1 : 0; i < 3; ++i)
-    for (int s = 1; s <= (cut ? 16 : 1) && (s == 1 || K / s >= 256); ++s) {
-      const long long blocks = (long long)cdiv(M, t[i].bm) * cdiv(N, t[i].bn) * s, slots = 256ll * t[i].per_cu;
-      const double deep = (double)(blocks / slots * t[i].per_cu + cdiv(blocks % slots, 256));
-      const double cost = deep * ((double)K / s + 256) * t[i].per_k * (sizeof(T) == 4 ? 4 : 1) + (s > 1 ? 5 + s * (double)M * N * 8 / 5e6 : 0);
+  for (int i = F32 ? 1 : 0; i < 3; ++i)
+    for (int s = 1; s <= (cut ? 16 : 1) && (s == 1 || K / s >= 128); ++s) {
+      const long long k = s > 1 ? slice_length(K, s) : K;
+      const long long blocks = (long long)cdiv(M, t[i].bm) * cdiv(N, t[i].bn) * cdiv(K, k), slots = 256ll * t[i].per_cu;
+      const double part = (double)(blocks % slots) / slots, deep = t[i].per_cu > 1 ? (double)cdiv(blocks % slots, 256) / t[i].per_cu : part;
+      const double rest = 0.5 * (part + deep), first = blocks < slots ? rest : 1.0;
+      const double round = t[i].alone + (t[i].full - t[i].alone) * rest;
+      const double cost = t[i].fixed * (1 + first) + k * ((double)(blocks / slots) * t[i].full + (rest > 0 ? round : 0)) +
+                          (s > 1 ? 5 + s * (double)M * N * 8 / 4.5e6 : 0);
       if (cost < least) least = cost, best = {i, t[i].bm, t[i].bn, s};
     }
   return best;
@@ -595,7 +608,7 @@ struct Plan {                    // of one call: packed operands, partial sums, 
 // bytes of the slices of a product of M x N over K (0: one piece), and their length
 template <typename T>
 long long slices_of(const Tile& t, long long M, long long N, long long K, int* kslice, int* slices) {
-  *kslice = (int)align_up(cdiv(K, t.slices), 64);
+  *kslice = t.slices > 1 ? (int)slice_length(K, t.slices) : (int)K;
   *slices = cdiv(K, *kslice);
   return *slices > 1 ? *slices * M * N * 4 : 0;
 }
