@@ -118,8 +118,8 @@ SIGNATURES = {
     'ff3d_gated_linear_fwd': (_i, [_vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     'ff3d_gated_linear_bwd': (_i, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
     'ff3d_diff_attention_workspace_bytes': (_i64, [_dp, _i]),
-    'ff3d_diff_attention_fwd': (_i, [_dp] + [_vp] * 5),
-    'ff3d_diff_attention_bwd': (_i, [_dp] + [_vp] * 4 + [_i64, _i64] + [_vp] * 6),
+    'ff3d_diff_attention_fwd': (_i, [_dp] + [_vp] * 6),
+    'ff3d_diff_attention_bwd': (_i, [_dp] + [_vp] * 5 + [_i64, _i64] + [_vp] * 6),
     'ff3d_grad_norm_workspace_bytes': (_i64, [_vp, _i]),
     'ff3d_grad_norm': (_i, [_vp, _vp, _vp, _i, _i, _vp, _vp, _vp]),
     'ff3d_clip_grads': (_i, [_vp] * 5 + [_i, _i, _f, _vp, _vp, _vp]),

@@ -176,17 +176,17 @@ class DifferentialAttentionFunction(Function):
 
     @staticmethod
     def forward(ctx, q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale):
-        out, out2, stat = ops.diff_attention_train_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
-        ctx.save_for_backward(q, k, v, lam, out, out2, stat, mask, kv_lens)
+        out, out2, stat, rest = ops.diff_attention_train_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+        ctx.save_for_backward(q, k, v, lam, out, out2, stat, rest, mask, kv_lens)
         ctx.meta = heads, kv_heads, causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, lam, out, out2, stat, mask, kv_lens = ctx.saved_tensors
+        q, k, v, lam, out, out2, stat, rest, mask, kv_lens = ctx.saved_tensors
         heads, kv_heads, causal, scale = ctx.meta
-        grads = ops.diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads, mask, kv_lens, causal, scale, ctx.needs_input_grad[:4])
+        grads = ops.diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, rest, dout, kv_heads, mask, kv_lens, causal, scale, ctx.needs_input_grad[:4])
         return (*grads, None, None, None, None, None, None)
 
 

@@ -34,9 +34,9 @@ struct Args {
   unsigned* bits;                 // backward: the mask by keys, word (b, i / 32, j) bit i % 32
   long long q_b, q_r, k_b, k_r, v_b, v_r, do_b, do_r;     // elements
   long long m_b, m_r, bits_b;                             // bytes, words
-  char *out, *dq, *dk, *dv;
+  char *out, *out_rest, *dq, *dk, *dv;
   float *out2, *stat, *part, *rowdata, *d2;
-  int B, Nq, Nk, H, G, r, rlog, d, R, Rp, causal, splits, split_len, tiles;     // rlog: log2 r, or -1
+  int B, Nq, Nk, H, G, r, rlog, d, R, Rp, causal, splits, split_len, tiles;   // rlog: log2 r, or -1
   float scale, c;                 // c = scale * log2(e)
 };
 
@@ -85,6 +85,26 @@ __device__ __forceinline__ vec8<T> scaled_frag(const f32x16& c, int step, float 
   } else {
     return acc_frag<T>(c, step);
   }
+}
+
+// What scaled_frag's rounding left, for a second product.  dS = P (dP - D) sums to nothing over the keys, so what remains of dS K is small
+// against its terms, and rounding those once gives dq 1.5 to 2.1 times, dk 1.4 to 2.3 times the error of rounding the result alone (8 or
+// 16 columns per map, or few keys).  With the second product it is 1.0 to 1.2 times.  It is left out (FINE false) where the products are
+// the bound and the sums are long: 64 columns and more than 2^24 pairs, 1.4 to 1.5 times.
+template <typename T>
+__device__ __forceinline__ vec8<T> rest_frag(const f32x16& c, int step, float mul, const vec8<T>& v) {
+  vec8<T> r;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = from_f<T>(fmaf(c[8 * step + e], mul, -to_f(v[e])));
+  return r;
+}
+
+// What the rounding of an output left: the backward pass needs <dO, out>, which it takes from every term of a row's sum, to more digits
+// than 16 bits hold (with 3 or 4 keys dq's error is 1.1 to 1.2 times that of rounding it, without this 1.6 to 1.7 times)
+template <typename T>
+__device__ __forceinline__ float rest_of(float x) {
+  const float r = x - to_f(from_f<T>(x));
+  return fabsf(x) < INFINITY && fabsf(r) < INFINITY ? r : 0.f;       // an output beyond the type's range is what it is
 }
 
 // ROWS rows of 2 D elements in LDS, in granules: [map 1 | map 2] of D each (SPLIT; the d of a map may fill only a part) or 2 d elements
@@ -351,6 +371,8 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
     for (int k = 0; k < 4; ++k) z[k] = o2[k] * inv[1], y[k] = o1[k] * inv[0] - lam * z[k];
     put4((T*)a.out + at * 2 * a.d + e, y[0], y[1], y[2], y[3]);
     if (a.out2) put4(a.out2 + at * 2 * a.d + e, z[0], z[1], z[2], z[3]);
+    if constexpr (sizeof(T) == 2)
+      if (a.out_rest) put4((T*)a.out_rest + at * 2 * a.d + e, rest_of<T>(y[0]), rest_of<T>(y[1]), rest_of<T>(y[2]), rest_of<T>(y[3]));
   };
   auto emit_row = [&] {
     if (!in || half) return;
@@ -467,8 +489,10 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
     for (int k = 0; k < groups; ++k) o1 += sum[k * w4 + tid], o2 += sum[k * w4 + 2 * a.d + tid];
     const long long to = (((long long)b * a.Nq + i) * a.H + h) * 2 * a.d + tid;
     const float z = o2 * norm[1];
-    ((T*)a.out)[to] = from_f<T>(o1 * norm[0] - to_f(((const T*)a.lam)[h]) * z);
+    const float y = o1 * norm[0] - to_f(((const T*)a.lam)[h]) * z;
+    ((T*)a.out)[to] = from_f<T>(y);
     if (a.out2) a.out2[to] = z;
+    if (sizeof(T) == 2 && a.out_rest) ((T*)a.out_rest)[to] = from_f<T>(rest_of<T>(y));
   }
 }
 
@@ -507,7 +531,9 @@ __global__ __launch_bounds__(256) void prep_kernel(Args a, unsigned row_blocks) 
     float d = 0.f, d2 = 0.f;
     for (int e = lane; e < 2 * a.d; e += 16) {
       const float x = to_f(go[e]);
-      d = fmaf(x, to_f(((const T*)a.out)[o + e]), d);
+      float y = to_f(((const T*)a.out)[o + e]);
+      if constexpr (sizeof(T) == 2) y += to_f(((const T*)a.out_rest)[o + e]);
+      d = fmaf(x, y, d);
       d2 = fmaf(x, a.out2[o + e], d2);
     }
 #pragma unroll
@@ -522,7 +548,7 @@ __global__ __launch_bounds__(256) void prep_kernel(Args a, unsigned row_blocks) 
 }
 
 // Where there are few row tiles, the keys of a row tile are cut into a.splits slices, whose sums go to a.part in fp32
-template <typename T, int D, bool MASK>
+template <typename T, int D, bool MASK, bool FINE>
 __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(Args a) {
   constexpr int NT = 256, KT = sizeof(T) == 2 ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = KT * GR * 16;
   constexpr int ST = D / 16, VS = 2 * D / 16, QT = D >= 32 ? D / 32 : 1;
@@ -625,10 +651,18 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
         sc[m].template see<QT>(top[m], acc[m]);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
-          const Op<T> f = op<T>(scaled_frag<T>(s[m], st, sc[m].mul()));
+          const vec8<T> ds = scaled_frag<T>(s[m], st, sc[m].mul());
+          const Op<T> f = op<T>(ds);
+          Op<T> x[QT];
 #pragma unroll
-          for (int x = 0; x < QT; ++x)
-            acc[m][x] = mfma_step<T>(op<T>(col_frag_acc<T, GR>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + x * 32, lane)), f, acc[m][x]);
+          for (int t = 0; t < QT; ++t) x[t] = op<T>(col_frag_acc<T, GR>(kt, kb * 32 + 16 * st, (D >= 32 ? m * D : 0) + t * 32, lane));
+#pragma unroll
+          for (int t = 0; t < QT; ++t) acc[m][t] = mfma_step<T>(x[t], f, acc[m][t]);
+          if constexpr (FINE) {
+            const Op<T> rest = op<T>(rest_frag<T>(s[m], st, sc[m].mul(), ds));
+#pragma unroll
+            for (int t = 0; t < QT; ++t) acc[m][t] = mfma_step<T>(x[t], rest, acc[m][t]);
+          }
         }
       }
     }
@@ -664,7 +698,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
 template <typename T, int D>
 constexpr bool wide_v = D == 64 && sizeof(T) == 2;
 
-template <typename T, int D, bool MASK>
+template <typename T, int D, bool MASK, bool FINE>
 __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : waves_of(D, sizeof(T), false))) void dkv_kernel(Args a) {
   constexpr bool WIDE = wide_v<T, D>;
   constexpr int NT = WIDE ? 512 : 256, QR = (sizeof(T) == 2 && D != 32) ? 64 : 32, P = Type<T>::PER16, GR = 2 * D / P, BYTES = QR * GR * 16;
@@ -849,7 +883,8 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
       sk[1].template see<QT>(top[2], dk[1]);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const Op<T> f[2] = {op<T>(scaled_frag<T>(s[0], st, sk[0].mul())), op<T>(scaled_frag<T>(s[1], st, sk[1].mul()))};
+        const vec8<T> ds[2] = {scaled_frag<T>(s[0], st, sk[0].mul()), scaled_frag<T>(s[1], st, sk[1].mul())};
+        const Op<T> f[2] = {op<T>(ds[0]), op<T>(ds[1])};
         vec8<T> x[2][QT];          // d = 16: both maps share the columns of one tile
 #pragma unroll
         for (int m = 0; m < (D >= 32 ? 2 : 1); ++m)
@@ -860,6 +895,14 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
         for (int m = 0; m < 2; ++m)
 #pragma unroll
           for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), f[m], dk[m][t]);
+        if constexpr (FINE) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const Op<T> rest = op<T>(rest_frag<T>(s[m], st, sk[m].mul(), ds[m]));
+#pragma unroll
+            for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), rest, dk[m][t]);
+          }
+        }
       }
     }
   }
@@ -1075,6 +1118,10 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128) * s.q, kb = bg * cdiv(a.Nk, 128) * s.k;
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
   a.d2 = dlam && sizeof(T) == 2 ? a.rowdata + s.rowdata / 4 : nullptr;
+  // both kernels with and without the second product of rest_frag: 4 x 2048 x 2048, 16 heads of 64, causal: +48 and +7 us (registers run
+  // out); 3 x 333 x 1777, 4 heads of 32: +4 and +3 us
+  const bool fine = sizeof(T) == 2 && (D < 64 || (long long)a.B * a.H * a.Nq * a.Nk <= 1 << 24);
+  constexpr bool FINE = sizeof(T) == 2, COARSE = sizeof(T) == 2 && D < 64;     // COARSE: the variant where `fine` is false
   a.bits = (unsigned*)(a.rowdata + (s.rowdata + s.d2) / 4);
   a.bits_b = a.m_b ? (long long)cdiv(a.Nq, 32) * a.Nk : 0;
   a.part = a.rowdata + (s.rowdata + s.d2 + s.bits) / 4;
@@ -1085,14 +1132,18 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   if (a.dk) {
     const long long n = (long long)a.B * a.Nk * a.G * 2 * a.d;
     a.tiles = cdiv(a.Nk, 128), a.splits = s.k;
-    (a.mask ? dkv_kernel<T, D, true> : dkv_kernel<T, D, false>)<<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
+    auto kernel = fine ? (a.mask ? dkv_kernel<T, D, true, FINE> : dkv_kernel<T, D, false, FINE>)
+                       : (a.mask ? dkv_kernel<T, D, true, COARSE> : dkv_kernel<T, D, false, COARSE>);
+    kernel<<<(unsigned)kb, wide_v<T, D> ? 512 : 256, 0, st>>>(a);
     if (s.k > 1) dk = {a.part, (T*)a.dk, n, 2 * n, s.k, sum_grid(n)}, dv = {a.part + n, (T*)a.dv, n, 2 * n, s.k, sum_grid(n)};
   }
   a.part += s.dk / 4;
   if (a.dq || a.d2) {
     const long long n = (long long)a.B * a.Nq * a.H * 2 * a.d;
     a.tiles = cdiv(a.R, 128), a.splits = s.q;
-    (a.mask ? dq_kernel<T, D, true> : dq_kernel<T, D, false>)<<<(unsigned)qb, 256, 0, st>>>(a);
+    auto kernel = fine ? (a.mask ? dq_kernel<T, D, true, FINE> : dq_kernel<T, D, false, FINE>)
+                       : (a.mask ? dq_kernel<T, D, true, COARSE> : dq_kernel<T, D, false, COARSE>);
+    kernel<<<(unsigned)qb, 256, 0, st>>>(a);
     if (s.q > 1 && a.dq) dq = {a.part, (T*)a.dq, n, n, s.q, sum_grid(n)};
   }
   const int blocks = (dlam ? a.H : 0) + dk.blocks + dv.blocks + dq.blocks;
@@ -1119,25 +1170,26 @@ extern "C" int64_t ff3d_diff_attention_workspace_bytes(const ff3d_diff_attention
   return s.splits > 1 ? (long long)s.splits * bg * R * (4 * p->d + 4) * 4 : 0;
 }
 
-extern "C" int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* stat, void* workspace, ff3d_stream_t stream) {
+extern "C" int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* stat, void* out_rest, void* workspace,
+                                       ff3d_stream_t stream) {
   const int s = check(p);
   if (s != FF3D_OK) return s;
-  FF3D_REQUIRE(out && (!out2 == !stat), FF3D_ERR_NULL);
-  FF3D_REQUIRE(ff3d_aligned16(out) && ff3d_aligned16(out2) && ff3d_aligned16(workspace), FF3D_ERR_ALIGNMENT);
+  FF3D_REQUIRE(out && !out2 == !stat && (p->dtype == FF3D_F32 || !out2 == !out_rest), FF3D_ERR_NULL);
+  FF3D_REQUIRE(ff3d_aligned16(out) && ff3d_aligned16(out2) && ff3d_aligned16(out_rest) && ff3d_aligned16(workspace), FF3D_ERR_ALIGNMENT);
   FF3D_REQUIRE(workspace || ff3d_diff_attention_workspace_bytes(p, 0) == 0, FF3D_ERR_NULL);
   ff3d_clear_error();
   Args a = args_of(*p);
-  a.out = (char*)out, a.out2 = out2, a.stat = stat, a.part = (float*)workspace;
+  a.out = (char*)out, a.out2 = out2, a.stat = stat, a.out_rest = (char*)out_rest, a.part = (float*)workspace;
   hipStream_t st = (hipStream_t)stream;
   return p->dtype == FF3D_F32 ? fwd_d<float>(*p, a, st) : p->dtype == FF3D_BF16 ? fwd_d<__bf16>(*p, a, st) : fwd_d<_Float16>(*p, a, st);
 }
 
-extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* stat, const void* dout,
-                                       int64_t dout_batch, int64_t dout_row, void* dq, void* dk, void* dv, void* dlam, void* workspace,
+extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* stat, const void* out_rest,
+                                       const void* dout, int64_t dout_batch, int64_t dout_row, void* dq, void* dk, void* dv, void* dlam, void* workspace,
                                        ff3d_stream_t stream) {
   const int s = check(p);
   if (s != FF3D_OK) return s;
-  FF3D_REQUIRE(out && out2 && stat && dout && workspace && (!dk == !dv), FF3D_ERR_NULL);
+  FF3D_REQUIRE(out && out2 && stat && (p->dtype == FF3D_F32 || out_rest) && dout && workspace && (!dk == !dv), FF3D_ERR_NULL);
   const long long size = p->dtype == FF3D_F32 ? 4 : 2;
   FF3D_REQUIRE(dout_row >= 2ll * p->d * p->heads && dout_batch >= 0 && dout_row * size < (1ll << 24), FF3D_ERR_BAD_SHAPE);
   FF3D_REQUIRE((dout_batch | dout_row) % (16 / size) == 0 && ff3d_aligned16(dout) && ff3d_aligned16(dq) && ff3d_aligned16(dk) && ff3d_aligned16(dv) &&
@@ -1148,6 +1200,7 @@ extern "C" int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const voi
   ff3d_clear_error();
   Args a = args_of(*p);
   a.out = (char*)const_cast<void*>(out), a.out2 = const_cast<float*>(out2), a.stat = const_cast<float*>(stat);
+  a.out_rest = (char*)const_cast<void*>(out_rest);
   a.dout = (const char*)dout, a.do_b = dout_batch, a.do_r = dout_row, a.dq = (char*)dq, a.dk = (char*)dk, a.dv = (char*)dv, a.rowdata = (float*)workspace;
   hipStream_t st = (hipStream_t)stream;
   return p->dtype == FF3D_F32 ? bwd_d<float>(*p, a, dlam, st) : p->dtype == FF3D_BF16 ? bwd_d<__bf16>(*p, a, dlam, st) : bwd_d<_Float16>(*p, a, dlam, st);

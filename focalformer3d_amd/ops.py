@@ -1936,12 +1936,13 @@ def _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, sc
     out = new(shape, dtype=q.dtype, device=dev)
     out2 = new(shape, device=dev) if save else None
     stat = new((B, kv_heads, 4, Nq * heads // kv_heads), device=dev) if save else None
+    rest = new(shape, dtype=q.dtype, device=dev) if save and q.dtype != torch.float32 else None
     if not empty:
         lib = _lib.load()
         n = lib.ff3d_diff_attention_workspace_bytes(p, 0)
         ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.check(lib.ff3d_diff_attention_fwd(p, _ptr(out), _ptr(out2), _ptr(stat), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
-    return out, out2, stat
+        _lib.check(lib.ff3d_diff_attention_fwd(p, _ptr(out), _ptr(out2), _ptr(stat), _ptr(rest), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
+    return out, out2, stat, rest
 
 
 @_on_device_of('q')
@@ -1959,12 +1960,13 @@ def diff_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, 
 
 @_on_device_of('q')
 def diff_attention_train_fwd(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
-    """``diff_attention`` -> (out, out2, stat) with what ``diff_attention_bwd`` needs."""
+    """``diff_attention`` -> (out, out2, stat, rest) with what ``diff_attention_bwd`` needs: the second map's output, the softmax
+    statistics and, in 16 bits, what the rounding of ``out`` left (else None)."""
     return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, True)
 
 
 @_on_device_of('q')
-def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None,
+def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, rest, dout, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None,
                        want=(True, True, True, True)):
     """Gradients of ``diff_attention`` for dout (B, Nq, heads * 2 d) -> (dq, dk, dv, dlam); None where ``want`` is false (dk and dv are
     computed together)."""
@@ -1973,9 +1975,11 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None
     stat_shape = (B, kv_heads, 4, Nq * heads // kv_heads)
     if (out.dtype is not dt or out.shape != q.shape or out2.shape != q.shape or stat.shape != stat_shape
             or not (out2.dtype is stat.dtype is torch.float32) or not (out.get_device() == out2.get_device() == stat.get_device() == q.get_device())
-            or not (out.is_contiguous() and out2.is_contiguous() and stat.is_contiguous())):
-        raise RuntimeError(f'diff_attention_bwd: out, out2, stat: expected what diff_attention_train_fwd gave: contiguous, {dt} and fp32, of '
-                           f'shapes {tuple(q.shape)}, {tuple(q.shape)} and {stat_shape}')
+            or not (out.is_contiguous() and out2.is_contiguous() and stat.is_contiguous())
+            or (dt is not torch.float32 and (rest is None or rest.dtype is not dt or rest.shape != q.shape or rest.get_device() != q.get_device()
+                                             or not rest.is_contiguous()))):
+        raise RuntimeError(f'diff_attention_bwd: out, out2, stat, rest: expected what diff_attention_train_fwd gave: contiguous, {dt} (out, '
+                           f'rest) and fp32 (out2, stat), of shapes {tuple(q.shape)} and {stat_shape} (stat)')
     dout, dop, dob, dor = _attn_rows(dout, 'dout', q, q.shape, per)
     empty = 0 in (B, Nq, Nk)
     new = torch.zeros if empty else torch.empty
@@ -1986,7 +1990,7 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, dout, kv_heads=None
     if not empty and any(want):
         lib = _lib.load()
         ws = torch.empty(lib.ff3d_diff_attention_workspace_bytes(p, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.ff3d_diff_attention_bwd(p, out.data_ptr(), out2.data_ptr(), stat.data_ptr(), dop, dob, dor, _ptr(dq), _ptr(dk),
+        _lib.check(lib.ff3d_diff_attention_bwd(p, out.data_ptr(), out2.data_ptr(), stat.data_ptr(), _ptr(rest), dop, dob, dor, _ptr(dq), _ptr(dk),
                                                _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), 'ff3d_diff_attention_bwd')
     return dq, dk if want[1] else None, dv if want[2] else None, dlam
 

@@ -774,7 +774,8 @@ int ff3d_gated_linear_bwd(const void* x, int64_t ldx, const void* weight, const 
  *   A row that attends no key gives zeros.  Keys and values that are read have to be finite: a NaN or infinity may reach rows that
  *   block its key (as 0 * NaN).
  * ff3d_diff_attention_fwd: out (B, Nq, heads * 2 d) dense; for the backward pass also out2 (the same shape, fp32: the second map's
- *   softmax times v) and stat (B, kv_heads, 4, Nq * heads / kv_heads) fp32 (row maxima in log2 units, 1 / row sums), else both NULL.
+ *   softmax times v), stat (B, kv_heads, 4, Nq * heads / kv_heads) fp32 (row maxima in log2 units, 1 / row sums) and, in 16 bits,
+ *   out_rest (the shape and type of out: what its rounding left; NULL in fp32), else all NULL.
  * ff3d_diff_attention_bwd: dout with its own strides -> dq, (dk, dv) dense in their inputs' shapes, dlam (heads); dq, the pair and
  *   dlam may be NULL.  Deterministic.  workspace: ff3d_diff_attention_workspace_bytes(p, backward), 16-byte aligned scratch. */
 typedef struct {
@@ -789,11 +790,11 @@ typedef struct {
   float scale;
 } ff3d_diff_attention_t;
 int64_t ff3d_diff_attention_workspace_bytes(const ff3d_diff_attention_t* p, int backward);
-int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* stat, void* workspace,
-                            ff3d_stream_t stream);
-int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* stat, const void* dout,
-                            int64_t dout_batch, int64_t dout_row, void* dq, void* dk, void* dv, void* dlam, void* workspace,
-                            ff3d_stream_t stream);
+int ff3d_diff_attention_fwd(const ff3d_diff_attention_t* p, void* out, float* out2, float* stat, void* out_rest,
+                            void* workspace, ff3d_stream_t stream);
+int ff3d_diff_attention_bwd(const ff3d_diff_attention_t* p, const void* out, const float* out2, const float* stat,
+                            const void* out_rest, const void* dout, int64_t dout_batch, int64_t dout_row, void* dq, void* dk,
+                            void* dv, void* dlam, void* workspace, ff3d_stream_t stream);
 
 /* Norm over all elements of n tensors and clipping by it (ABI 2.12):
  *   norm = (sum |g|^2)^(1/2) (kind 2), sum |g| (kind 1) or max |g| (kind 0), sums in fp64, result fp32 on the device;

@@ -69,12 +69,12 @@ def test_diff_attention_entry_checks_its_arguments():
     ok = dict(q=P, k=P, v=P, lam=P, mask=None, kv_lens=None, q_batch=320, q_row=64, k_batch=320, k_row=64, v_batch=320, v_row=64, mask_batch=0, mask_row=0,
               B=2, Nq=5, Nk=5, heads=2, kv_heads=2, d=16, causal=0, dtype=0, scale=0.25)
 
-    def run(out=P, out2=None, lse=None, ws=None, **k):
-        return lib.ff3d_diff_attention_fwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, ws, None)
-    assert lib.ff3d_diff_attention_fwd(None, P, None, None, None, None) == -4
+    def run(out=P, out2=None, lse=None, rest=None, ws=None, **k):
+        return lib.ff3d_diff_attention_fwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, rest, ws, None)
+    assert lib.ff3d_diff_attention_fwd(None, P, None, None, None, None, None) == -4
     for n in ('q', 'k', 'v', 'lam', 'out'):
         assert run(**{n: None}) == -4, n
-    assert run(out2=P) == -4 and run(lse=P) == -4
+    assert run(out2=P) == -4 and run(lse=P) == -4 and run(out2=P, lse=P, dtype=1) == -4 and run(rest=P, dtype=1) == -4
     assert run(dtype=2) == -2 and run(d=24) == -5
     for bad in (dict(B=0), dict(Nq=0), dict(Nk=-1), dict(heads=3), dict(kv_heads=0), dict(scale=0.0), dict(scale=float('nan')), dict(q_row=60), dict(k_row=32),
                 dict(q_batch=-320), dict(mask_row=-1), dict(Nk=1 << 30), dict(q_row=1 << 22)):
@@ -88,10 +88,11 @@ def test_diff_attention_entry_checks_its_arguments():
     assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 0) == 0
     assert lib.ff3d_diff_attention_workspace_bytes(_lib.DiffAttention(**ok), 1) == 4 * (6 + 1) * 64 * 4  # rows rounded up to 64
 
-    def bwd(out=P, out2=P, lse=P, dout=P, db=320, dr=64, dq=P, dk=P, dv=P, dlam=P, ws=P, **k):
-        return lib.ff3d_diff_attention_bwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, dout, db, dr, dq, dk, dv, dlam, ws, None)
+    def bwd(out=P, out2=P, lse=P, rest=None, dout=P, db=320, dr=64, dq=P, dk=P, dv=P, dlam=P, ws=P, **k):
+        return lib.ff3d_diff_attention_bwd(_lib.DiffAttention(**{**ok, **k}), out, out2, lse, rest, dout, db, dr, dq, dk, dv, dlam, ws, None)
     for n in ('out', 'out2', 'lse', 'dout', 'ws', 'dk', 'dv'):
         assert bwd(**{n: None}) == -4, n
+    assert bwd(dtype=1) == -4
     assert bwd(dr=32) == -1 and bwd(dr=66) == -3 and bwd(dq=P + 4) == -3
 
 
