@@ -5,10 +5,11 @@
 //          first pieces, which travel as kernel arguments: no table in memory, so a call can be captured and costs no copy) and
 //          leaves one partial result.  Squares are summed in fp64: the square of any fp32 is exact and cannot overflow there, and
 //          the units are idle in a kernel that waits for memory.
-//   scale  every block adds all partial results again, in the same order (at most 1024 + one per tensor: 2 us, hidden behind the
-//          other blocks' loads), so there is no third launch and no counter to reset; then scales its piece.  Pieces are taken in
+//   scale  every block adds all partial results again, in the same order (at most 1024 + one per tensor, a few KB that the caches hold), so there is no third launch and no counter to reset; then scales its piece.  Pieces are taken in
 //          the opposite order: the end of the first pass is what the caches still hold.
 // Bound by memory: 4 N read, 4 N read again (from the 256 MB cache where the gradients fit it), 4 N written in fp32.
+// 88 million fp32 elements: norm 94 us (3.75 TB/s), scale 132 us (5.3 TB/s of both directions); 2.6 million in 35 tensors: 5.2
+// and 7.4 us.
 #include <algorithm>
 #include <new>
 

@@ -773,6 +773,7 @@ int ff3d_gated_linear_bwd(const void* x, int64_t ldx, const void* weight, const 
  *   causal: query i attends keys j <= i + Nk - Nq.
  *   A row that attends no key gives zeros.  Keys and values that are read have to be finite: a NaN or infinity may reach rows that
  *   block its key (as 0 * NaN).
+ *   fp32 operands are split into three bf16 planes (six products, as exact as fp32 ones): an infinite operand gives NaN.
  * ff3d_diff_attention_fwd: out (B, Nq, heads * 2 d) dense; for the backward pass also out2 (the same shape, fp32: the second map's
  *   softmax times v), stat (B, kv_heads, 4, Nq * heads / kv_heads) fp32 (row maxima in log2 units, 1 / row sums) and, in 16 bits,
  *   out_rest (the shape and type of out: what its rounding left; NULL in fp32), else all NULL.
