@@ -735,7 +735,7 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
 int check(const void* x, const void* w, const void* h, int64_t ldx, int64_t ldh, int M, int C, int F, int act, int dtype, int pack, const void* ws, int64_t need) {
   FF3D_REQUIRE(x && w && h, FF3D_ERR_NULL);
   FF3D_REQUIRE(dtype == FF3D_F32 || dtype == FF3D_BF16 || dtype == FF3D_F16, FF3D_ERR_BAD_DTYPE);
-  FF3D_REQUIRE(M > 0 && C > 0 && F > 0 && ldx >= C && ldh >= F && act >= 0 && act <= 3 && (pack & ~3) == 0, FF3D_ERR_BAD_SHAPE);
+  FF3D_REQUIRE(M > 0 && M < 0x7fffff00 && C > 0 && F > 0 && ldx >= C && ldh >= F && act >= 0 && act <= 3 && (pack & ~3) == 0, FF3D_ERR_BAD_SHAPE);
   const long long size = dtype == FF3D_F32 ? 4 : 2, per = 16 / size;
   // byte offsets inside a block's rows and inside the weight are 31 bits
   FF3D_REQUIRE(2ll * F * align_up(C, per) * size < 0x7fffffffll && align_up(2ll * F, per) * 256 * size < 0x7fffffffll && ldx * 256 * size < 0x7fffffffll,

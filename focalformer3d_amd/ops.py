@@ -1815,7 +1815,9 @@ def _gated_args(x, weight, bias, act):
         _same(bias, x, 'bias', (F2,))
         bias = bias.contiguous()
     x2 = x if x.dim() == 2 else x.reshape(-1, C_)
-    if x2.stride(1) != 1 or x2.stride(0) < C_:
+    if x2.shape[0] >= 0x7fffff00:
+        raise RuntimeError(f'gated_linear: {x2.shape[0]} rows: fewer than {0x7fffff00} in a call')
+    if x2.stride(1) != 1 or x2.stride(0) < C_ or x2.stride(0) >= 1 << 20:          # (the kernels' offsets inside a tile are 31 bits)
         x2 = x2.contiguous()
     weight = weight.contiguous()
     per = 4 if code == 0 else 8

@@ -373,7 +373,7 @@ class DifferentialAttention(nn.Module):
             self.__dict__.pop(name, None)
 
     def _project(self, x, linear):
-        if x.dtype != torch.float32 or torch.is_grad_enabled() or not x.is_contiguous():
+        if x.dtype != torch.float32 or torch.is_grad_enabled() or not x.is_contiguous() or x.numel() == 0:
             return F.linear(x, linear.weight, linear.bias)
         return _lin(self, x, linear.weight, linear.bias)
 
@@ -395,7 +395,7 @@ class DifferentialAttention(nn.Module):
         q = self._project(xp, self.q_proj)                 # (under autocast the projections' type is not the parameters')
         o = differential_attention(q, self._project(xp, self.k_proj), self._project(x, self.v_proj), self.lam().to(q.dtype), self.num_heads,
                                    kv_heads=self.kv_heads, mask=mask)
-        heads = o.view(B, N, self.num_heads, -1)
+        heads = o.view(B, N, self.num_heads, C // self.num_heads)
         o = F.rms_norm(heads, heads.shape[-1:], self.head_norm.to(o.dtype), self.eps) * (1.0 - self.lambda_init)
         out = self._project(o.reshape(B, N, C), self.out_proj)
         return x + self.dropout_layer(self.proj_drop(out))
@@ -733,7 +733,7 @@ class GatedFFN(nn.Module):
         w, b = self.in_proj.weight, self.in_proj.bias
         if torch.is_grad_enabled():
             from .autograd import gated_linear
-            return gated_linear(x, w, b, self.act), self.out_proj
+            return gated_linear(x, w.to(x.dtype), b.to(x.dtype), self.act), self.out_proj       # (their types differ under autocast)
         if x.dtype == torch.float32 and getattr(self, 'gemm_dtype', torch.float32) == torch.bfloat16:
             # bf16 mode: operands on the bf16 matrix cores, fp32 rows out
             w16, b16 = _cached(self, '_bf16_w', w, b, lambda: (w.detach().to(torch.bfloat16), b.detach().to(torch.bfloat16)))
@@ -742,7 +742,8 @@ class GatedFFN(nn.Module):
 
     def delta(self, x):
         y, last = self.hidden(x)
-        return _lin(self, y, last.weight, last.bias) if y.dtype == torch.float32 else F.linear(y, last.weight, last.bias)
+        own = y.dtype == torch.float32 and y.numel() > 0
+        return _lin(self, y, last.weight, last.bias) if own else F.linear(y, last.weight, last.bias)
 
     def fused_add_ln(self, x, norm, pos=None):
         """There is no one-launch form: the caller runs the projection and the fused add + LayerNorm."""

@@ -124,16 +124,34 @@ def test_gated_ffn_module(act):
         close(m(x), plain_gated(m, P, xd), 4 * 2.0 ** -8, 'bf16 mode, new weights')
 
 
+def test_modules_without_queries():
+    m, ffn, x = attention_module(64, 4, 2, 5), None, torch.zeros(2, 0, 64, device='cuda', requires_grad=True)
+    from focalformer3d_amd.transformer import GatedFFN
+    ffn = GatedFFN(64, 96).cuda()
+    y = ffn(m(x, query_pos=x))
+    assert y.shape == x.shape
+    y.sum().backward()
+    assert all(float(p.grad.abs().sum()) == 0.0 for p in [*ffn.in_proj.parameters()])
+    with torch.no_grad():
+        assert ffn.eval()(m.eval()(x)).shape == x.shape
+
+
 def test_modules_under_autocast():
     """Activations in bf16, parameters in fp32: the operators run in the activations' type.  Roundings of 2^-8 at 6 places, enlarged 9 times
     by the difference of the maps."""
+    from focalformer3d_amd.transformer import GatedFFN
     m = attention_module(64, 4, 2, 5).train()
     x = torch.randn(2, 20, 64, device='cuda', requires_grad=True)
     want = plain_attention(m, doubles(m), x.detach().double(), None, None)
     with torch.autocast('cuda', torch.bfloat16):
         got = m(x)
     close(got.float(), want, 6 * 9 * 2.0 ** -8, 'autocast')
-    got.float().square().sum().backward()
+    ffn = GatedFFN(64, 96).cuda()
+    with torch.autocast('cuda', torch.bfloat16):
+        y = ffn(x.bfloat16())                                     # straight behind a projection
+    close(y.float(), plain_gated(ffn, doubles(ffn), x.detach().bfloat16().double()), 4 * 2.0 ** -8, 'autocast, bf16 input')
+    (y.float().square().sum() + got.float().square().sum()).backward()
+    assert all(bool(torch.isfinite(p.grad).all()) and p.grad.dtype == torch.float32 for p in ffn.parameters())
     assert all(bool(torch.isfinite(p.grad).all()) and p.grad.dtype == torch.float32 for p in m.parameters())
 
 
@@ -205,3 +223,73 @@ def test_training_step_with_clipped_gradients():
     values = [p.detach().clone() for p in params]
     torch.optim.SGD(params, lr=0.5).step()
     assert sum(not torch.equal(p, v) for p, v in zip(params, values)) > len(params) // 2
+
+
+def test_head_with_both_modules_replays():
+    """The captured head against eager launches, over inputs that change between the replays, with eager work and synchronisation between."""
+    from focalformer3d_amd.runtime import GraphedHead
+    from focalformer3d_amd.synthetic import stage_features
+    head = _head(False).eval()
+    first = stage_features(1, 128, 180, 3, seed=1, device='cuda')
+    graphed = GraphedHead(head, first)
+    for seed in (2, 3, 4):
+        inputs = stage_features(1, 128, 180, 3, seed=seed, device='cuda')
+        with torch.no_grad():
+            want = [t.clone() for t in head.get_bboxes_padded(head(inputs, None, None), max_out=200)]
+        torch.cuda.synchronize()
+        for _ in range(2):
+            got = graphed(inputs)
+            graphed.wait()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_bf16_mode_of_the_decoder():
+    """set_gemm_dtype(torch.bfloat16) reaches both modules: finite results near the fp32 ones.  Projections round operands to bf16 (2^-8) at 6
+    places per layer, 6 layers, enlarged at most 9 times by the difference of the maps and scaled by 0.2."""
+    from focalformer3d_amd.synthetic import stage_features
+    head = _head(False).eval()
+    inputs = stage_features(1, 128, 180, 3, seed=1, device='cuda')
+    with torch.no_grad():
+        a = head(inputs, None, [{}])[0][0]['center'].clone()
+        head.set_gemm_dtype(torch.bfloat16)
+        b = head(inputs, None, [{}])[0][0]['center']
+    assert bool(torch.isfinite(b).all()) and float((a - b).norm() / a.norm()) <= 36 * 9 * 0.2 * 2.0 ** -8
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16])
+def test_captured_training_chain(dtype):
+    """Attention, gated projection, their gradients and the clipping in one captured graph, replayed over changing inputs with eager work
+    between, each replay against the eager chain.  (No eager graph of the leaves is alive during the capture.)"""
+    from focalformer3d_amd import ops
+    from focalformer3d_amd.autograd import differential_attention, gated_linear
+    torch.manual_seed(9)
+    r = lambda *s: torch.randn(*s, device='cuda').to(dtype)  # noqa: E731
+    leaves = [r(2, 50, 128), r(2, 70, 64), r(2, 70, 64), r(4), r(2 * 96, 128) * 0.1, r(2 * 96)]
+    dout, mask = r(2, 50, 96), torch.rand(2, 50, 70, device='cuda') < 0.3
+    static = [t.clone().requires_grad_(True) for t in leaves]
+
+    def chain(q, k, v, lam, w, b):
+        y = differential_attention(q, k, v, lam, 4, kv_heads=2, mask=mask)
+        h = gated_linear(y, w, b, 'silu')
+        grads = [g.contiguous() for g in torch.autograd.grad(h, (q, k, v, lam, w, b), dout)]
+        return [h.detach(), ops.clip_grads(grads, 0.5), *grads]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        chain(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = chain(*static)
+    for step in range(4):
+        new = [r(*t.shape) * (0.1 if t.dim() == 2 else 1.0) for t in leaves]
+        with torch.no_grad():
+            for s, n in zip(static, new):
+                s.copy_(n)
+        graph.replay()
+        want = chain(*[n.clone().requires_grad_(True) for n in new])
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b), step

@@ -42,7 +42,7 @@ def test_c_entries_check_their_arguments():
     run = lambda **k: f(*{**ok, **k}.values(), None)  # noqa: E731
     assert run(x=None) == -4 and run(w=None) == -4 and run(h=None) == -4
     assert run(dt=2) == -2 and run(dt=7) == -2
-    for bad in (dict(M=0), dict(C=0), dict(F=-1), dict(ldx=15), dict(act=4), dict(pack=4), dict(C=1 << 20, F=1 << 20, ldx=1 << 20)):
+    for bad in (dict(M=0), dict(M=0x7fffff00), dict(C=0), dict(F=-1), dict(ldx=15), dict(act=4), dict(pack=4), dict(C=1 << 20, F=1 << 20, ldx=1 << 20)):
         assert run(**bad) == -1, bad
     assert run(ldx=17) == -3 and run(x=ctypes.c_void_p(4100)) == -3 and run(w=ctypes.c_void_p(4104)) == -3
     assert run(C=15) == -3 and run(C=15, pack=1) == -3
