@@ -17,6 +17,7 @@ over the flattened BEV pyramid (FD:927-933 under autograd: M = frames x 42 525 r
 The training-mode forward that uses them is focalformer3d_amd/train_forward.py; the inference modules do not route through
 autograd.
 """
+import functools
 import os
 import weakref
 
@@ -171,23 +172,31 @@ class MaskedSelfAttentionFunction(Function):
         return gq, gk, gv, None, None, None
 
 
+def _once(backward):
+    """``once_differentiable`` without its cost where no graph of the gradients is built."""
+    checked = once_differentiable(backward)
+
+    @functools.wraps(backward)
+    def call(ctx, *grads):
+        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+    return call
+
+
 class DifferentialAttentionFunction(Function):
     """softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v per head (ops.diff_attention_train_fwd / _bwd)."""
 
     @staticmethod
     def forward(ctx, q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale):
-        out, out2, stat, rest = ops.diff_attention_train_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
-        ctx.save_for_backward(q, k, v, lam, out, out2, stat, rest, mask, kv_lens)
-        ctx.meta = heads, kv_heads, causal, scale
-        return out
+        results, keep, ctx.dims = ops.diff_attention_train_keep(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+        ctx.save_for_backward(*keep, *results)
+        return results[0]
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
-        q, k, v, lam, out, out2, stat, rest, mask, kv_lens = ctx.saved_tensors
-        heads, kv_heads, causal, scale = ctx.meta
-        grads = ops.diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, rest, dout, kv_heads, mask, kv_lens, causal, scale, ctx.needs_input_grad[:4])
-        return (*grads, None, None, None, None, None, None)
+        saved = ctx.saved_tensors
+        p, keep = ops._diff_attention_again(saved[:6], ctx.dims)
+        return (*ops._diff_attention_grads(p, keep, ctx.dims, *saved[6:], dout, ctx.needs_input_grad[:4]), None, None, None, None, None, None)
 
 
 def differential_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
@@ -208,7 +217,7 @@ class GatedLinearFunction(Function):
         return ops.gated_linear(x, weight, bias, act)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dh):
         x, weight, bias = ctx.saved_tensors
         return (*ops.gated_linear_bwd(x, weight, bias, ctx.act, dh, ctx.needs_input_grad[:3]), None)

@@ -1798,6 +1798,13 @@ def _ptr(t):
     return C.c_void_p(0 if t is None else t.data_ptr())
 
 
+def _new_like(t, zero=False):
+    """An uninitialised (or zeroed) contiguous tensor of t's shape, type and device (empty_like takes a third of the time of empty)."""
+    if t.is_contiguous():
+        return torch.zeros_like(t) if zero else torch.empty_like(t)
+    return (torch.zeros if zero else torch.empty)(t.shape, dtype=t.dtype, device=t.device)
+
+
 def _gated_args(x, weight, bias, act):
     """Checked operands -> (x as rows, weight, bias, F, C, which operands have to be packed, dtype code, activation code)."""
     code, acode = _DTYPE.get(x.dtype), _ACTS.get(act)
@@ -1853,10 +1860,9 @@ def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     M = x2.shape[0]
     _same(dh, x, 'dh', (*x.shape[:-1], F_))
     want_b = want[2] and bias is not None
-    new = torch.zeros if M == 0 else torch.empty
-    dx = new(x.shape, dtype=x.dtype, device=x.device) if want[0] else None
-    dw = new(2 * F_, C_, dtype=x.dtype, device=x.device) if want[1] else None
-    db = new(2 * F_, dtype=x.dtype, device=x.device) if want_b else None
+    dx = _new_like(x, M == 0) if want[0] else None
+    dw = _new_like(weight, M == 0) if want[1] else None
+    db = _new_like(bias, M == 0) if want_b else None
     if M == 0 or not (want[0] or want[1] or want_b):
         return dx, dw, db
     dh2 = dh.reshape(-1, F_)
@@ -1887,7 +1893,7 @@ _DIFF_ATTENTION = struct.Struct('6Q8q8if4x')            # the fields of _lib.Dif
 
 
 def _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale):
-    """Checked arguments -> (struct, the tensors it points to, heads * 2 d and the other sizes)."""
+    """Checked arguments -> (struct, the tensors it points to, (B, Nq, Nk, heads, kv_heads, d, causal, dtype code, scale))."""
     code = _DTYPE.get(q.dtype)
     if code is None:
         raise RuntimeError(f'diff_attention: expected fp32, bf16 or fp16 tensors, got {q.dtype}')
@@ -1925,26 +1931,61 @@ def _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, s
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float('inf'):
         raise ValueError(f'diff_attention: scale {scale}: expected a positive number')
-    p = _lib.DiffAttention.from_buffer_copy(_DIFF_ATTENTION.pack(qp, kp, vp, lam.data_ptr(), mp, lp, qb, qr, kb, kr, vb, vr, mb, mr,
-                                                                 B, Nq, Nk, heads, kv_heads, d, 1 if causal else 0, code, scale))
-    return p, (q, k, v, lam, mask, kv_lens), (B, Nq, Nk, kv_heads, per)
+    dims = B, Nq, Nk, heads, kv_heads, d, 1 if causal else 0, code, scale
+    p = _lib.DiffAttention.from_buffer_copy(_DIFF_ATTENTION.pack(qp, kp, vp, lam.data_ptr(), mp, lp, qb, qr, kb, kr, vb, vr, mb, mr, *dims))
+    return p, (q, k, v, lam, mask, kv_lens), dims
+
+
+def _diff_attention_again(keep, dims):
+    """The struct of checked arguments that autograd kept (addresses and strides are asked for again: a hook may have moved them)."""
+    q, k, v, lam, mask, kv_lens = keep
+    (qb, qr, qc), (kb, kr, kc), (vb, vr, vc) = q.stride(), k.stride(), v.stride()
+    mb, mr, mc = (0, 0, 1) if mask is None else mask.stride()
+    if not qc == kc == vc == 1 or (mc != 1 and dims[2] > 1):
+        return _diff_attention_args(q, k, v, lam, dims[3], dims[4], mask, kv_lens, dims[6], dims[8])[:2]
+    mp, mb = (0, 0) if mask is None else (mask.data_ptr(), mb if mask.shape[0] > 1 else 0)
+    return _lib.DiffAttention.from_buffer_copy(_DIFF_ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), lam.data_ptr(), mp, 0 if kv_lens is None else kv_lens.data_ptr(), qb, qr, kb, kr, vb, vr, mb, mr,
+        *dims)), keep
 
 
 def _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, save):
-    p, keep, (B, Nq, Nk, kv_heads, _) = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
-    dev, shape = q.device, q.shape
+    """-> (out, out2, stat, rest), the checked arguments, their sizes."""
+    p, keep, dims = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    B, Nq, Nk, heads, kv_heads = dims[:5]
+    q = keep[0]
     empty = 0 in (B, Nq, Nk)
-    new = torch.zeros if empty else torch.empty
-    out = new(shape, dtype=q.dtype, device=dev)
-    out2 = new(shape, device=dev) if save else None
-    stat = new((B, kv_heads, 4, Nq * heads // kv_heads), device=dev) if save else None
-    rest = new(shape, dtype=q.dtype, device=dev) if save and q.dtype != torch.float32 else None
+    out = _new_like(q, empty)
+    out2 = stat = rest = None
+    if save:
+        new = torch.zeros if empty else torch.empty
+        out2 = new(q.shape, device=q.device)
+        stat = new((B, kv_heads, 4, Nq * heads // kv_heads), device=q.device)
+        if q.dtype is not torch.float32:
+            rest = _new_like(out, empty)
     if not empty:
         lib = _lib.load()
         n = lib.ff3d_diff_attention_workspace_bytes(p, 0)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.check(lib.ff3d_diff_attention_fwd(p, _ptr(out), _ptr(out2), _ptr(stat), _ptr(rest), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
-    return out, out2, stat, rest
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _lib.check(lib.ff3d_diff_attention_fwd(p, out.data_ptr(), _ptr(out2), _ptr(stat), _ptr(rest), _ptr(ws), _stream()), 'ff3d_diff_attention_fwd')
+    return (out, out2, stat, rest), keep, dims
+
+
+def _diff_attention_grads(p, keep, dims, out, out2, stat, rest, dout, want):
+    """Gradients from checked arguments and what the forward pass gave; dout is checked here."""
+    q, k, v, lam = keep[:4]
+    B, Nq, Nk = dims[:3]
+    dout, dop, dob, dor = _attn_rows(dout, 'dout', q, q.shape, 4 if dims[7] == 0 else 8)
+    empty = 0 in (B, Nq, Nk)
+    dq = _new_like(q, empty) if want[0] else None
+    dk, dv = (_new_like(k, empty), _new_like(v, empty)) if want[1] or want[2] else (None, None)
+    dlam = _new_like(lam, empty) if want[3] else None
+    if not empty and any(want):
+        lib = _lib.load()
+        ws = torch.empty(lib.ff3d_diff_attention_workspace_bytes(p, 1), dtype=torch.uint8, device=q.device)
+        _lib.check(lib.ff3d_diff_attention_bwd(p, out.data_ptr(), out2.data_ptr(), stat.data_ptr(), _ptr(rest), dop, dob, dor, _ptr(dq), _ptr(dk),
+                                               _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), 'ff3d_diff_attention_bwd')
+    return dq, dk if want[1] else None, dv if want[2] else None, dlam
 
 
 @_on_device_of('q')
@@ -1957,13 +1998,19 @@ def diff_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, 
     mask (Nq, Nk) or (B, Nq, Nk) bool / uint8, True = not attended; kv_lens (B,) int32 on the device: keys from there on are absent and
     not read; causal: query i attends keys j <= i + Nk - Nq.  A row without keys gives zeros.  scale: d ** -0.5 by default.
     Keys and values that are read have to be finite.  The differentiable form is ``autograd.differential_attention``."""
-    return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, False)[0]
+    return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, False)[0][0]
 
 
 @_on_device_of('q')
 def diff_attention_train_fwd(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
     """``diff_attention`` -> (out, out2, stat, rest) with what ``diff_attention_bwd`` needs: the second map's output, the softmax
     statistics and, in 16 bits, what the rounding of ``out`` left (else None)."""
+    return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, True)[0]
+
+
+@_on_device_of('q')
+def diff_attention_train_keep(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
+    """``diff_attention_train_fwd`` -> (its results, the operands as the kernels read them, sizes): what autograd keeps."""
     return _diff_attention_fwd(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale, True)
 
 
@@ -1972,29 +2019,14 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, rest, dout, kv_head
                        want=(True, True, True, True)):
     """Gradients of ``diff_attention`` for dout (B, Nq, heads * 2 d) -> (dq, dk, dv, dlam); None where ``want`` is false (dk and dv are
     computed together)."""
-    p, keep, (B, Nq, Nk, kv_heads, per) = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
-    dev, dt = q.device, q.dtype
-    stat_shape = (B, kv_heads, 4, Nq * heads // kv_heads)
-    if (out.dtype is not dt or out.shape != q.shape or out2.shape != q.shape or stat.shape != stat_shape
-            or not (out2.dtype is stat.dtype is torch.float32) or not (out.get_device() == out2.get_device() == stat.get_device() == q.get_device())
-            or not (out.is_contiguous() and out2.is_contiguous() and stat.is_contiguous())
-            or (dt is not torch.float32 and (rest is None or rest.dtype is not dt or rest.shape != q.shape or rest.get_device() != q.get_device()
-                                             or not rest.is_contiguous()))):
-        raise RuntimeError(f'diff_attention_bwd: out, out2, stat, rest: expected what diff_attention_train_fwd gave: contiguous, {dt} (out, '
-                           f'rest) and fp32 (out2, stat), of shapes {tuple(q.shape)} and {stat_shape} (stat)')
-    dout, dop, dob, dor = _attn_rows(dout, 'dout', q, q.shape, per)
-    empty = 0 in (B, Nq, Nk)
-    new = torch.zeros if empty else torch.empty
-    pair = want[1] or want[2]
-    dq = new(q.shape, dtype=dt, device=dev) if want[0] else None
-    dk, dv = (new(k.shape, dtype=dt, device=dev), new(v.shape, dtype=dt, device=dev)) if pair else (None, None)
-    dlam = new(heads, dtype=dt, device=dev) if want[3] else None
-    if not empty and any(want):
-        lib = _lib.load()
-        ws = torch.empty(lib.ff3d_diff_attention_workspace_bytes(p, 1), dtype=torch.uint8, device=dev)
-        _lib.check(lib.ff3d_diff_attention_bwd(p, out.data_ptr(), out2.data_ptr(), stat.data_ptr(), _ptr(rest), dop, dob, dor, _ptr(dq), _ptr(dk),
-                                               _ptr(dv), _ptr(dlam), _ptr(ws), _stream()), 'ff3d_diff_attention_bwd')
-    return dq, dk if want[1] else None, dv if want[2] else None, dlam
+    p, keep, dims = _diff_attention_args(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
+    dt, stat_shape = q.dtype, (dims[0], dims[4], 4, dims[1] * heads // dims[4])
+    kept = [('out', out, dt, q.shape), ('out2', out2, torch.float32, q.shape), ('stat', stat, torch.float32, stat_shape)]
+    for name, t, dtype, shape in kept + ([('rest', rest, dt, q.shape)] if dt is not torch.float32 else []):
+        if (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape or t.get_device() != q.get_device()
+                or not t.is_contiguous()):
+            raise RuntimeError(f'diff_attention_bwd: {name}: expected what diff_attention_train_fwd gave: contiguous, {dtype}, {tuple(shape)}')
+    return _diff_attention_grads(p, keep, dims, out, out2, stat, rest, dout, want)
 
 
 _NORM_KINDS = {2: 2, 1: 1, float('inf'): 0}
