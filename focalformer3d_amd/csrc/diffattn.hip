@@ -96,7 +96,8 @@ __device__ __forceinline__ vec8<T> scaled_frag(const f32x16& c, int step, float 
 
 // What scaled_frag's rounding left, for a second product.  dS = P (dP - D) sums to nothing over the keys, so what remains of dS K is small
 // against its terms, and rounding those once gives dq 1.5 to 2.1 times, dk 1.4 to 2.3 times the error of rounding the result alone (8 or
-// 16 columns per map, or few keys).  With the second product it is 1.0 to 1.2 times.  It is left out (FINE false) where the products are
+// 16 columns per map, or few keys).  With the second product it is 1.0 to 1.2 times.  dv is treated alike (1.4 times, and more where few
+// weights serve many columns).  It is left out (FINE false) where the products are
 // the bound and the sums are long: 64 columns and more than 2^24 pairs, 1.4 to 1.5 times.
 template <typename T>
 __device__ __forceinline__ vec8<T> rest_frag(const f32x16& c, int step, float mul, const vec8<T>& v) {
@@ -878,13 +879,19 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
       sv.template see<VT>(top[0], dv);
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
-        const Op<T> f = op<T>(scaled_frag<T>(w, st, sv.mul()));
+        const vec8<T> wv = scaled_frag<T>(w, st, sv.mul());
+        const Op<T> f = op<T>(wv);
         vec8<T> x[VT];
 #pragma unroll
         for (int t = 0; t < VT; ++t) x[t] = col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, t * 32, lane);
         if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), f, dv[t]);
+        if constexpr (FINE) {
+          const Op<T> rest = op<T>(rest_frag<T>(w, st, sv.mul(), wv));
+#pragma unroll
+          for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), rest, dv[t]);
+        }
       }
       sk[0].template see<QT>(top[1], dk[0]);
       sk[1].template see<QT>(top[2], dk[1]);
@@ -1127,6 +1134,7 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   a.d2 = dlam && sizeof(T) == 2 ? a.rowdata + s.rowdata / 4 : nullptr;
   // both kernels with and without the second product of rest_frag: 1 x 4096, 16 heads over 4 of 64, causal: +48 and +7 us (registers run
   // out); 3 x 333 x 1777, 4 heads of 32: +4 and +3 us
+  if (a.Nk == 1) a.scale = 0.f;    // the weight of a single key is 1 whatever its score: dq and dk are zero, not the rounding of dP - D
   const bool fine = sizeof(T) == 2 && (D < 64 || (long long)a.B * a.H * a.Nq * a.Nk <= 1 << 24);
   constexpr bool FINE = sizeof(T) == 2, COARSE = sizeof(T) == 2 && D < 64;     // COARSE: the variant where `fine` is false
   a.bits = (unsigned*)(a.rowdata + (s.rowdata + s.d2) / 4);

@@ -162,6 +162,17 @@ def test_diff_attention_wanted_gradients_only():
         assert all((t is None) == (j != i) for j, t in enumerate(got)) and torch.equal(got[i], full[i])
 
 
+@pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('Nq,H,G,d', [(1, 12, 12, 16), (5, 4, 2, 64), (40, 2, 1, 32)])
+def test_diff_attention_one_key(dtype, Nq, H, G, d):
+    """Its weight is 1 whatever the score: no gradient reaches q and k, and out = (1 - lam) v."""
+    got = _check(*_inputs(3, Nq, 1, H, G, d, DT[dtype], 33), H, G)
+    assert float(got[1].abs().max()) == 0.0 and float(got[2].abs().max()) == 0.0
+    lens = torch.tensor([1, 0, 1], dtype=torch.int32, device='cuda')
+    got = _check(*_inputs(3, Nq, 1, H, G, d, DT[dtype], 34), H, G, kv_lens=lens)
+    assert float(got[1].abs().max()) == 0.0 and float(got[2].abs().max()) == 0.0 and float(got[0].detach()[1].abs().max()) == 0.0
+
+
 def test_diff_attention_empty():
     from focalformer3d_amd import ops
     q, k, v, lam, dout = _inputs(2, 5, 6, 2, 2, 16, torch.float32, 12)
