@@ -508,30 +508,49 @@ __global__ __launch_bounds__(NW * 64) void gated_rows_kernel(GemmArgs p) {
   });
 }
 
-// out[i] = sum of the slices in order, W elements per thread (n a multiple of W)
+// out[i] = sum of the slices part[k n + i] in order
+template <typename T>
+struct SumJob {
+  const float* part;
+  T* out;
+  long long n;
+  int slices, blocks, wide;       // wide: four elements per thread
+};
 template <typename T, int W>
-__global__ __launch_bounds__(256) void sum_slices_kernel(const float* parts, T* out, int slices, long long n) {
+__device__ __forceinline__ void sum_slices(const SumJob<T>& j, int block) {
   struct alignas(4 * W) In { float v[W]; };
   struct alignas(W * sizeof(T)) Out { T v[W]; };
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n / W; i += (long long)gridDim.x * 256) {
+  for (long long i = (long long)block * 256 + threadIdx.x; i < j.n / W; i += (long long)j.blocks * 256) {
     float s[W] = {};
 #pragma unroll 8
-    for (int k = 0; k < slices; ++k) {
-      const In v = ((const In*)(parts + k * n))[i];
+    for (int k = 0; k < j.slices; ++k) {
+      const In v = ((const In*)(j.part + k * j.n))[i];
 #pragma unroll
       for (int e = 0; e < W; ++e) s[e] += v.v[e];
     }
     Out o;
 #pragma unroll
     for (int e = 0; e < W; ++e) o.v[e] = from_f<T>(s[e]);
-    ((Out*)out)[i] = o;
+    ((Out*)j.out)[i] = o;
   }
 }
+// the slices of dx, of dW and the column sums of d, in one launch behind the products
 template <typename T>
-void sum_slices(const float* parts, T* out, int slices, long long n, hipStream_t st) {
-  const unsigned grid = (unsigned)(n / 1024 + 1 < 4096 ? n / 1024 + 1 : 4096);
-  if (n % 4 == 0 && ff3d_aligned16(out)) sum_slices_kernel<T, 4><<<grid, 256, 0, st>>>(parts, out, slices, n);
-  else sum_slices_kernel<T, 1><<<grid, 256, 0, st>>>(parts, out, slices, n);
+__global__ __launch_bounds__(256) void sum_kernel(SumJob<T> j0, SumJob<T> j1, SumJob<T> j2) {
+  int at = blockIdx.x;
+  SumJob<T> j = j0;
+  if (at >= j.blocks) {
+    at -= j.blocks, j = j1;
+    if (at >= j.blocks) at -= j.blocks, j = j2;
+  }
+  if (j.wide) sum_slices<T, 4>(j, at);
+  else sum_slices<T, 1>(j, at);
+}
+template <typename T>
+SumJob<T> sum_job(const float* part, T* out, int slices, long long n) {
+  const int wide = n % 4 == 0 && ff3d_aligned16(out);
+  const long long items = wide ? n / 4 : n, blocks = (items + 255) / 256;
+  return {part, out, n, slices, (int)(blocks < 2048 ? blocks : 2048), wide};
 }
 
 // rows of `cols` elements with stride ld into rows of whole granules, zeros behind
@@ -607,7 +626,7 @@ int dispatch(const Tile& t, const GemmArgs& a, hipStream_t st) {
 
 struct Plan {                    // of one call: packed operands, partial sums, and where they lie in the workspace
   int P, Cp, ldd, mblocks;
-  long long x, w, d, part, colsum, total;
+  long long x, w, d, part, part_w, colsum, total;
 };
 // bytes of the slices of a product of M x N over K (0: one piece), and their length
 template <typename T>
@@ -626,7 +645,7 @@ Plan plan(long long M, int C, int F, int pack, bool bwd) {
   auto take = [&](long long bytes) { const long long o = at; at += align_up(bytes, 256); return o; };
   p.x = (pack & 1) ? take(M * p.Cp * sizeof(T)) : 0;
   p.w = (pack & 2) ? take(2ll * F * p.Cp * sizeof(T)) : 0;
-  p.mblocks = 0, p.d = p.part = p.colsum = 0;
+  p.mblocks = 0, p.d = p.part = p.part_w = p.colsum = 0;
   if (bwd) {
     p.d = take(M * p.ldd * sizeof(T));
     p.mblocks = cdiv(M, pick<T>(M, F, p.Cp, true, false).bm);
@@ -634,7 +653,7 @@ Plan plan(long long M, int C, int F, int pack, bool bwd) {
     int k, n;
     const long long dx = slices_of<T>(pick<T>(M, C, 2ll * F, false, true), M, C, 2ll * F, &k, &n);
     const long long dw = slices_of<T>(pick<T>(2ll * F, C, M, false, true), 2ll * F, C, M, &k, &n);
-    p.part = take(dx > dw ? dx : dw);
+    p.part = take(dx), p.part_w = take(dw);
   }
   p.total = at;
   return p;
@@ -681,9 +700,9 @@ int fwd(const T* x, long long ldx, const T* w, const T* bias, T* h, int M, int C
   return dispatch<T, true, true, EPI_GATED>(pick<T>(M, F, pl.Cp, true, false), a, st);
 }
 
-// out (a.M x a.N) = the sum over a.K, in one piece or in slices that are added in order
+// out (a.M x a.N) = the sum over a.K, in one piece or in slices that `sum` is then to add
 template <typename T, bool AROW, bool BROW>
-int product(GemmArgs a, T* out, float* part, hipStream_t st) {
+int product(GemmArgs a, T* out, float* part, SumJob<T>& sum, hipStream_t st) {
   const Tile t = pick<T>(a.M, a.N, a.K, false, true);
   slices_of<T>(t, a.M, a.N, a.K, &a.kslice, &a.slices);
   a.ldo = a.N;
@@ -692,9 +711,8 @@ int product(GemmArgs a, T* out, float* part, hipStream_t st) {
     return dispatch<T, AROW, BROW, EPI_PLAIN>(t, a, st);
   }
   a.out = part, a.vec_out = a.N % 4 == 0;
-  const int s = dispatch<T, AROW, BROW, EPI_PARTIAL>(t, a, st);
-  if (s == FF3D_OK) sum_slices<T>(part, out, a.slices, (long long)a.M * a.N, st);
-  return s;
+  sum = sum_job<T>(part, out, a.slices, (long long)a.M * a.N);
+  return dispatch<T, AROW, BROW, EPI_PARTIAL>(t, a, st);
 }
 
 template <typename T>
@@ -712,12 +730,13 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
     if (s != FF3D_OK) return s;
   }
   const long long d_bytes = (long long)M * pl.ldd * sizeof(T);
+  SumJob<T> sum_x = {}, sum_w = {}, sum_b = {};
   if (dx) {
     GemmArgs a = {};
     a.a = (const char*)d, a.lda = pl.ldd, a.a_bytes = d_bytes;
     a.b = (const char*)w, a.ldb = ldw, a.b_bytes = ((2ll * F - 1) * ldw + pl.Cp) * (long long)sizeof(T), a.bcols = pl.Cp;
     a.M = M, a.N = C, a.K = 2 * F;
-    const int s = product<T, true, false>(a, dx, (float*)(ws + pl.part), st);
+    const int s = product<T, true, false>(a, dx, (float*)(ws + pl.part), sum_x, st);
     if (s != FF3D_OK) return s;
   }
   if (dw) {
@@ -725,10 +744,12 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
     a.a = (const char*)d, a.lda = pl.ldd, a.a_bytes = d_bytes, a.acols = pl.ldd;
     a.b = (const char*)x, a.ldb = ldx, a.b_bytes = ((M - 1) * ldx + pl.Cp) * (long long)sizeof(T), a.bcols = pl.Cp;
     a.M = 2 * F, a.N = C, a.K = M;
-    const int s = product<T, false, false>(a, dw, (float*)(ws + pl.part), st);
+    const int s = product<T, false, false>(a, dw, (float*)(ws + pl.part_w), sum_w, st);
     if (s != FF3D_OK) return s;
   }
-  if (db) sum_slices<T>((const float*)(ws + pl.colsum), db, pl.mblocks, 2ll * F, st);
+  if (db) sum_b = sum_job<T>((const float*)(ws + pl.colsum), db, pl.mblocks, 2ll * F);
+  const int blocks = sum_x.blocks + sum_w.blocks + sum_b.blocks;
+  if (blocks) sum_kernel<T><<<blocks, 256, 0, st>>>(sum_x, sum_w, sum_b);
   return ff3d_launch_status();
 }
 

@@ -1812,23 +1812,28 @@ def _gated_args(x, weight, bias, act):
         raise RuntimeError(f'gated_linear: expected fp32, bf16 or fp16 tensors, got {x.dtype}')
     if acode is None:
         raise ValueError(f'gated_linear: unknown activation {act!r} (one of {", ".join(_ACTS)})')
-    if x.dim() < 1 or weight.dim() != 2 or weight.shape[0] % 2 or 0 in weight.shape:
-        raise RuntimeError(f'gated_linear: expected x (..., C) and weight (2 F, C), got {tuple(x.shape)} and {tuple(weight.shape)}')
-    F2, C_ = weight.shape
-    _same(weight, x, 'weight')
+    shape = weight.shape
+    if x.dim() < 1 or len(shape) != 2 or shape[0] % 2 or 0 in shape:
+        raise RuntimeError(f'gated_linear: expected x (..., C) and weight (2 F, C), got {tuple(x.shape)} and {tuple(shape)}')
+    F2, C_ = shape
+    dtype, dev = x.dtype, x.get_device()
+    if weight.dtype is not dtype or weight.get_device() != dev:
+        _same(weight, x, 'weight')
     if x.shape[-1] != C_:
         raise RuntimeError(f'x: expected rows of {C_}, got {tuple(x.shape)}')
     if bias is not None:
-        _same(bias, x, 'bias', (F2,))
+        if bias.dtype is not dtype or bias.get_device() != dev or bias.shape != (F2,):
+            _same(bias, x, 'bias', (F2,))
         bias = bias.contiguous()
     x2 = x if x.dim() == 2 else x.reshape(-1, C_)
     if x2.shape[0] >= 0x7fffff00:
         raise RuntimeError(f'gated_linear: {x2.shape[0]} rows: fewer than {0x7fffff00} in a call')
-    if x2.stride(1) != 1 or x2.stride(0) < C_ or x2.stride(0) >= 1 << 20:          # (the kernels' offsets inside a tile are 31 bits)
-        x2 = x2.contiguous()
+    row, col = x2.stride()
+    if col != 1 or row < C_ or row >= 1 << 20:             # (the kernels' offsets inside a tile are 31 bits)
+        x2, row = x2.contiguous(), C_
     weight = weight.contiguous()
     per = 4 if code == 0 else 8
-    pack = 3 if C_ % per else (1 if x2.stride(0) % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
+    pack = 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
     return x2, weight, bias, F2 // 2, C_, pack, code, acode
 
 
