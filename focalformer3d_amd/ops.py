@@ -8,6 +8,7 @@ UT = utils.py, BC = transfusion_bbox_coder.py of the reference plugin).
 import array
 import ctypes as C
 import functools
+import operator
 import os
 import struct
 
@@ -2034,6 +2035,7 @@ def diff_attention_bwd(q, k, v, lam, heads, out, out2, stat, rest, dout, kv_head
     return _diff_attention_grads(p, keep, dims, out, out2, stat, rest, dout, want)
 
 
+_dtype_of, _shape_of = operator.attrgetter('dtype'), operator.attrgetter('shape')
 _NORM_KINDS = {2: 2, 1: 1, float('inf'): 0}
 
 
@@ -2041,17 +2043,18 @@ def _grad_list(tensors, name, numel=None):
     """Host arrays (pointers, element counts, dtype codes) of a list of dense CUDA tensors on one device, and whether all are contiguous.
     (A call's time on many small tensors is this function's: one pass per property, no per-tensor Python beyond it.)"""
     dev = tensors[0].get_device()
-    codes = [_DTYPE.get(t.dtype) for t in tensors]
-    plain = False not in [t.is_contiguous() for t in tensors]
-    if not plain or None in codes or [t.get_device() for t in tensors] != [dev] * len(tensors):
+    T = torch.Tensor
+    codes = list(map(_DTYPE.get, map(_dtype_of, tensors)))
+    plain = all(map(T.is_contiguous, tensors))
+    if not plain or None in codes or set(map(T.get_device, tensors)) != {dev}:
         for i, t in enumerate(tensors):
             if not isinstance(t, torch.Tensor) or t.get_device() != dev or t.dtype not in _DTYPE or t.layout != torch.strided:
                 raise RuntimeError(f'{name}[{i}]: expected a dense fp32, bf16 or fp16 tensor on cuda:{dev}')
             if not _dense(t):
                 raise RuntimeError(f'{name}[{i}]: expected a tensor without gaps or overlaps, got shape {tuple(t.shape)}, strides {t.stride()}')
-    ptrs = array.array('Q', [t.data_ptr() for t in tensors])
+    ptrs = array.array('Q', list(map(T.data_ptr, tensors)))
     if numel is None:
-        numel = array.array('q', [t.numel() for t in tensors])
+        numel = array.array('q', list(map(T.numel, tensors)))
     return ptrs, numel, array.array('i', codes), plain
 
 
@@ -2108,7 +2111,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     dev, n = grads[0].device, len(grads)
     if out is not None:
         out = list(out)
-        if [o.shape for o in out] != [g.shape for g in grads] or out[0].get_device() != grads[0].get_device():
+        if list(map(_shape_of, out)) != list(map(_shape_of, grads)) or out[0].get_device() != grads[0].get_device():
             raise RuntimeError(f'out: expected one tensor per gradient, of its shape and on {dev}')
         optrs, _, ocodes, out_plain = _grad_list(out, 'out', numel)
         if not (plain and out_plain):
