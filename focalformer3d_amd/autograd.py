@@ -212,15 +212,14 @@ class GatedLinearFunction(Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, act):
-        ctx.save_for_backward(x, weight, bias)
-        ctx.act = act
-        return ops.gated_linear(x, weight, bias, act)
+        h, keep, ctx.dims = ops.gated_linear_keep(x, weight, bias, act)
+        ctx.save_for_backward(*keep)
+        return h
 
     @staticmethod
     @_once
     def backward(ctx, dh):
-        x, weight, bias = ctx.saved_tensors
-        return (*ops.gated_linear_bwd(x, weight, bias, ctx.act, dh, ctx.needs_input_grad[:3]), None)
+        return (*ops._gated_grads(ops._gated_again(ctx.saved_tensors, ctx.dims), ctx.dims[5], dh, ctx.needs_input_grad[:3]), None)
 
 
 def gated_linear(x, weight, bias=None, act='silu'):

@@ -1838,12 +1838,8 @@ def _gated_args(x, weight, bias, act):
     return x2, weight, bias, F2 // 2, C_, pack, code, acode
 
 
-@_on_device_of('x')
-def gated_linear(x, weight, bias=None, act='silu'):
-    """h = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel (ff3d_gated_linear_fwd): x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F)
-    or None, all fp32, bf16 or fp16 -> (..., F).  act: 'silu', 'gelu' (erf form), 'relu' or 'sigmoid'.  Sums in fp32, one rounding.
-    The differentiable form is ``autograd.gated_linear``."""
-    x2, weight, bias, F_, C_, pack, code, acode = _gated_args(x, weight, bias, act)
+def _gated_fwd(x, args):
+    x2, weight, bias, F_, C_, pack, code, acode = args
     M = x2.shape[0]
     h = torch.empty((*x.shape[:-1], F_), dtype=x.dtype, device=x.device)
     if M == 0:
@@ -1860,25 +1856,58 @@ def gated_linear(x, weight, bias=None, act='silu'):
 
 
 @_on_device_of('x')
+def gated_linear(x, weight, bias=None, act='silu'):
+    """h = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel (ff3d_gated_linear_fwd): x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F)
+    or None, all fp32, bf16 or fp16 -> (..., F).  act: 'silu', 'gelu' (erf form), 'relu' or 'sigmoid'.  Sums in fp32, one rounding.
+    The differentiable form is ``autograd.gated_linear``."""
+    return _gated_fwd(x, _gated_args(x, weight, bias, act))
+
+
+@_on_device_of('x')
+def gated_linear_keep(x, weight, bias=None, act='silu'):
+    """``gated_linear`` -> (h, the operands as the kernels read them, sizes): what autograd keeps."""
+    args = _gated_args(x, weight, bias, act)
+    return _gated_fwd(x, args), args[:3], (*args[3:], x.shape)
+
+
+@_on_device_of('x')
 def gated_linear_bwd(x, weight, bias, act, dh, want=(True, True, True)):
     """Gradients of ``gated_linear`` for dh (..., F) -> (dx, dweight, dbias); None where ``want`` is false (or there is no bias)."""
-    x2, weight, bias, F_, C_, pack, code, acode = _gated_args(x, weight, bias, act)
+    args = _gated_args(x, weight, bias, act)
+    _same(dh, x, 'dh', (*x.shape[:-1], args[3]))
+    return _gated_grads(args, x.shape, dh, want)
+
+
+def _gated_again(keep, dims):
+    """The checked operands that autograd kept (addresses and strides are asked for again: a hook may have moved them)."""
+    x2, weight, bias = keep
+    F_, C_, _, code, acode, _ = dims
+    row, col = x2.stride()
+    if col != 1 or row < C_ or row >= 1 << 20 or not weight.is_contiguous() or not (bias is None or bias.is_contiguous()):
+        x2, weight, bias = x2.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous()
+        row = C_
+    per = 4 if code == 0 else 8
+    pack = 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
+    return x2, weight, bias, F_, C_, pack, code, acode
+
+
+def _gated_grads(args, shape, dh, want):
+    """Gradients from checked operands; x has the given shape, dh the type and number of elements of h."""
+    x2, weight, bias, F_, C_, pack, code, acode = args
     M = x2.shape[0]
-    _same(dh, x, 'dh', (*x.shape[:-1], F_))
     want_b = want[2] and bias is not None
-    dx = _new_like(x, M == 0) if want[0] else None
+    dx = _new_like(x2, M == 0) if want[0] else None
     dw = _new_like(weight, M == 0) if want[1] else None
     db = _new_like(bias, M == 0) if want_b else None
-    if M == 0 or not (want[0] or want[1] or want_b):
-        return dx, dw, db
-    dh2 = dh.reshape(-1, F_)
-    if dh2.stride(1) != 1 or dh2.stride(0) < F_:
-        dh2 = dh2.contiguous()
-    lib = _lib.load()
-    ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 1), dtype=torch.uint8, device=x.device)
-    _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh2.stride(0), _ptr(dx), _ptr(dw), _ptr(db),
-                                         M, C_, F_, acode, code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
-    return dx, dw, db
+    if M > 0 and (want[0] or want[1] or want_b):
+        dh2 = dh.reshape(M, F_)
+        if dh2.stride(1) != 1 or dh2.stride(0) < F_:
+            dh2 = dh2.contiguous()
+        lib = _lib.load()
+        ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 1), dtype=torch.uint8, device=x2.device)
+        _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh2.stride(0), _ptr(dx), _ptr(dw), _ptr(db),
+                                             M, C_, F_, acode, code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
+    return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db
 
 
 def _attn_rows(t, name, like, shape, per):
