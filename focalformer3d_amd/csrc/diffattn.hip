@@ -1133,7 +1133,7 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
   a.d2 = dlam && sizeof(T) == 2 ? a.rowdata + s.rowdata / 4 : nullptr;
   // both kernels with and without the second product of rest_frag: 1 x 4096, 16 heads over 4 of 64, causal: +48 and +7 us (registers run
-  // out); 3 x 333 x 1777, 4 heads of 32: +4 and +3 us
+  // out); 3 x 333 x 1777, 4 heads of 32: +6 and +3 us
   if (a.Nk == 1) a.scale = 0.f;    // the weight of a single key is 1 whatever its score: dq and dk are zero, not the rounding of dP - D
   const bool fine = sizeof(T) == 2 && (D < 64 || (long long)a.B * a.H * a.Nq * a.Nk <= 1 << 24);
   constexpr bool FINE = sizeof(T) == 2, COARSE = sizeof(T) == 2 && D < 64;     // COARSE: the variant where `fine` is false

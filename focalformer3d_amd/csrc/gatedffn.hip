@@ -14,7 +14,7 @@
 // columns of one output row and stores them together.
 // Measured on one MI355X (a large library product: 1309 TFLOP/s in bf16, 154 in fp32): 16384 x 1024 -> 2736 in bf16, 184 GFLOP each: forward
 // 196 .. 211 us, d 271, dx 181, dW 286 + 10 (the matrix unit is the bound; d adds reading dh and writing d, dW's 88 tiles in two slices fill
-// 69 % of the chip); 2880 x 256 -> 1024 in fp32, 3 GFLOP each: 31, 39, 33, 35 us and 5 for each sum of slices (bound by splitting operands
+// 69 % of the chip); 2880 x 256 -> 1024 in fp32, 3 GFLOP each: 31, 39, 33, 35 us and 10 for the sums of slices (bound by splitting operands
 // and by latency); 4 x 1024 -> 2736 in bf16: 8 us, the weight at 1.4 TB/s.
 #include <type_traits>
 

@@ -293,3 +293,24 @@ def test_captured_training_chain(dtype):
         torch.cuda.synchronize()
         for a, b in zip(out, want):
             assert torch.equal(a, b), step
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.float16])
+def test_operands_that_hooks_move(dtype):
+    """Operands that were packed to host memory between the passes, transposed and unaligned ones among them: the same gradients."""
+    from focalformer3d_amd.autograd import differential_attention, gated_linear
+    torch.manual_seed(11)
+    r = lambda *s: torch.randn(*s, device='cuda').to(dtype)  # noqa: E731
+    q, k, v = r(50, 2, 128).transpose(0, 1), r(2, 70, 65)[..., 1:], r(2, 70, 64)
+    leaves = [t.requires_grad_(True) for t in (q, k, v, r(1).expand(4), r(2 * 96, 128) * 0.1, r(2 * 96))]
+    mask, lens, dout = torch.rand(50, 70, device='cuda') < 0.3, torch.tensor([70, 31], dtype=torch.int32, device='cuda'), r(2, 50, 96)
+
+    def grads():
+        y = differential_attention(*leaves[:4], 4, kv_heads=2, mask=mask, kv_lens=lens)
+        return y, gated_linear(y, leaves[4], leaves[5], 'gelu')
+    y, h = grads()
+    want = torch.autograd.grad(h, leaves, dout)
+    with torch.autograd.graph.save_on_cpu():
+        y, h = grads()
+    for a, b, t in zip(torch.autograd.grad(h, leaves, dout), want, leaves):
+        assert torch.equal(a, b) and a.shape == t.shape
