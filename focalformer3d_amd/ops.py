@@ -1859,6 +1859,7 @@ def _gated_fwd(x, args):
 def gated_linear(x, weight, bias=None, act='silu'):
     """h = act(x Wg^T + bg) * (x Wu^T + bu) in one kernel (ff3d_gated_linear_fwd): x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F)
     or None, all fp32, bf16 or fp16 -> (..., F).  act: 'silu', 'gelu' (erf form), 'relu' or 'sigmoid'.  Sums in fp32, one rounding.
+    (An infinite fp32 operand gives NaN: it is split into bf16 planes.)
     The differentiable form is ``autograd.gated_linear``."""
     return _gated_fwd(x, _gated_args(x, weight, bias, act))
 
