@@ -314,3 +314,52 @@ def test_operands_that_hooks_move(dtype):
         y, h = grads()
     for a, b, t in zip(torch.autograd.grad(h, leaves, dout), want, leaves):
         assert torch.equal(a, b) and a.shape == t.shape
+
+
+def test_offsets_beyond_31_bits():
+    """Keys, rows and gradients with more than 2^31 elements: what lies at the end is read and written.
+
+    Attention: all keys are zero but the last, whose scores are 32 in both maps, so it has all the weight but 4.4e6 e^-32 = 6e-8 of it: out is
+    (1 - lam) v and dv (1 - lam) dO of the last key up to three roundings of 2^-8 (weight, value, result)."""
+    from focalformer3d_amd import ops
+    G, d, Nk = 4, 64, 4_400_000
+    bf = torch.bfloat16
+    q = torch.ones(1, 1, G * 2 * d, device='cuda', dtype=bf)
+    k, v = torch.zeros(1, Nk, G * 2 * d, device='cuda', dtype=bf), torch.zeros(1, Nk, G * 2 * d, device='cuda', dtype=bf)
+    assert k.numel() > 1 << 31
+    k[0, -1] = 4.0
+    v[0, -1], dout = torch.randn(G * 2 * d, device='cuda').to(bf), torch.randn(1, 1, G * 2 * d, device='cuda').to(bf)
+    lam = torch.full((G,), 0.25, device='cuda', dtype=bf)
+    saved = ops.diff_attention_train_fwd(q, k, v, lam, G)
+    want = 0.75 * v[0, -1].double()
+    assert bool(((saved[0][0, 0].double() - want).abs() <= 3 * 2.0 ** -8 * want.abs() + 1e-6).all())
+    _, dk, dv, _ = ops.diff_attention_bwd(q, k, v, lam, G, *saved, dout)
+    want = 0.75 * dout[0, 0].double()
+    assert bool(((dv[0, -1].double() - want).abs() <= 3 * 2.0 ** -8 * want.abs() + 1e-6).all())
+    assert float(dv[0, 1 << 21].abs().max()) <= 1e-10 and bool(torch.isfinite(dk[0, -1]).all())
+    del k, v, dk, dv, saved
+
+    # rows of the gated projection: the last ones against the same rows alone (another tile and order of sums: fp32 sums of 1024 products)
+    M, C, F_ = 2_200_000, 1024, 16
+    x = torch.zeros(M, C, device='cuda', dtype=bf)
+    assert x.numel() > 1 << 31
+    tail = torch.randn(40, C, device='cuda').to(bf)
+    x[-40:] = tail
+    w, dh = (torch.randn(2 * F_, C, device='cuda') * 0.03).to(bf), torch.zeros(M, F_, device='cuda', dtype=bf)
+    dh[-40:] = torch.randn(40, F_, device='cuda').to(bf)
+    h = ops.gated_linear(x, w)
+    ref = ops.gated_linear(tail, w)
+    assert bool(((h[-40:].double() - ref.double()).abs() <= 2.0 ** -7 * ref.double().abs() + 1e-5).all()) and float(h[:-40].abs().max()) == 0.0
+    dx, dw, _ = ops.gated_linear_bwd(x, w, None, 'silu', dh)
+    rx, rw, _ = ops.gated_linear_bwd(tail, w, None, 'silu', dh[-40:])
+    # d is rounded to bf16 on both sides from sums in another order (2^-7 where they straddle a step), then summed over 32 and 40 terms
+    assert float((dx[-40:].double() - rx.double()).norm() / rx.double().norm()) <= 2.0 ** -6
+    assert float((dw.double() - rw.double()).norm() / rw.double().norm()) <= 2.0 ** -6
+    del x, dx, h
+
+    g = torch.full(((1 << 31) + 5,), 2.0 ** -10, device='cuda', dtype=bf)
+    g[-1] = 64.0
+    norm = ops.clip_grads([g], 1.0)
+    want = ((2.0 ** 31 + 4) * 2.0 ** -20 + 4096.0) ** 0.5
+    assert abs(float(norm) - want) <= 2.0 ** -22 * want
+    assert abs(float(g[-1]) - 64.0 / want) <= 2.0 ** -8 and abs(float(g[5]) * want * 1024 - 1) <= 2.0 ** -7
