@@ -1806,6 +1806,23 @@ def _new_like(t, zero=False):
     return (torch.zeros if zero else torch.empty)(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _whole_rows(t, apart=float('inf')):
+    """t (M, n) -> (itself, or a view or copy of it, with dense rows fewer than ``apart`` elements apart; its row stride).  The stride of a
+    single row says nothing (``contiguous()`` keeps it, whatever it is) and is replaced."""
+    (M, n), (row, col) = t.shape, t.stride()
+    if col == 1 and n <= row < apart:
+        return t, row
+    if M == 1 and (col == 1 or n == 1):
+        return t.as_strided((1, n), (n, 1)), n
+    return t.clone(memory_format=torch.contiguous_format), n
+
+
+def _gated_pack(x2, row, weight, C_, code):
+    """Which operands have to be packed into rows of whole aligned granules: bit 0 x, bit 1 the weight."""
+    per = 4 if code == 0 else 8
+    return 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
+
+
 def _gated_args(x, weight, bias, act):
     """Checked operands -> (x as rows, weight, bias, F, C, which operands have to be packed, dtype code, activation code)."""
     code, acode = _DTYPE.get(x.dtype), _ACTS.get(act)
@@ -1829,13 +1846,9 @@ def _gated_args(x, weight, bias, act):
     x2 = x if x.dim() == 2 else x.reshape(-1, C_)
     if x2.shape[0] >= 0x7fffff00:
         raise RuntimeError(f'gated_linear: {x2.shape[0]} rows: fewer than {0x7fffff00} in a call')
-    row, col = x2.stride()
-    if col != 1 or row < C_ or row >= 1 << 20:             # (the kernels' offsets inside a tile are 31 bits)
-        x2, row = x2.contiguous(), C_
+    x2, row = _whole_rows(x2, 1 << 20)                     # (the kernels' offsets inside a tile are 31 bits)
     weight = weight.contiguous()
-    per = 4 if code == 0 else 8
-    pack = 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
-    return x2, weight, bias, F2 // 2, C_, pack, code, acode
+    return x2, weight, bias, F2 // 2, C_, _gated_pack(x2, row, weight, C_, code), code, acode
 
 
 def _gated_fwd(x, args):
@@ -1883,13 +1896,9 @@ def _gated_again(keep, dims):
     """The checked operands that autograd kept (addresses and strides are asked for again: a hook may have moved them)."""
     x2, weight, bias = keep
     F_, C_, _, code, acode, _ = dims
-    row, col = x2.stride()
-    if col != 1 or row < C_ or row >= 1 << 20 or not weight.is_contiguous() or not (bias is None or bias.is_contiguous()):
-        x2, weight, bias = x2.contiguous(), weight.contiguous(), None if bias is None else bias.contiguous()
-        row = C_
-    per = 4 if code == 0 else 8
-    pack = 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
-    return x2, weight, bias, F_, C_, pack, code, acode
+    x2, row = _whole_rows(x2, 1 << 20)
+    weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
+    return x2, weight, bias, F_, C_, _gated_pack(x2, row, weight, C_, code), code, acode
 
 
 def _gated_grads(args, shape, dh, want):
@@ -1901,12 +1910,10 @@ def _gated_grads(args, shape, dh, want):
     dw = _new_like(weight, M == 0) if want[1] else None
     db = _new_like(bias, M == 0) if want_b else None
     if M > 0 and (want[0] or want[1] or want_b):
-        dh2 = dh.reshape(M, F_)
-        if dh2.stride(1) != 1 or dh2.stride(0) < F_:
-            dh2 = dh2.contiguous()
+        dh2, dh_row = _whole_rows(dh.reshape(M, F_))
         lib = _lib.load()
         ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 1), dtype=torch.uint8, device=x2.device)
-        _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh2.stride(0), _ptr(dx), _ptr(dw), _ptr(db),
+        _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh_row, _ptr(dx), _ptr(dw), _ptr(db),
                                              M, C_, F_, acode, code, pack, _ptr(ws), _stream()), 'ff3d_gated_linear_bwd')
     return dx if dx is None or len(shape) == 2 else dx.view(shape), dw, db
 
