@@ -8,7 +8,7 @@
 //   gated_bwd  the same products again with dh in the epilogue -> d (rounded to the type once, as the operand of the two products
 //              below has to be) and the column sums of the unrounded d.  g and u are recomputed instead of saved: 2 M C F more
 //              multiply-adds, against 2 M F values written and read again and against rounding them, which alone would take the
-//              gradients from 1.4 to 1.7 times the error of a single rounding
+//              gradients from 1.4 to 1.7 times the error of a single rounding.  In fp16 d is scaled first (RANGED below)
 //   plain      dx and, with its row sum cut into slices that a second kernel adds in order, dW: results do not depend on timing
 // A block computes C^T tiles: the n side (features of W, columns of the output) is the row operand, so a lane holds 4 consecutive
 // columns of one output row and stores them together.
@@ -40,7 +40,38 @@ struct GemmArgs {
   int F, act, mt, nt, slices, kslice;
   int vec_out, vec_out2, vec_dh;     // 16-byte accesses of rows of out, of its second half (EPI_GATED_BWD) and of dh are aligned
   int out_pad;                  // EPI_GATED_BWD: zero columns behind the 2 F
+  const float4* range;          // fp16 gradients: what d's scale follows from (Range), nrange of them
+  int nrange;
 };
+
+// fp16 holds 2^-24 .. 2^16, and a gradient's terms need not lie there where its sums do: dh u act' overflows behind a scaled loss, or loses
+// its digits below 2^-14 (dh of 1e-6 over 4096 rows: dW off by 62 times the error of one rounding).  d is therefore stored times a power of
+// two, the largest with |d| < 2^15 for certain, and dx, dW and their slices are multiplied back in fp32.  The certainty is
+//   |d| <= 1.14 (max_m max|dh_m| |x_m|  max_n |w_n| + max|dh| (max|b| + 1)),       |act'| <= 1.14, |act(g)| <= |g| or 1
+// over finite values (one that is not gives a row that is not, whatever the scale), a few binades above the largest d of ordinary data: what is
+// lost of d lies 2^-29 and more below the bound.  One scale serves the whole matrix, since dx sums over its columns and dW over its rows.
+// It costs one reading of dh, x and W:
+// 16384 x 1024 -> 2736 in 34 us (134 MB, 4.0 TB/s; forward and backward 915 instead of 866), 2880 x 256 -> 1024 in 6 us.
+template <typename T>
+constexpr bool RANGED = sizeof(T) == 2 && !std::is_same_v<T, __bf16>;
+constexpr int RANGE_BLOCKS = 256, RANGE_THREADS = 1024;
+
+__device__ __forceinline__ float max_wave(float v) {
+#pragma unroll
+  for (int x = 32; x > 0; x >>= 1) v = fmaxf(v, __shfl_xor(v, x));
+  return v;
+}
+// e of the scale 2^e, the same in every wave that asks
+__device__ __forceinline__ int range_exp(const GemmArgs& p, int lane) {
+  float4 m = {0.f, 0.f, 0.f, 0.f};
+  for (int i = lane; i < p.nrange; i += 64) {
+    const float4 r = p.range[i];
+    m.x = fmaxf(m.x, r.x), m.y = fmaxf(m.y, r.y), m.z = fmaxf(m.z, r.z), m.w = fmaxf(m.w, r.w);
+  }
+  const float bound = 1.14f * (max_wave(m.x) * sqrtf(max_wave(m.z)) + max_wave(m.y) * (max_wave(m.w) + 1.f));
+  const int ex = (int)(__float_as_uint(bound) >> 23) - 127;
+  return __builtin_amdgcn_readfirstlane(bound > 0.f ? 14 - ex : 0);
+}
 
 // exp for the type: fp32 outputs take the full-precision function, 16-bit ones the hardware's exp2 of the rounded product
 template <typename T>
@@ -351,7 +382,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
       }
       __syncthreads();
     }
-    float sg[TN / 2][4][4] = {}, su[TN / 2][4][4] = {};
+    float sg[TN / 2][4][4] = {}, su[TN / 2][4][4] = {}, scale = 1.f;
+    if constexpr (RANGED<T> && EPI == EPI_GATED_BWD) scale = ff3d_pow2(range_exp(p, lane));
     with_act(p.act, [&](auto act) {                  // outside the loops: the elements' chains run beside each other
     constexpr int ACT = decltype(act)::value;
 #pragma unroll
@@ -383,6 +415,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
               act_both<T, ACT>(g[i], a, da);
               o[i] = d[i] * u[i] * da, o2[i] = d[i] * a;
               sg[pr][q][i] += o[i], su[pr][q][i] += o2[i];
+              if constexpr (RANGED<T>) o[i] *= scale, o2[i] *= scale;
             }
             store4((T*)(at + TILE), o2, 4, true);
           }
@@ -423,6 +456,8 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
     }
   } else if constexpr (EPI == EPI_PLAIN) {
     static_assert(BM * GO * 16 <= STAGES * STAGE, "the tile fits where the operands were");
+    float undo = 1.f;
+    if constexpr (RANGED<T>) undo = ff3d_pow2(-range_exp(p, lane));
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
@@ -431,12 +466,14 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
         for (int j = 0; j < TM; ++j) {
           float o[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[e] = acc[i][j][4 * q + e];
+          for (int e = 0; e < 4; ++e) o[e] = RANGED<T> ? acc[i][j][4 * q + e] * undo : acc[i][j][4 * q + e];
           store4((T*)(lds + out_at((wm * TM + j) * 32 + (lane & 31), (wn * TN + i) * 32 + 8 * q + 4 * half)), o, 4, true);
         }
     __syncthreads();
     store_tile(lds, (T*)p.out, p.ldo, p.N, p.vec_out);
   } else {
+    float undo = 1.f;
+    if constexpr (RANGED<T>) undo = ff3d_pow2(-range_exp(p, lane));
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
@@ -448,7 +485,7 @@ __global__ __launch_bounds__(WM* WN * 64) void gemm_kernel(GemmArgs p) {
           if (m < p.M && left > 0) {
             float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = acc[i][j][4 * q + e];
+            for (int e = 0; e < 4; ++e) o[e] = RANGED<T> ? acc[i][j][4 * q + e] * undo : acc[i][j][4 * q + e];
             store4((float*)p.out + ((long long)slice * p.M + m) * p.ldo + n, o, left, p.vec_out);
           }
         }
@@ -506,6 +543,72 @@ __global__ __launch_bounds__(NW * 64) void gated_rows_kernel(GemmArgs p) {
     ((T*)p.out)[(long long)(m0 + ml) * p.ldo + n0 + nl] = from_f<T>(act_f<T, ACT>(g) * u);
   }
   });
+}
+
+// Range, one per block: max_m max|dh_m| |x_m|, max|dh|, max_n |w_n|^2, max|b|, all over finite values.  A wave takes a row of dh and of x, or
+// one of the weight, at a time; rows of x and of the weight are whole aligned granules (K elements, zeros behind their own).
+template <typename T>
+__global__ __launch_bounds__(RANGE_THREADS) void range_kernel(GemmArgs p, float4* range) {
+  constexpr int P = Type<T>::PER16;
+  __shared__ float4 found[RANGE_THREADS / 64];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  float4 m = {0.f, 0.f, 0.f, 0.f};
+  auto finite = [](T v) {
+    const float a = fabsf(to_f(v));
+    return a < INFINITY ? a : 0.f;                   // a NaN compares false
+  };
+  auto largest = [&](const T* row, int n, bool vec) {
+    float top = 0.f;
+    int c = lane * P;
+    if (vec) {
+#pragma unroll 4
+      for (; c + P <= n; c += 64 * P) {
+        const vec8<T> v = *(const vec8<T>*)(row + c);
+#pragma unroll
+        for (int e = 0; e < P; ++e) top = fmaxf(top, finite(v[e]));
+      }
+      for (int e = c; e < min(c + P, n); ++e) top = fmaxf(top, finite(row[e]));
+    } else {
+#pragma unroll 4
+      for (int e = lane; e < n; e += 64) top = fmaxf(top, finite(row[e]));
+    }
+    return max_wave(top);
+  };
+  auto squares = [&](const char* row) {
+    float s = 0.f;
+#pragma unroll 4
+    for (int c = lane * P; c < p.K; c += 64 * P) {
+      const vec8<T> v = *(const vec8<T>*)(row + c * (int)sizeof(T));
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const float a = finite(v[e]);
+        s = fmaf(a, a, s);
+      }
+    }
+#pragma unroll
+    for (int x = 32; x > 0; x >>= 1) s += __shfl_xor(s, x);
+    return s;
+  };
+  const long long rows = p.M + 2ll * p.F;
+  for (long long r = (long long)blockIdx.x * (RANGE_THREADS / 64) + wave; r < rows; r += (long long)gridDim.x * (RANGE_THREADS / 64)) {
+    if (r < p.M) {
+      const float top = largest((const T*)p.dh + r * p.lddh, p.F, p.vec_dh);
+      m.x = fmaxf(m.x, top * sqrtf(squares(p.a + r * p.lda * (long long)sizeof(T)))), m.y = fmaxf(m.y, top);
+    } else {
+      const long long n = r - p.M;
+      m.z = fmaxf(m.z, squares(p.b + n * p.ldb * (long long)sizeof(T)));
+      if (p.bias) m.w = fmaxf(m.w, finite(((const T*)p.bias)[n]));
+    }
+  }
+  if (lane == 0) found[wave] = m;                    // the same in every lane
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < RANGE_THREADS / 64; ++w) {
+      const float4 o = found[w];
+      m.x = fmaxf(m.x, o.x), m.y = fmaxf(m.y, o.y), m.z = fmaxf(m.z, o.z), m.w = fmaxf(m.w, o.w);
+    }
+    range[blockIdx.x] = m;
+  }
 }
 
 // out[i] = sum of the slices part[k n + i] in order
@@ -626,7 +729,7 @@ int dispatch(const Tile& t, const GemmArgs& a, hipStream_t st) {
 
 struct Plan {                    // of one call: packed operands, partial sums, and where they lie in the workspace
   int P, Cp, ldd, mblocks;
-  long long x, w, d, part, part_w, colsum, total;
+  long long x, w, d, part, part_w, colsum, range, total;
 };
 // bytes of the slices of a product of M x N over K (0: one piece), and their length
 template <typename T>
@@ -645,7 +748,7 @@ Plan plan(long long M, int C, int F, int pack, bool bwd) {
   auto take = [&](long long bytes) { const long long o = at; at += align_up(bytes, 256); return o; };
   p.x = (pack & 1) ? take(M * p.Cp * sizeof(T)) : 0;
   p.w = (pack & 2) ? take(2ll * F * p.Cp * sizeof(T)) : 0;
-  p.mblocks = 0, p.d = p.part = p.part_w = p.colsum = 0;
+  p.mblocks = 0, p.d = p.part = p.part_w = p.colsum = p.range = 0;
   if (bwd) {
     p.d = take(M * p.ldd * sizeof(T));
     p.mblocks = cdiv(M, pick<T>(M, F, p.Cp, true, false).bm);
@@ -654,6 +757,7 @@ Plan plan(long long M, int C, int F, int pack, bool bwd) {
     const long long dx = slices_of<T>(pick<T>(M, C, 2ll * F, false, true), M, C, 2ll * F, &k, &n);
     const long long dw = slices_of<T>(pick<T>(2ll * F, C, M, false, true), 2ll * F, C, M, &k, &n);
     p.part = take(dx), p.part_w = take(dw);
+    if (RANGED<T>) p.range = take(RANGE_BLOCKS * sizeof(float4));
   }
   p.total = at;
   return p;
@@ -722,10 +826,18 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
   long long ldw = C;
   pack_operands<T>(pl, pack, x, ldx, w, ldw, M, C, F, ws, st);
   T* d = (T*)(ws + pl.d);
+  float4* range = (float4*)(ws + pl.range);
+  int nrange = 0;
   {
     GemmArgs a = gated_args<T>(x, ldx, w, ldw, bias, M, C, pl.Cp, F, act);
     a.out = d, a.ldo = pl.ldd, a.dh = dh, a.lddh = lddh, a.colsum = db ? (float*)(ws + pl.colsum) : nullptr;
     a.out_pad = pl.ldd - 2 * F, a.vec_out = 1, a.vec_out2 = F * sizeof(T) % 16 == 0, a.vec_dh = vec_ok(dh, lddh, sizeof(T));
+    if constexpr (RANGED<T>) {
+      const int rows = cdiv(M + 2ll * F, RANGE_THREADS / 64);
+      nrange = rows < RANGE_BLOCKS ? rows : RANGE_BLOCKS;
+      range_kernel<T><<<nrange, RANGE_THREADS, 0, st>>>(a, range);
+      a.range = range, a.nrange = nrange;
+    }
     const int s = dispatch<T, true, true, EPI_GATED_BWD>(pick<T>(M, F, pl.Cp, true, false), a, st);
     if (s != FF3D_OK) return s;
   }
@@ -735,7 +847,7 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
     GemmArgs a = {};
     a.a = (const char*)d, a.lda = pl.ldd, a.a_bytes = d_bytes;
     a.b = (const char*)w, a.ldb = ldw, a.b_bytes = ((2ll * F - 1) * ldw + pl.Cp) * (long long)sizeof(T), a.bcols = pl.Cp;
-    a.M = M, a.N = C, a.K = 2 * F;
+    a.M = M, a.N = C, a.K = 2 * F, a.range = range, a.nrange = nrange;
     const int s = product<T, true, false>(a, dx, (float*)(ws + pl.part), sum_x, st);
     if (s != FF3D_OK) return s;
   }
@@ -743,7 +855,7 @@ int bwd(const T* x, long long ldx, const T* w, const T* bias, const T* dh, long 
     GemmArgs a = {};
     a.a = (const char*)d, a.lda = pl.ldd, a.a_bytes = d_bytes, a.acols = pl.ldd;
     a.b = (const char*)x, a.ldb = ldx, a.b_bytes = ((M - 1) * ldx + pl.Cp) * (long long)sizeof(T), a.bcols = pl.Cp;
-    a.M = 2 * F, a.N = C, a.K = M;
+    a.M = 2 * F, a.N = C, a.K = M, a.range = range, a.nrange = nrange;
     const int s = product<T, false, false>(a, dw, (float*)(ws + pl.part_w), sum_w, st);
     if (s != FF3D_OK) return s;
   }
@@ -771,7 +883,8 @@ int check(const void* x, const void* w, const void* h, int64_t ldx, int64_t ldh,
 
 extern "C" int64_t ff3d_gated_linear_workspace_bytes(int M, int C, int F, int dtype, int pack, int backward) {
   if (M <= 0 || C <= 0 || F <= 0) return 0;
-  return dtype == FF3D_F32 ? plan<float>(M, C, F, pack, backward).total : plan<__bf16>(M, C, F, pack, backward).total;
+  if (dtype == FF3D_F32) return plan<float>(M, C, F, pack, backward).total;
+  return dtype == FF3D_F16 ? plan<_Float16>(M, C, F, pack, backward).total : plan<__bf16>(M, C, F, pack, backward).total;
 }
 
 extern "C" int ff3d_gated_linear_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, void* h, int M, int C, int F, int act,

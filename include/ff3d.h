@@ -754,6 +754,8 @@ int ff3d_conv3x3_small_f16x3_group(int n, const void* const* x_hi, const void* c
  *   stride is no multiple of 16 bytes or the base is not 16-byte aligned (without the bit such an operand is FF3D_ERR_ALIGNMENT).
  * workspace: ff3d_gated_linear_workspace_bytes of the same M, C, F, dtype, pack and backward, 16-byte aligned; its content is
  *   scratch.  2 F * C and M-independent row offsets stay below 2^31 bytes; results do not depend on timing (ordered sums).
+ *   In fp16 the gradients' terms are scaled by a power of two, so that dx, dw and db keep their digits for a dh near either end of fp16's
+ *   range; what is not finite in x, weight or dh reaches the rows and columns that it belongs to.
  * fp32 operands are split into three bf16 planes (six products, as exact as fp32 ones): an infinite operand gives NaN. */
 int64_t ff3d_gated_linear_workspace_bytes(int M, int C, int F, int dtype, int pack, int backward);
 int ff3d_gated_linear_fwd(const void* x, int64_t ldx, const void* weight, const void* bias, void* h, int M, int C, int F, int act,

@@ -1,4 +1,4 @@
-"""Calls of the operators in three types that their documentation allows: rows of unusual strides."""
+"""Calls of the operators in three types that their documentation allows: rows of unusual strides, gradients near the ends of fp16's range."""
 import pytest
 import torch
 
@@ -66,3 +66,95 @@ def test_gated_linear_of_one_value(dtype):
     want = gated64(x.detach(), w.detach(), None, 'silu', torch.ones(1, 1, device='cuda', dtype=dt))
     for t, e in zip((h, x.grad, w.grad), want):
         assert_within(t, e)
+
+
+# ------------------------------------------------------------------------------------------------ fp16's range
+def _gated_gradients(x, w, b, act, dh):
+    from focalformer3d_amd import ops
+    return ops.gated_linear_bwd(x, w, b, act, dh)
+
+
+@pytest.mark.parametrize('act', ['silu', 'gelu', 'relu', 'sigmoid'])
+@pytest.mark.parametrize('M,C,F,bias', [(2000, 64, 96, True), (300, 40, 33, False)])
+def test_small_fp16_gradients_keep_their_digits(act, M, C, F, bias):
+    """dh of 2^-19: dg and du lie below fp16's normal numbers, dx and dW do not.  A power of two scales the operands of both products exactly,
+    so the results are those for 2^12 dh, up to one rounding of each, whose step does not fall below 2^-24."""
+    r = _randn(27)
+    x, w, b = (r(M, C) * 8).half(), (r(2 * F, C) * 0.3).half(), (r(2 * F) * 0.3).half() if bias else None
+    small = (r(M, F) * 2.0 ** -19).half()
+    big = (small.double() * 4096).half()
+    assert torch.equal(big.double(), small.double() * 4096) and float(small.abs().max()) < 2.0 ** -14
+    for name, s, t in zip(('dx', 'dw', 'db'), _gated_gradients(x, w, b, act, small), _gated_gradients(x, w, b, act, big)):
+        if s is None:
+            continue
+        s, t = s.double() * 4096, t.double()
+        assert bool(((s - t).abs() <= 2 * 2.0 ** -11 * t.abs() * 1.01 + 4096 * 2.0 ** -25).all()), name
+    # and dW, which sums many rows, is as near the exact result as one rounding of its terms and one of itself leave it
+    exact = gated64(x, w, b, act, small)[2][0]
+    err = (_gated_gradients(x, w, b, act, small)[1].double() - exact).norm()
+    assert float(err) <= 1.5 * float((exact.half().double() - exact).norm())
+
+
+def test_large_fp16_gradients_stay_finite():
+    """dh u act' beyond 65504 at one place, dx and dW within the range: the sums are what the formula says.  The rounding of that one term, at
+    most 2^-11 of it, is common to a whole row of dx and of dW, whose own roundings are 0.42 of that in the mean (a relative error uniform in
+    +- 2^-11 m^-1, m uniform in the binade): sqrt(1 + 0.42^-2) = 2.6; 2.75 with the scatter."""
+    from focalformer3d_amd import ops
+    M, C, F = 70, 48, 64
+    r = _randn(28)
+    x, w, dh = (r(M, C) * 0.05).half(), (r(2 * F, C) * 0.03).half(), (r(M, F) * 0.1).half()
+    b = torch.full((2 * F,), 6.0, device='cuda', dtype=torch.half)
+    dh[5, 7] = 30000.0                                   # times u = 6: 1.8e5
+    want = gated64(x, w, b, 'silu', dh)
+    got = (ops.gated_linear(x, w, b), *ops.gated_linear_bwd(x, w, b, 'silu', dh))
+    assert float(want[1][0].abs().max()) < 65504 and float(want[2][0].abs().max()) < 65504
+    for name, t, (value, _) in list(zip(('h', 'dx', 'dw'), got, want)):
+        assert bool(t.isfinite().all()), name
+        assert float((t.double() - value).norm()) <= 2.75 * float((value.half().double() - value).norm()), name
+    rows = torch.arange(M, device='cuda') != 5           # and the other rows keep their digits
+    e = want[1][0][rows]
+    assert float((got[1][rows].double() - e).norm()) <= 1.5 * float((e.half().double() - e).norm())
+
+
+def test_infinite_fp16_gradient_stays_in_its_row():
+    from focalformer3d_amd import ops
+    r = _randn(29)
+    x, w, dh = r(70, 40).half(), (r(64, 40) * 0.1).half(), (r(70, 32) * 0.1).half()
+    want = ops.gated_linear_bwd(x, w, None, 'silu', dh)[0]
+    for bad in (float('inf'), float('nan')):
+        d2 = dh.clone()
+        d2[9, 3] = bad
+        got = ops.gated_linear_bwd(x, w, None, 'silu', d2)[0]
+        keep = torch.arange(70, device='cuda') != 9
+        assert not bool(got[9].isfinite().any())
+        # (the scale of the operands may be another power of two)
+        assert bool(((got[keep].double() - want[keep].double()).abs() <= 2.0 ** -10 * want[keep].double().abs() + 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+def test_gated_gradients_without_signal(dtype):
+    """A gradient of zeros, and one that underflows in every product."""
+    from focalformer3d_amd import ops
+    r = _randn(30)
+    x, w, b = r(40, 24).to(DT[dtype]), r(32, 24).to(DT[dtype]), r(32).to(DT[dtype])
+    for t in ops.gated_linear_bwd(x, w, b, 'silu', torch.zeros(40, 16, device='cuda', dtype=DT[dtype])):
+        assert not t.any()
+    for t in ops.gated_linear_bwd(torch.zeros_like(x), w, b * 0, 'silu', torch.ones(40, 16, device='cuda', dtype=DT[dtype])):
+        assert not t.any()
+
+
+def test_fp16_gradients_in_a_graph():
+    """Replays over gradients of very different sizes, each against the eager call."""
+    from focalformer3d_amd import ops
+    r = _randn(31)
+    x, w, b, dh = r(500, 64).half(), (r(96, 64) * 0.1).half(), r(96).half(), r(500, 48).half()
+    ops.gated_linear_bwd(x, w, b, 'gelu', dh)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.gated_linear_bwd(x, w, b, 'gelu', dh)
+    for f in (1.0, 2.0 ** -14, 1000.0, 0.0, 2.0 ** -6):
+        dh.copy_((r(500, 48) * f).half())
+        g.replay()
+        want = ops.gated_linear_bwd(x, w, b, 'gelu', dh)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want))
