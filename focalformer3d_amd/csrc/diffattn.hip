@@ -13,9 +13,11 @@
 // DMA; their transposed reads use ds_read_b64_tr_b16.
 //   forward  one pass with running maximum and sum per map; with few rows the keys are cut into slices that a second kernel joins
 //   dq       columns = queries, loops over keys;  dk / dv  columns = keys, loops over the rows.  No atomics: results do not depend
-//            on timing.  Scores are recomputed from q, k and the saved maximum and sum of each row: the exponent
+//            on timing.  Scores are recomputed from q, k and the saved reference and sum of each row: the exponent
 //            of a large probability is then near zero and exact, where score - log-sum-exp would lose a digit.
-// fp16: dS of a long row is far below fp16's normal range, so its columns carry a running power-of-two scale (Scaled).
+// fp16: dS of a long row is far below fp16's normal range, so its columns carry a running power-of-two scale (Scaled).  The forward pass's
+// weights are taken times 2^7 or 2^15 (FP16_UP): next to a weight of 1, one below 2^-14 would lose digits and one of 2^-25 vanish, and
+// tens of thousands of such keys carry a visible share of a row (10 * 2^-24 each: their sum was off by 4 %).
 //
 // Measured on one MI355X (large copy 4.77 TB/s, large bf16 product 1309 TFLOP/s):
 //   1 x 4096, 16 heads over 4 key heads of 64 columns per map, causal, bf16: forward 184 us (560 TFLOP/s of 2 products of 2 d and 4 d),
@@ -244,6 +246,8 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
   typedef FwdShape<T, D, ROWS> Shape;
   constexpr int NW = Shape::NW, NT = ROWS ? NW * 64 : 64, KT = Shape::KT, GR = 2 * D / Type<T>::PER16, BYTES = Shape::BYTES;
   constexpr int VT = 2 * D / 32, ST = D / 16, BLOCK_ROWS = ROWS ? NW * 32 : 32;
+  // log2 of what the largest weight of a row is taken as: with references up to 2^8 behind (ROWS), 2^15 is the most that any becomes
+  constexpr float FP16_UP = sizeof(T) == 2 && !__is_same(T, __bf16) ? (ROWS ? 7.f : 15.f) : 0.f;
   __shared__ __attribute__((aligned(16))) char lds[Shape::LDS];
   __shared__ float found[ROWS ? 1 : NW][4][64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, half = lane >> 5;
@@ -338,7 +342,7 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
 #pragma unroll
           for (int v = 0; v < VT; ++v) o[m][v] *= f;
         }
-        const float base = ref[m] == -INFINITY ? 0.f : ref[m];
+        const float base = ref[m] == -INFINITY ? 0.f : ref[m] - FP16_UP;
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
@@ -386,11 +390,11 @@ __global__ __launch_bounds__((FwdShape<T, D, ROWS>::NW * 64), (waves_of(D, sizeo
     if (!in || half) return;
     if (a.splits > 1) {
 #pragma unroll
-      for (int m = 0; m < 2; ++m) part[4 * a.d + 2 * m] = ref[m], part[4 * a.d + 2 * m + 1] = l[m];
+      for (int m = 0; m < 2; ++m) part[4 * a.d + 2 * m] = ref[m] - FP16_UP, part[4 * a.d + 2 * m + 1] = l[m];
     } else if (a.stat) {
 #pragma unroll
       for (int m = 0; m < 2; ++m) {
-        a.stat[((long long)bg * 4 + m) * a.R + row] = ref[m] == -INFINITY ? 0.f : ref[m];
+        a.stat[((long long)bg * 4 + m) * a.R + row] = ref[m] == -INFINITY ? 0.f : ref[m] - FP16_UP;
         a.stat[((long long)bg * 4 + 2 + m) * a.R + row] = inv[m];
       }
     }
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a) {
 
 // ---- backward -----------------------------------------------------------------------------------------------------------------
 // Before the products, in one launch: the first row_blocks blocks write the rows' values, the others the mask's words.
-// rowdata (B G, ROWDATA, Rp): maxima, D1 = <dO, out> + lam D2, D2 = <dO, O2>, 1 / sum 1, lam / sum 2; zeros behind R, whose
+// rowdata (B G, ROWDATA, Rp): references of the exponents, D1 = <dO, out> + lam D2, D2 = <dO, O2>, 1 / sum 1, lam / sum 2; zeros behind R, whose
 // probabilities are therefore 0.  16 lanes per row.
 // Words: 32 queries' mask bytes of a key in one word.  The dk / dv kernel then needs a word or two per lane and step, and can ask for them
 // a step ahead (16 byte loads behind the step's DMA, in order, would make it wait for that: 93 instead of 122 us at 4 x 720 x 720, 8 heads

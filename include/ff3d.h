@@ -778,7 +778,8 @@ int ff3d_gated_linear_bwd(const void* x, int64_t ldx, const void* weight, const 
  *   block its key (as 0 * NaN).
  *   fp32 operands are split into three bf16 planes (six products, as exact as fp32 ones): an infinite operand gives NaN.
  * ff3d_diff_attention_fwd: out (B, Nq, heads * 2 d) dense; for the backward pass also out2 (the same shape, fp32: the second map's
- *   softmax times v), stat (B, kv_heads, 4, Nq * heads / kv_heads) fp32 (row maxima in log2 units, 1 / row sums) and, in 16 bits,
+ *   softmax times v), stat (B, kv_heads, 4, Nq * heads / kv_heads) fp32 (what the exponents of a row are taken
+ *   less, in log2 units, and 1 / row sums) and, in 16 bits,
  *   out_rest (the shape and type of out: what its rounding left; NULL in fp32), else all NULL.
  * ff3d_diff_attention_bwd: dout with its own strides -> dq, (dk, dv) dense in their inputs' shapes, dlam (heads); dq, the pair and
  *   dlam may be NULL.  Deterministic.  workspace: ff3d_diff_attention_workspace_bytes(p, backward), 16-byte aligned scratch. */

@@ -1,4 +1,6 @@
-"""Calls of the operators in three types that their documentation allows: rows of unusual strides, gradients near the ends of fp16's range."""
+"""Calls of the operators in three types that their documentation allows: rows of unusual strides, gradients near the ends of fp16's range, long caches."""
+import math
+
 import pytest
 import torch
 
@@ -158,3 +160,24 @@ def test_fp16_gradients_in_a_graph():
         want = ops.gated_linear_bwd(x, w, b, 'gelu', dh)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+# ------------------------------------------------------------------------------------------------ long caches
+@pytest.mark.parametrize('Nq,H,Nk', [(1, 2, 120000), (600, 8, 40000), (4500, 8, 20000)])
+def test_fp16_weights_of_many_faint_keys(Nq, H, Nk):
+    """Tens of thousands of keys have 10.45 * 2^-24 of the largest weight each, between two of fp16's smallest numbers, and values that make their
+    sum count.  The three sizes are slices of the keys, blocks of 32 and blocks of 128 rows.  With weights kept to 2^-11 the output is off
+    by a rounding of the weights and its own, and all terms are of one sign: 3 * 2^-11 of it with the fp32 sums."""
+    from focalformer3d_amd import ops
+    d, top = 8, 1829 / 128                               # exp(-top) = 10.448 * 2^-24; top and all else is exact in fp16
+    q = torch.zeros(1, Nq, H * 2 * d, device='cuda', dtype=torch.half)
+    k, v = torch.zeros(1, Nk, 2 * d, device='cuda', dtype=torch.half), torch.full((1, Nk, 2 * d), 2.0, device='cuda', dtype=torch.half)
+    q[..., ::d], k[0, 0, ::d], v[0, 0] = 1.0, top, 0.25
+    lam = torch.zeros(H, device='cuda', dtype=torch.half)
+    faint = (Nk - 1) * math.exp(-top)
+    want = (0.25 + 2.0 * faint) / (1.0 + faint)
+    out = ops.diff_attention(q, k, v, lam, H, kv_heads=1, scale=1.0)
+    assert float((out.double() - want).abs().max()) <= 3 * 2.0 ** -11 * want
+    saved = ops.diff_attention_train_fwd(q, k, v, lam, H, kv_heads=1, scale=1.0)
+    assert torch.equal(saved[0], out)
+    assert float((saved[1].double() - want).abs().max()) <= 3 * 2.0 ** -11 * want
