@@ -98,14 +98,22 @@ __device__ __forceinline__ vec8<T> scaled_frag(const f32x16& c, int step, float 
 
 // What scaled_frag's rounding left, for a second product.  dS = P (dP - D) sums to nothing over the keys, so what remains of dS K is small
 // against its terms, and rounding those once gives dq 1.5 to 2.1 times, dk 1.4 to 2.3 times the error of rounding the result alone (8 or
-// 16 columns per map, or few keys).  With the second product it is 1.0 to 1.2 times.  dv is treated alike (1.4 times, and more where few
-// weights serve many columns).  It is left out (FINE false) where the products are
-// the bound and the sums are long: 64 columns and more than 2^24 pairs, 1.4 to 1.5 times.
+// 16 columns per map, or few keys).  With the second product it is 1.0 to 1.1 times.  dv is treated alike (1.4 times, and more where few
+// weights serve many columns).  It is left out (FINE false) where the products are the bound and the sums are long: see `fine` below.
 template <typename T>
 __device__ __forceinline__ vec8<T> rest_frag(const f32x16& c, int step, float mul, const vec8<T>& v) {
   vec8<T> r;
+  if constexpr (__is_same(T, __bf16)) {              // in pairs, without taking the halves of a register apart
+    const u32x4 h = __builtin_bit_cast(u32x4, v);
+    u32x4 w;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = from_f<T>(fmaf(c[8 * step + e], mul, -to_f(v[e])));
+    for (int e = 0; e < 4; ++e)
+      w[e] = pack_bf16(c[8 * step + 2 * e] - __uint_as_float(h[e] << 16), c[8 * step + 2 * e + 1] - __uint_as_float(h[e] & 0xffff0000u));
+    r = __builtin_bit_cast(vec8<T>, w);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r[e] = from_f<T>(fmaf(c[8 * step + e], mul, -to_f(v[e])));
+  }
   return r;
 }
 
@@ -663,6 +671,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
         sc[m].template see<QT>(top[m], acc[m]);
 #pragma unroll
         for (int st = 0; st < 2; ++st) {
+          if constexpr (FINE && D == 64) __builtin_amdgcn_sched_barrier(0);
           const vec8<T> ds = scaled_frag<T>(s[m], st, sc[m].mul());
           const Op<T> f = op<T>(ds);
           Op<T> x[QT];
@@ -674,6 +683,7 @@ __global__ __launch_bounds__(256, waves_of(D, sizeof(T), true)) void dq_kernel(A
             const Op<T> rest = op<T>(rest_frag<T>(s[m], st, sc[m].mul(), ds));
 #pragma unroll
             for (int t = 0; t < QT; ++t) acc[m][t] = mfma_step<T>(x[t], rest, acc[m][t]);
+            if constexpr (D == 64) __builtin_amdgcn_sched_barrier(0);
           }
         }
       }
@@ -862,63 +872,69 @@ __global__ __launch_bounds__((wide_v<T, D> ? 512 : 256), (wide_v<T, D> ? 2 : wav
 #pragma unroll
         for (int st = 0; st < G; ++st) dp = mfma_step<T>(op<T>(x[st]), y[st], dp);
       }
-      f32x16 w;
-      float top[3] = {0.f, 0.f, 0.f};
+      // With the keys in LDS 16 rows at a time: their weights and dS are used up before the next ones are formed, which keeps registers free
+      // (64 columns with the second products: 371 us in bf16 and 549 in fp16, 1192 and 1133 where all 32 rows' are formed first).  Elsewhere
+      // it costs 2 to 10 %.
+      constexpr int STEPS = WIDE ? 1 : 2;
 #pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const int rr = rb * 32 + 8 * y + 4 * half;
-        float r4[ROWDATA][4];
+      for (int s0 = 0; s0 < 2; s0 += STEPS) {
+        f32x16 w;                  // elements 8 s0 .. 8 (s0 + STEPS) - 1
+        float top[3] = {0.f, 0.f, 0.f};
 #pragma unroll
-        for (int n = 0; n < ROWDATA; ++n) *(u32x4*)r4[n] = *(const u32x4*)(rd + n * QR + rr);
+        for (int y = 2 * s0; y < 2 * (s0 + STEPS); ++y) {
+          const int rr = rb * 32 + 8 * y + 4 * half;
+          float r4[ROWDATA][4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const int e = 4 * y + x;
-          const float p1 = exp2_(fmaf(s[0][e], a.c, -r4[0][x])) * r4[4][x], p2 = exp2_(fmaf(s[1][e], a.c, -r4[1][x])) * r4[5][x];
-          w[e] = p1 - p2;
-          s[0][e] = p1 * (dp[e] - r4[2][x]);
-          s[1][e] = -p2 * (dp[e] - r4[3][x]);
-          top[0] = fmaxf(top[0], fabsf(w[e])), top[1] = fmaxf(top[1], fabsf(s[0][e])), top[2] = fmaxf(top[2], fabsf(s[1][e]));
+          for (int n = 0; n < ROWDATA; ++n) *(u32x4*)r4[n] = *(const u32x4*)(rd + n * QR + rr);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int e = 4 * y + x;
+            const float p1 = exp2_(fmaf(s[0][e], a.c, -r4[0][x])) * r4[4][x], p2 = exp2_(fmaf(s[1][e], a.c, -r4[1][x])) * r4[5][x];
+            w[e] = p1 - p2;
+            s[0][e] = p1 * (dp[e] - r4[2][x]);
+            s[1][e] = -p2 * (dp[e] - r4[3][x]);
+            top[0] = fmaxf(top[0], fabsf(w[e])), top[1] = fmaxf(top[1], fabsf(s[0][e])), top[2] = fmaxf(top[2], fabsf(s[1][e]));
+          }
+          if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
         }
-      }
-      sv.template see<VT>(top[0], dv);
+        sv.template see<VT>(top[0], dv);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const vec8<T> wv = scaled_frag<T>(w, st, sv.mul());
-        const Op<T> f = op<T>(wv);
-        vec8<T> x[VT];
+        for (int st = s0; st < s0 + STEPS; ++st) {
+          const vec8<T> wv = scaled_frag<T>(w, st, sv.mul());
+          const Op<T> f = op<T>(wv);
+          vec8<T> x[VT];
 #pragma unroll
-        for (int t = 0; t < VT; ++t) x[t] = col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, t * 32, lane);
-        if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
+          for (int t = 0; t < VT; ++t) x[t] = col_frag_acc<T, GR>(ot, rb * 32 + 16 * st, t * 32, lane);
 #pragma unroll
-        for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), f, dv[t]);
-        if constexpr (FINE) {
-          const Op<T> rest = op<T>(rest_frag<T>(w, st, sv.mul(), wv));
+          for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), f, dv[t]);
+          if constexpr (FINE) {
+            const Op<T> rest = op<T>(rest_frag<T>(w, st, sv.mul(), wv));
 #pragma unroll
-          for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), rest, dv[t]);
+            for (int t = 0; t < VT; ++t) dv[t] = mfma_step<T>(op<T>(x[t]), rest, dv[t]);
+          }
         }
-      }
-      sk[0].template see<QT>(top[1], dk[0]);
-      sk[1].template see<QT>(top[2], dk[1]);
+        sk[0].template see<QT>(top[1], dk[0]);
+        sk[1].template see<QT>(top[2], dk[1]);
 #pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        const vec8<T> ds[2] = {scaled_frag<T>(s[0], st, sk[0].mul()), scaled_frag<T>(s[1], st, sk[1].mul())};
-        const Op<T> f[2] = {op<T>(ds[0]), op<T>(ds[1])};
-        vec8<T> x[2][QT];          // d = 16: both maps share the columns of one tile
+        for (int st = s0; st < s0 + STEPS; ++st) {
+          const vec8<T> ds[2] = {scaled_frag<T>(s[0], st, sk[0].mul()), scaled_frag<T>(s[1], st, sk[1].mul())};
+          const Op<T> f[2] = {op<T>(ds[0]), op<T>(ds[1])};
+          vec8<T> x[2][QT];        // d = 16: both maps share the columns of one tile
 #pragma unroll
-        for (int m = 0; m < (D >= 32 ? 2 : 1); ++m)
+          for (int m = 0; m < (D >= 32 ? 2 : 1); ++m)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) x[m][t] = col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + t * 32, lane);
-        if constexpr (WIDE) __builtin_amdgcn_sched_barrier(0);
+            for (int t = 0; t < QT; ++t) x[m][t] = col_frag_acc<T, GR>(qt, rb * 32 + 16 * st, (D >= 32 ? m * D : 0) + t * 32, lane);
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+          for (int m = 0; m < 2; ++m)
 #pragma unroll
-          for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), f[m], dk[m][t]);
-        if constexpr (FINE) {
+            for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), f[m], dk[m][t]);
+          if constexpr (FINE) {
 #pragma unroll
-          for (int m = 0; m < 2; ++m) {
-            const Op<T> rest = op<T>(rest_frag<T>(s[m], st, sk[m].mul(), ds[m]));
+            for (int m = 0; m < 2; ++m) {
+              const Op<T> rest = op<T>(rest_frag<T>(s[m], st, sk[m].mul(), ds[m]));
 #pragma unroll
-            for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), rest, dk[m][t]);
+              for (int t = 0; t < QT; ++t) dk[m][t] = mfma_step<T>(op<T>(x[D >= 32 ? m : 0][t]), rest, dk[m][t]);
+            }
           }
         }
       }
@@ -1136,10 +1152,12 @@ int bwd(const ff3d_diff_attention_t& p, Args a, T* dlam, hipStream_t st) {
   const long long bg = (long long)a.B * a.G, rows = bg * a.Rp, qb = bg * cdiv(a.R, 128) * s.q, kb = bg * cdiv(a.Nk, 128) * s.k;
   if (rows > 0x7fffffffll * 16 || qb > 0x7fffffffll || kb > 0x7fffffffll) return FF3D_ERR_BAD_SHAPE;
   a.d2 = dlam && sizeof(T) == 2 ? a.rowdata + s.rowdata / 4 : nullptr;
-  // both kernels with and without the second product of rest_frag: 1 x 4096, 16 heads over 4 of 64, causal: +48 and +7 us (registers run
-  // out); 3 x 333 x 1777, 4 heads of 32: +6 and +3 us
   if (a.Nk == 1) a.scale = 0.f;    // the weight of a single key is 1 whatever its score: dq and dk are zero, not the rounding of dP - D
-  const bool fine = sizeof(T) == 2 && (D < 64 || (long long)a.B * a.H * a.Nq * a.Nk <= 1 << 24);
+  // The second products of rest_frag cost, at 1 x 4096, 16 heads over 4 of 64, causal: dk / dv 303 -> 371 us and dq 155 -> 192 in bf16,
+  // 415 -> 549 and 190 -> 232 in fp16; at 3 x 333 x 1777, 4 heads of 32: +6 and +3 us.  Without them the error is 1.4 to 1.45 times that of
+  // one rounding instead of 1.0 at 2200 keys or rows, more where a row attends few keys.  The rule goes by the lengths of the sums alone,
+  // over the keys and over the rows of a key head, so that a sequence's gradients have the same accuracy in every batch.
+  const bool fine = sizeof(T) == 2 && (D < 64 || (long long)a.R * a.Nk < 1 << 24 || a.R < 1024 || a.Nk < 1024);
   constexpr bool FINE = sizeof(T) == 2, COARSE = sizeof(T) == 2 && D < 64;     // COARSE: the variant where `fine` is false
   a.bits = (unsigned*)(a.rowdata + (s.rowdata + s.d2) / 4);
   a.bits_b = a.m_b ? (long long)cdiv(a.Nq, 32) * a.Nk : 0;

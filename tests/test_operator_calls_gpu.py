@@ -1,10 +1,10 @@
-"""Calls of the operators in three types that their documentation allows: rows of unusual strides, gradients near the ends of fp16's range, long caches."""
+"""Calls of the operators in three types that their documentation allows: rows of unusual strides, gradients near the ends of fp16's range, sequences in large batches, long caches."""
 import math
 
 import pytest
 import torch
 
-from tests.operators_util import assert_within, gated64
+from tests.operators_util import assert_within, blocked_pairs, diff_attention64, gated64
 
 pytestmark = pytest.mark.gpu
 DT = {'f32': torch.float32, 'bf16': torch.bfloat16, 'f16': torch.float16}
@@ -160,6 +160,26 @@ def test_fp16_gradients_in_a_graph():
         want = ops.gated_linear_bwd(x, w, b, 'gelu', dh)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+# ------------------------------------------------------------------------------------------------ batches
+@pytest.mark.parametrize('dtype', ['bf16', 'f16'])
+def test_accuracy_does_not_depend_on_the_batch(dtype):
+    """64 tokens of 16 heads of 64 columns, alone and as one of 512 sequences: the error of its gradients stays that of one rounding (1.3: with
+    the scatter of a norm of some thousand errors)."""
+    from focalformer3d_amd import ops
+    dt, B, N, H, d = DT[dtype], 512, 64, 16, 64
+    r = _randn(32, dt)
+    q, k, v, lam, dout = r(B, N, H * 2 * d), r(B, N, H * 2 * d), r(B, N, H * 2 * d), r(H).clamp(-1, 1), r(B, N, H * 2 * d)
+    n = 2
+    want = diff_attention64(q[:n], k[:n], v[:n], lam, H, H, blocked_pairs(n, N, N, None, None, False, 'cuda'), None, dout[:n])
+    for part in (n, B):
+        a = [t[:part] for t in (q, k, v)]
+        saved = ops.diff_attention_train_fwd(*a, lam, H)
+        got = ops.diff_attention_bwd(*a, lam, H, *saved, dout[:part])
+        for name, t, (exact, _) in zip(('dq', 'dk', 'dv'), got, want[1:]):
+            one = (exact.to(dt).double() - exact).norm()
+            assert float((t[:n].double() - exact).norm() / one) <= 1.3, (part, name)
 
 
 # ------------------------------------------------------------------------------------------------ long caches
