@@ -23,7 +23,7 @@ import weakref
 
 import torch
 import torch.nn.functional as F
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import ops
@@ -182,6 +182,12 @@ def _once(backward):
     return call
 
 
+def is_dual(*tensors):
+    """Does any of the tensors (None among them) carry a forward-mode tangent?  The operators below have no forward-mode derivative; routes
+    that would drop the tangent without a word take the autograd function instead, which refuses it."""
+    return forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 class DifferentialAttentionFunction(Function):
     """softmax(scale q1 k1^T) v - lam softmax(scale q2 k2^T) v per head (ops.diff_attention_train_fwd / _bwd)."""
 
@@ -200,8 +206,8 @@ class DifferentialAttentionFunction(Function):
 
 
 def differential_attention(q, k, v, lam, heads, kv_heads=None, mask=None, kv_lens=None, causal=False, scale=None):
-    """Differentiable ``ops.diff_attention`` (same arguments); without gradients to compute it is that operator."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam)):
+    """Differentiable ``ops.diff_attention`` (same arguments); without gradients to compute it is that operator.  Reverse mode only."""
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, lam))) or is_dual(q, k, v, lam):
         return DifferentialAttentionFunction.apply(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
     return ops.diff_attention(q, k, v, lam, heads, kv_heads, mask, kv_lens, causal, scale)
 
@@ -223,7 +229,8 @@ class GatedLinearFunction(Function):
 
 
 def gated_linear(x, weight, bias=None, act='silu'):
-    """Differentiable ``ops.gated_linear``: x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F) or None, one type of fp32, bf16, fp16."""
+    """Differentiable ``ops.gated_linear``: x (..., C), weight (2 F, C) = [Wg ; Wu], bias (2 F) or None, one type of fp32, bf16, fp16.
+    Reverse mode only."""
     return GatedLinearFunction.apply(x, weight, bias, act)
 
 

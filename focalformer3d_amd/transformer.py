@@ -373,7 +373,8 @@ class DifferentialAttention(nn.Module):
             self.__dict__.pop(name, None)
 
     def _project(self, x, linear):
-        if x.dtype != torch.float32 or torch.is_grad_enabled() or not x.is_contiguous() or x.numel() == 0:
+        from .autograd import is_dual
+        if x.dtype != torch.float32 or torch.is_grad_enabled() or not x.is_contiguous() or x.numel() == 0 or is_dual(x, linear.weight, linear.bias):
             return F.linear(x, linear.weight, linear.bias)
         return _lin(self, x, linear.weight, linear.bias)
 
@@ -730,9 +731,9 @@ class GatedFFN(nn.Module):
 
     def hidden(self, x):
         """Everything before the last Linear -> (hidden activation, last Linear)."""
+        from .autograd import gated_linear, is_dual
         w, b = self.in_proj.weight, self.in_proj.bias
-        if torch.is_grad_enabled():
-            from .autograd import gated_linear
+        if torch.is_grad_enabled() or is_dual(x, w, b):
             return gated_linear(x, w.to(x.dtype), b.to(x.dtype), self.act), self.out_proj       # (their types differ under autocast)
         if x.dtype == torch.float32 and getattr(self, 'gemm_dtype', torch.float32) == torch.bfloat16:
             # bf16 mode: operands on the bf16 matrix cores, fp32 rows out

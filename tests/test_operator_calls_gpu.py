@@ -1,4 +1,4 @@
-"""Calls of the operators in three types that their documentation allows: rows of unusual strides, gradients near the ends of fp16's range, sequences in large batches, long caches."""
+"""Calls of the operators in three types that their documentation allows: rows of unusual strides, forward-mode differentiation, gradients near the ends of fp16's range, sequences in large batches, long caches."""
 import math
 
 import pytest
@@ -68,6 +68,37 @@ def test_gated_linear_of_one_value(dtype):
     want = gated64(x.detach(), w.detach(), None, 'silu', torch.ones(1, 1, device='cuda', dtype=dt))
     for t, e in zip((h, x.grad, w.grad), want):
         assert_within(t, e)
+
+
+# ------------------------------------------------------------------------------------------------ forward mode
+def test_forward_mode_is_refused():
+    """Neither operator has a forward-mode derivative: a dual operand is an error, not a result without a tangent."""
+    import torch.autograd.forward_ad as fw
+    from focalformer3d_amd.autograd import differential_attention, gated_linear
+    from focalformer3d_amd.transformer import DifferentialAttention, GatedFFN
+    r = _randn(24)
+    q, k, v, lam = r(1, 6, 32), r(1, 7, 32), r(1, 7, 32), r(1)
+    x, w = r(5, 16), r(8, 16)
+    ffn, attention = GatedFFN(16, 32).cuda().eval(), DifferentialAttention(32, 2, batch_first=True).cuda().eval()
+    want, h, y = differential_attention(q, k, v, lam, 1), gated_linear(x, w), ffn(x)
+    with fw.dual_level():
+        for i in range(4):
+            args = [q, k, v, lam]
+            args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                    differential_attention(*args, 1)
+        dual = fw.make_dual(x, torch.ones_like(x))
+        for grad in (True, False):
+            with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                gated_linear(dual, w)
+            with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                ffn(dual)
+            with torch.set_grad_enabled(grad), pytest.raises((RuntimeError, NotImplementedError), match='forward'):
+                attention(fw.make_dual(q, torch.ones_like(q)))
+        assert torch.equal(differential_attention(q, k, v, lam, 1), want) and torch.equal(gated_linear(x, w), h) and torch.equal(ffn(x), y)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: differential_attention(t, k, v, lam, 1), (q,), (torch.ones_like(q),))
 
 
 # ------------------------------------------------------------------------------------------------ fp16's range
