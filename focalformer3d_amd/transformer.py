@@ -739,7 +739,8 @@ class GatedFFN(nn.Module):
             # bf16 mode: operands on the bf16 matrix cores, fp32 rows out
             w16, b16 = _cached(self, '_bf16_w', w, b, lambda: (w.detach().to(torch.bfloat16), b.detach().to(torch.bfloat16)))
             return ops.gated_linear(x.to(torch.bfloat16), w16, b16, self.act).float(), self.out_proj
-        return ops.gated_linear(x, w.detach(), b.detach(), self.act), self.out_proj
+        # (fp32 rows stay fp32 here, as in FFN; 16-bit ones come from projections under autocast)
+        return ops.gated_linear(x, w.detach().to(x.dtype), b.detach().to(x.dtype), self.act), self.out_proj
 
     def delta(self, x):
         y, last = self.hidden(x)

@@ -1,4 +1,5 @@
-"""Calls of the operators in three types that their documentation allows: rows of unusual strides, forward-mode differentiation, gradients near the ends of fp16's range, sequences in large batches, long caches."""
+"""Calls of the operators in three types that their documentation allows: rows of unusual strides, forward-mode differentiation, modules with 16-bit
+activations, gradients near the ends of fp16's range, sequences in large batches, long caches."""
 import math
 
 import pytest
@@ -99,6 +100,30 @@ def test_forward_mode_is_refused():
         assert torch.equal(differential_attention(q, k, v, lam, 1), want) and torch.equal(gated_linear(x, w), h) and torch.equal(ffn(x), y)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: differential_attention(t, k, v, lam, 1), (q,), (torch.ones_like(q),))
+
+
+# ------------------------------------------------------------------------------------------------ modules in 16 bits
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float16])
+def test_gated_ffn_evaluates_what_it_trains_on(dtype):
+    """16-bit activations beside fp32 parameters under autocast: the inference route takes what the training route takes.  Four roundings of
+    the type (input, hidden row, weights, result)."""
+    from focalformer3d_amd.transformer import GatedFFN
+    torch.manual_seed(25)
+    m = GatedFFN(64, 96).cuda()
+    x = torch.randn(2, 20, 64, device='cuda')
+    P = {n: p.detach().double() for n, p in m.named_parameters()}
+
+    def plain(x):
+        g, u = torch.nn.functional.linear(x, P['in_proj.weight'], P['in_proj.bias']).chunk(2, -1)
+        return x + torch.nn.functional.linear(torch.nn.functional.silu(g) * u, P['out_proj.weight'], P['out_proj.bias'])
+    for inp in (x.to(dtype), x):
+        want = plain(inp.double())
+        with torch.autocast('cuda', dtype):
+            y = m.train()(inp)
+            with torch.no_grad():
+                for z in (m.train()(inp), m.eval()(inp)):
+                    assert float((z.double() - want).norm() / want.norm()) <= 4 * torch.finfo(dtype).eps / 2
+        assert float((y.double() - want).norm() / want.norm()) <= 4 * torch.finfo(dtype).eps / 2
 
 
 # ------------------------------------------------------------------------------------------------ fp16's range
