@@ -734,7 +734,9 @@ class GatedFFN(nn.Module):
         from .autograd import gated_linear, is_dual
         w, b = self.in_proj.weight, self.in_proj.bias
         if torch.is_grad_enabled() or is_dual(x, w, b):
-            return gated_linear(x, w.to(x.dtype), b.to(x.dtype), self.act), self.out_proj       # (their types differ under autocast)
+            if x.is_cuda and torch.is_autocast_enabled('cuda'):                                  # as the Linear layers around it
+                x = x.to(torch.get_autocast_dtype('cuda'))
+            return gated_linear(x, w.to(x.dtype), b.to(x.dtype), self.act), self.out_proj
         if x.dtype == torch.float32 and getattr(self, 'gemm_dtype', torch.float32) == torch.bfloat16:
             # bf16 mode: operands on the bf16 matrix cores, fp32 rows out
             w16, b16 = _cached(self, '_bf16_w', w, b, lambda: (w.detach().to(torch.bfloat16), b.detach().to(torch.bfloat16)))

@@ -126,6 +126,25 @@ def test_gated_ffn_evaluates_what_it_trains_on(dtype):
         assert float((y.double() - want).norm() / want.norm()) <= 4 * torch.finfo(dtype).eps / 2
 
 
+def test_gated_ffn_under_autocast_runs_in_the_autocast_type():
+    """fp32 activations, as a LayerNorm under autocast hands them on, are cast as the Linear layers beside the operator cast theirs."""
+    from focalformer3d_amd.transformer import GatedFFN
+    torch.manual_seed(26)
+    m = GatedFFN(64, 96).cuda().train()
+    x = torch.randn(30, 64, device='cuda', requires_grad=True)
+    h32 = m.hidden(x)[0]
+    for dtype in (torch.bfloat16, torch.float16):
+        with torch.autocast('cuda', dtype):
+            h = m.hidden(x)[0]
+            y = m(x)
+        assert h.dtype == dtype and h32.dtype == torch.float32
+        assert float((h.double() - h32.double()).norm() / h32.double().norm()) <= 4 * torch.finfo(dtype).eps / 2
+        grads = torch.autograd.grad(y.float().square().sum(), [x, *m.parameters()])
+        assert all(g.dtype == torch.float32 and bool(g.isfinite().all()) for g in grads)
+        with torch.autocast('cuda', dtype), torch.autocast('cuda', enabled=False):
+            assert m.hidden(x)[0].dtype == torch.float32
+
+
 # ------------------------------------------------------------------------------------------------ fp16's range
 def _gated_gradients(x, w, b, act, dh):
     from focalformer3d_amd import ops
