@@ -795,7 +795,10 @@ int fwd(const T* x, long long ldx, const T* w, const T* bias, T* h, int M, int C
   GemmArgs a = gated_args<T>(x, ldx, w, ldw, bias, M, C, pl.Cp, F, act);
   a.out = h, a.ldo = F, a.vec_out = vec_ok(h, F, sizeof(T));
   const long long small = (long long)cdiv(M, 32) * cdiv(F, 32);
-  if (M <= 32) {                   // 600 rows of 256 -> 1024 in fp32: 19 us like this, 14 us in tiles
+  // Few rows / tiles, in us.  1024 -> 2736: bf16 7.9 / 9.2 at 4 rows, 9.0 / 9.3 at 8, 9.9 / 9.3 at 12, 15.9 / 9.5 at 33, fp32 14 / 37 at 4,
+  // 25 / 38 at 64, 36 / 38 at 96, 39 / 38 at 128.  256 -> 1024: bf16 4.9 / 4.9 at 8, 5.4 / 5.0 at 12, fp32 6.7 / 12.2 at 4, 10.3 / 12.7 at 96,
+  // 19.5 / 13.3 at 600.  The same at 512 -> 512 and 1536 -> 4096, and in fp16.
+  if (M <= (sizeof(T) == 2 ? 8 : 96)) {
     a.nt = cdiv(F, 32);
     if (pl.Cp * (int)sizeof(T) >= 2048) gated_rows_kernel<T, 8><<<(unsigned)small, 512, 0, st>>>(a);
     else gated_rows_kernel<T, 4><<<(unsigned)small, 256, 0, st>>>(a);

@@ -98,9 +98,9 @@ def test_accuracy_of_the_gated_projection(dtype, act):
         assert ratio(t, want[0], dt) <= most, name
 
 
-# the few-row kernel with eight waves: rows of 2048 bytes and more
+# the few-row kernel with eight waves (rows of 2048 bytes and more), up to its last number of rows and past it
 @pytest.mark.parametrize('dtype', ['f32', 'bf16', 'f16'])
-@pytest.mark.parametrize('M', [1, 4, 31, 32])
+@pytest.mark.parametrize('M', [1, 4, 8, 9, 31, 32, 33, 70, 96, 97])
 @pytest.mark.parametrize('C,F,bias', [(1024, 333, True), (1032, 64, False), (1347, 40, True)])
 def test_few_rows_of_wide_blocks(dtype, M, C, F, bias):
     from focalformer3d_amd import ops
