@@ -1806,21 +1806,13 @@ def _new_like(t, zero=False):
     return (torch.zeros if zero else torch.empty)(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _whole_rows(t, apart=float('inf')):
-    """t (M, n) -> (itself, or a view or copy of it, with dense rows fewer than ``apart`` elements apart; its row stride).  The stride of a
-    single row says nothing (``contiguous()`` keeps it, whatever it is) and is replaced."""
-    (M, n), (row, col) = t.shape, t.stride()
-    if col == 1 and n <= row < apart:
-        return t, row
+def _whole_rows(t):
+    """t (M, n) with rows that a kernel cannot take -> (a view or copy of it with dense rows, their stride).  The stride of a single row says
+    nothing (``contiguous()`` keeps it, whatever it is) and is replaced."""
+    (M, n), col = t.shape, t.stride(1)
     if M == 1 and (col == 1 or n == 1):
         return t.as_strided((1, n), (n, 1)), n
     return t.clone(memory_format=torch.contiguous_format), n
-
-
-def _gated_pack(x2, row, weight, C_, code):
-    """Which operands have to be packed into rows of whole aligned granules: bit 0 x, bit 1 the weight."""
-    per = 4 if code == 0 else 8
-    return 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
 
 
 def _gated_args(x, weight, bias, act):
@@ -1846,9 +1838,13 @@ def _gated_args(x, weight, bias, act):
     x2 = x if x.dim() == 2 else x.reshape(-1, C_)
     if x2.shape[0] >= 0x7fffff00:
         raise RuntimeError(f'gated_linear: {x2.shape[0]} rows: fewer than {0x7fffff00} in a call')
-    x2, row = _whole_rows(x2, 1 << 20)                     # (the kernels' offsets inside a tile are 31 bits)
+    row, col = x2.stride()
+    if col != 1 or row < C_ or row >= 1 << 20:             # (the kernels' offsets inside a tile are 31 bits)
+        x2, row = _whole_rows(x2)
     weight = weight.contiguous()
-    return x2, weight, bias, F2 // 2, C_, _gated_pack(x2, row, weight, C_, code), code, acode
+    per = 4 if code == 0 else 8
+    pack = 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
+    return x2, weight, bias, F2 // 2, C_, pack, code, acode
 
 
 def _gated_fwd(x, args):
@@ -1896,9 +1892,13 @@ def _gated_again(keep, dims):
     """The checked operands that autograd kept (addresses and strides are asked for again: a hook may have moved them)."""
     x2, weight, bias = keep
     F_, C_, _, code, acode, _ = dims
-    x2, row = _whole_rows(x2, 1 << 20)
+    row, col = x2.stride()
+    if col != 1 or row < C_ or row >= 1 << 20:
+        x2, row = _whole_rows(x2)
     weight, bias = weight.contiguous(), None if bias is None else bias.contiguous()
-    return x2, weight, bias, F_, C_, _gated_pack(x2, row, weight, C_, code), code, acode
+    per = 4 if code == 0 else 8
+    pack = 3 if C_ % per else (1 if row % per or x2.data_ptr() % 16 else 0) | (2 if weight.data_ptr() % 16 else 0)
+    return x2, weight, bias, F_, C_, pack, code, acode
 
 
 def _gated_grads(args, shape, dh, want):
@@ -1910,7 +1910,10 @@ def _gated_grads(args, shape, dh, want):
     dw = _new_like(weight, M == 0) if want[1] else None
     db = _new_like(bias, M == 0) if want_b else None
     if M > 0 and (want[0] or want[1] or want_b):
-        dh2, dh_row = _whole_rows(dh.reshape(M, F_))
+        dh2 = dh.reshape(M, F_)
+        dh_row, col = dh2.stride()
+        if col != 1 or dh_row < F_:
+            dh2, dh_row = _whole_rows(dh2)
         lib = _lib.load()
         ws = torch.empty(lib.ff3d_gated_linear_workspace_bytes(M, C_, F_, code, pack, 1), dtype=torch.uint8, device=x2.device)
         _lib.check(lib.ff3d_gated_linear_bwd(_ptr(x2), x2.stride(0), _ptr(weight), _ptr(bias), _ptr(dh2), dh_row, _ptr(dx), _ptr(dw), _ptr(db),
