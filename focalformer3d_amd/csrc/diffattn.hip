@@ -9,7 +9,8 @@
 // serve all of them, a single new token fills r columns of a tile, and the gradients of shared heads are summed where they arise.
 // Score tiles are 32 x 32 with the long-lived side as columns (queries in the forward and dq kernels, keys in the dk / dv kernel):
 // a lane owns half a column of scores, so the softmax statistics of a row are one value per lane, and the tile, rounded, is already
-// the operand of the next product (ff3d_mma.h).  Keys and values (queries and dO) pass through LDS once per block in two stages, by
+// the operand of the next product (ff3d_mma.h): the weights are rounded once before P v, which makes the error of out 1.06 to 1.23 times that
+// of rounding it alone.  Keys and values (queries and dO) pass through LDS once per block in two stages, by
 // DMA; their transposed reads use ds_read_b64_tr_b16.
 //   forward  one pass with running maximum and sum per map; with few rows the keys are cut into slices that a second kernel joins
 //   dq       columns = queries, loops over keys;  dk / dv  columns = keys, loops over the rows.  No atomics: results do not depend
@@ -21,9 +22,10 @@
 //
 // Measured on one MI355X (large copy 4.77 TB/s, large bf16 product 1309 TFLOP/s):
 //   1 x 4096, 16 heads over 4 key heads of 64 columns per map, causal, bf16: forward 184 us (560 TFLOP/s of 2 products of 2 d and 4 d),
-//     dq 154, dk / dv 308, what comes before and behind them 31.  Bound by the turn of matrix and vector work (two exponentials a pair) in
-//     the two waves of a SIMD that the accumulators leave room for.
-//   4 x 720, 8 heads of 16, fp32, masked: 44, 56, 72 and 13 us.  Bound by splitting the fp32 operands and by the exponentials.
+//     dq 154, dk / dv 306 .. 312, what comes before and behind them 31.  Bound by the turn of matrix and vector work (two exponentials a pair) in
+//     the two waves of a SIMD that the accumulators leave room for (matrix unit 34, 42 and 24 % busy), and in dk / dv by 76 bytes a lane of
+//     registers that spill.  fp16: forward 166, backward 590 where bf16 takes 445 (the scales of its columns).
+//   4 x 720, 8 heads of 16, fp32, masked: 45, 57, 74 and 12 us.  Bound by splitting the fp32 operands and by the exponentials.
 //   8 tokens over 16384 keys, 16 heads over 4 of 64, bf16: 47 us for keys and values at 4.3 TB/s, 5.5 for joining the slices.
 #include "ff3d_mma.h"
 

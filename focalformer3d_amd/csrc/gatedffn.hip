@@ -6,14 +6,14 @@
 //   gated      both projections in one block: a wave owns the same 32 columns of g and of u, so the activation and the product
 //              happen on its accumulators and g, u never reach memory
 //   gated_bwd  the same products again with dh in the epilogue -> d (rounded to the type once, as the operand of the two products
-//              below has to be) and the column sums of the unrounded d.  g and u are recomputed instead of saved: 2 M C F more
-//              multiply-adds, against 2 M F values written and read again and against rounding them, which alone would take the
-//              gradients from 1.4 to 1.7 times the error of a single rounding.  In fp16 d is scaled first (RANGED below)
+//              below has to be: dx and dW are off by 1.41 times the error of a single rounding) and the column sums of the unrounded
+//              d.  g and u are recomputed instead of saved: 2 M C F more multiply-adds, against 2 M F values written and read again
+//              and against rounding them, which alone would make that 1.7 times.  In fp16 d is scaled first (RANGED below)
 //   plain      dx and, with its row sum cut into slices that a second kernel adds in order, dW: results do not depend on timing
 // A block computes C^T tiles: the n side (features of W, columns of the output) is the row operand, so a lane holds 4 consecutive
 // columns of one output row and stores them together.
 // Measured on one MI355X (a large library product: 1309 TFLOP/s in bf16, 154 in fp32): 16384 x 1024 -> 2736 in bf16, 184 GFLOP each: forward
-// 196 .. 211 us, d 271, dx 181, dW 286 + 10 (the matrix unit is the bound; d adds reading dh and writing d, dW's 88 tiles in two slices fill
+// 194 .. 214 us, d 270, dx 181, dW 287 + 10 (the matrix unit is the bound; d adds reading dh and writing d, dW's 88 tiles in two slices fill
 // 69 % of the chip); 2880 x 256 -> 1024 in fp32, 3 GFLOP each: 31, 39, 33, 35 us and 10 for the sums of slices (bound by splitting operands
 // and by latency); 4 x 1024 -> 2736 in bf16: 8 us, the weight at 1.4 TB/s.
 #include <type_traits>
