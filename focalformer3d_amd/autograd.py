@@ -173,12 +173,15 @@ class MaskedSelfAttentionFunction(Function):
 
 
 def _once(backward):
-    """``once_differentiable`` without its cost where no graph of the gradients is built."""
+    """``once_differentiable`` without its cost where no graph of the gradients is built, and without its gap: it lets a second derivative
+    pass as zero where no incoming gradient requires one (``out.sum()``), although the saved operands do.  Here it is refused there too."""
     checked = once_differentiable(backward)
 
     @functools.wraps(backward)
     def call(ctx, *grads):
-        return checked(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        return checked(ctx, *(None if g is None else g.detach().requires_grad_(True) for g in grads))
     return call
 
 

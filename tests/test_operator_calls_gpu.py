@@ -1,4 +1,4 @@
-"""Calls of the operators in three types that their documentation allows: rows of unusual strides, forward-mode differentiation, modules with 16-bit
+"""Calls of the operators in three types that their documentation allows: rows of unusual strides, forward-mode differentiation, second derivatives, modules with 16-bit
 activations, gradients near the ends of fp16's range, sequences in large batches, long caches."""
 import math
 
@@ -100,6 +100,21 @@ def test_forward_mode_is_refused():
         assert torch.equal(differential_attention(q, k, v, lam, 1), want) and torch.equal(gated_linear(x, w), h) and torch.equal(ffn(x), y)
     with pytest.raises(RuntimeError):
         torch.func.jvp(lambda t: differential_attention(t, k, v, lam, 1), (q,), (torch.ones_like(q),))
+
+
+# ------------------------------------------------------------------------------------------------ second derivatives
+def test_second_derivatives_are_refused():
+    """A graph of the gradients can be asked for; differentiating it again is an error, also where the incoming gradient is a constant."""
+    from focalformer3d_amd.autograd import differential_attention, gated_linear
+    r = _randn(33)
+    q, lam, w = r(1, 6, 64).requires_grad_(True), r(2).requires_grad_(True), r(8, 64).requires_grad_(True)
+    for y, leaf in ((differential_attention(q, q, q, lam, 2), q), (differential_attention(q.detach(), q.detach(), q.detach(), lam, 2), lam),
+                    (gated_linear(q, w), w)):
+        want, = torch.autograd.grad(y.sum(), leaf, retain_graph=True)
+        got, = torch.autograd.grad(y.sum(), leaf, create_graph=True)
+        assert torch.equal(got, want) and got.requires_grad
+        with pytest.raises(RuntimeError, match='twice'):
+            (y.sum() + got.square().sum()).backward()
 
 
 # ------------------------------------------------------------------------------------------------ modules in 16 bits
