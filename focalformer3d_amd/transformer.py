@@ -734,7 +734,7 @@ class GatedFFN(nn.Module):
         from .autograd import gated_linear, is_dual
         w, b = self.in_proj.weight, self.in_proj.bias
         if torch.is_grad_enabled() or is_dual(x, w, b):
-            if x.is_cuda and torch.is_autocast_enabled('cuda'):                                  # as the Linear layers around it
+            if x.is_cuda and x.dtype != torch.float64 and torch.is_autocast_enabled('cuda'):     # as the Linear layers around it
                 x = x.to(torch.get_autocast_dtype('cuda'))
             return gated_linear(x, w.to(x.dtype), b.to(x.dtype), self.act), self.out_proj
         if x.dtype == torch.float32 and getattr(self, 'gemm_dtype', torch.float32) == torch.bfloat16:

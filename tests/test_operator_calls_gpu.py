@@ -158,6 +158,8 @@ def test_gated_ffn_under_autocast_runs_in_the_autocast_type():
         assert all(g.dtype == torch.float32 and bool(g.isfinite().all()) for g in grads)
         with torch.autocast('cuda', dtype), torch.autocast('cuda', enabled=False):
             assert m.hidden(x)[0].dtype == torch.float32
+        with torch.autocast('cuda', dtype), pytest.raises(RuntimeError, match='float64'):      # which autocast leaves as it is
+            m.hidden(x.double())
 
 
 # ------------------------------------------------------------------------------------------------ fp16's range
