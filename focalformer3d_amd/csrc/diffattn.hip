@@ -9,7 +9,7 @@
 // serve all of them, a single new token fills r columns of a tile, and the gradients of shared heads are summed where they arise.
 // Score tiles are 32 x 32 with the long-lived side as columns (queries in the forward and dq kernels, keys in the dk / dv kernel):
 // a lane owns half a column of scores, so the softmax statistics of a row are one value per lane, and the tile, rounded, is already
-// the operand of the next product (ff3d_mma.h): the weights are rounded once before P v, which makes the error of out 1.06 to 1.23 times that
+// the operand of the next product (ff3d_mma.h): the weights are rounded once before P v, which makes the error of out 1.06 to 1.45 times that
 // of rounding it alone.  Keys and values (queries and dO) pass through LDS once per block in two stages, by
 // DMA; their transposed reads use ds_read_b64_tr_b16.
 //   forward  one pass with running maximum and sum per map; with few rows the keys are cut into slices that a second kernel joins
